@@ -301,6 +301,38 @@ int q40_attn_paged(const void* page_tbl, int idx_bytes, int64_t tbl_stride, cons
                    const void* q, const void* kpool, const void* vpool, void* o, int P, int B,
                    int Lmax, int H, int Hkv, int D, int page_size, void* stream);
 
+/* Paged attention over fp16 pages or pages held in 8 bits, with all keys visible or a window of them: sequence b's one query
+ * (at q + b*q_stride elements, position seq_lens[b] - 1) attends its last `window` keys (0: all) and its first `sinks`.  cache_type
+ * says what the pools [Hkv, P, D] hold: Q40_CACHE_F16, or signed 8-bit codes or e4m3 codes, element = code * scale with one fp32 scale >= 0 for
+ * each page and kv head, k_scale / v_scale [Hkv, P / page_size] (P a multiple of page_size; NULL for fp16).  Table, lengths (NULL: Lmax each;
+ * at most Lmax <= 2^30 count) and the order of tokens as in q40_attn_paged.  A sequence without keys gets zeros.  Keys that are not visible are not
+ * read.  An element whose scale is NaN is NaN.  Results do not depend on Lmax.  Workspace: *_workspace_bytes bytes, 16-byte aligned, no
+ * initialisation (0 bytes: may be NULL); calls that may overlap need one each.  No counterpart in the reference. */
+#define Q40_CACHE_F16 0
+#define Q40_CACHE_I8 1
+#define Q40_CACHE_E4M3 2
+size_t q40_attn_pages_workspace_bytes(int B, int H, int Hkv, int Lmax, int window, int sinks);
+int q40_attn_pages(const void* page_tbl, int idx_bytes, int64_t tbl_stride, const int32_t* seq_lens, const void* q, int64_t q_stride,
+                   const void* kpool, const void* vpool, const float* k_scale, const float* v_scale, int cache_type, void* o, int64_t P,
+                   int B, int Lmax, int H, int Hkv, int D, int page_size, int window, int sinks, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* Appends new tokens' keys and values (rows of k_stride / v_stride elements, Hkv heads side by side) to pages as q40_attn_pages
+ * reads them.  offsets NULL: T == B, row b is sequence b's one new token, at position pos[b].  Else rows offsets[b] .. offsets[b+1] - 1
+ * (int32 [B + 1], ascending) are sequence b's, at positions pos[b], pos[b] + 1, ...  With tables [n_pos, D/2] keys are rotated to their
+ * positions (from n_pos on: as n_pos - 1), and queries q [T, H*D], if given, are written rotated to q_out [T, H*D] (row stride H*D); a
+ * rotated value is computed in fp32 and rounded once.  Rows of no sequence, positions below 0 or behind the sequence's tbl_width
+ * pages, page ids outside of the pool: nothing is written for them (zeros to q_out, for rows of no sequence and positions below 0).
+ * 8-bit pools: a page's scale is max(scale so far, largest magnitude of its new rows / 127 or 448), where a page whose first slot is written has
+ * none so far; if it grows, the page's rows in front of the new ones are coded anew.  A value that is not finite makes the scale NaN until
+ * the page is begun anew.  Tokens of one call that go to one slot, in 8 bits also sequences that append to one page, leave those slots (that
+ * page and its scale) undefined.  16-byte aligned, strides multiples of 8.  No counterpart in the reference beyond the append of
+ * hf_model_q40_kv_shared.py:365-371 to its own cache. */
+int q40_page_append(const void* page_tbl, int idx_bytes, int64_t tbl_stride, int tbl_width, const int32_t* pos, const int32_t* offsets,
+                    const void* q, int64_t q_stride, void* q_out, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                    const void* cos_tbl, const void* sin_tbl, int n_pos, void* kpool, void* vpool, float* k_scale, float* v_scale,
+                    int cache_type, int64_t P, int B, int T, int H, int Hkv, int D, int page_size, void* stream);
+
 /* Bytes of fp32 scratch q40_attn_shared_prefix needs (partial max / sum / output of each
  * prefix split).  No initialisation required. */
 size_t q40_attn_shared_prefix_workspace_bytes(int B, int H, int D, int prefix_len);
@@ -438,6 +470,11 @@ int q40_silu_mul(const void* a, const void* b, void* y, int64_t n, void* stream)
  * scaled_dot_product_attention of hf_model_q40_kv_shared.py:375-405 (mask built at :499-504). */
 int q40_attn_causal(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* o,
                     int64_t ldo, int S, int H, int Hkv, int D, void* stream);
+
+/* q40_attn_causal for a prompt's positions offset .. offset + S - 1, whose keys and values are rows 0 .. offset + S - 1 of k and v, with a
+ * window: the query at position p attends the keys j <= p with p - j < window or j < sinks.  offset + S <= 2^30. */
+int q40_attn_causal_window(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* o, int64_t ldo,
+                           int S, int H, int Hkv, int D, int offset, int window, int sinks, void* stream);
 
 /* The layers of a prompt pass, enqueued by one call: per layer q40_rmsnorm (adding the previous layer's output), q40_gemm_tiled_tc_multi
  * for wq, wk and wv (keys and values into the prompt cache), q40_rope_qk, q40_attn_causal, wo, q40_rmsnorm, q40_gemm_tiled_tc_ws with the SiLU

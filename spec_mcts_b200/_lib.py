@@ -47,6 +47,8 @@ SIGNATURES = {
                                c_void_p, c_void_p]),
     "q40_gemm_kn_tc_multi": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                      c_int, c_int, c_void_p, c_int, c_void_p]),
+    "q40_attn_causal_window": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64] + [c_int] * 7 +
+                               [c_void_p]),
     "q40_attn_causal": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int,
                                 c_int, c_int, c_int, c_void_p]),
     "q40_tp_layout": (c_int, [c_int, c_int, c_int, c_void_p]),
@@ -97,6 +99,11 @@ SIGNATURES = {
                                 c_int, c_void_p]),
     "q40_attn_paged": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "q40_attn_pages_workspace_bytes": (c_size_t, [c_int] * 6),
+    "q40_attn_pages": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64] + [c_void_p] * 4 + [c_int, c_void_p, c_int64] +
+                       [c_int] * 8 + [c_void_p, c_size_t, c_void_p]),
+    "q40_page_append": (c_int, [c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
+                                c_int64, c_void_p, c_void_p, c_int] + [c_void_p] * 4 + [c_int, c_int64] + [c_int] * 6 + [c_void_p]),
     "q40_attn_shared_prefix_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "q40_attn_shared_prefix": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int, c_int64,
                                        c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,

@@ -88,9 +88,11 @@ struct WarpRows {
   }
 
   // KEYS keys of a tile: S = Q K^T, online softmax, O += P V.  With MASK, key i of the tile counts for row g below n0 and for row g + 8
-  // below n1.  A row all of whose scores so far are -inf keeps its sum and outputs at zero.
-  template <bool MASK, int KEYS = TILE_KEYS>
-  __device__ __forceinline__ void step(uint32_t kt, uint32_t vt, float scale_log2, int n0, int n1, int lane) {
+  // below n1.  With WINDOW, moreover, it counts from key from0 or from1 on, or below `first`.  A row all of whose scores so far are -inf
+  // keeps its sum and outputs at zero.
+  template <bool MASK, int KEYS = TILE_KEYS, bool WINDOW = false>
+  __device__ __forceinline__ void step(uint32_t kt, uint32_t vt, float scale_log2, int n0, int n1, int lane, int from0 = 0, int from1 = 0,
+                                       int first = 0) {
     const int t = lane & 3;
     constexpr int NT = KEYS / 8;
     float s[NT][4];
@@ -118,6 +120,7 @@ struct WarpRows {
       for (int j = 0; j < 4; ++j) {
         s[nt][j] *= scale_log2;
         if (MASK && nt * 8 + 2 * t + (j & 1) >= ((j >> 1) ? n1 : n0)) s[nt][j] = -CUDART_INF_F;
+        if (WINDOW && nt * 8 + 2 * t + (j & 1) < ((j >> 1) ? from1 : from0) && nt * 8 + 2 * t + (j & 1) >= first) s[nt][j] = -CUDART_INF_F;
         mx[j >> 1] = fmaxf(mx[j >> 1], s[nt][j]);
       }
     float corr[2];

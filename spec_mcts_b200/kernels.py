@@ -41,7 +41,7 @@ GROUP_SIZE = 64
 __all__ = [
     "quantize_q40", "dequantize_q40", "triton_deq_int40", "triton_q_int40", "triton_q_int40_sliced",
     "quantize_q40_rows", "matmul", "matmul_q40", "linear_q40", "flash_attn", "page_flash_attn",
-    "triton_attn", "chunk_attn", "shared_prefix_attn", "matmul_split_k", "rmsnorm", "rope_", "silu_mul",
+    "page_flash_attn_q8", "page_append", "causal_attn", "triton_attn", "chunk_attn", "shared_prefix_attn", "matmul_split_k", "rmsnorm", "rope_", "silu_mul",
     "gemv_fused", "gemv_stream", "stream_status", "embed_rows", "tc_error_flag", "relayout_tiled", "relayout_cache_config",
     "Q40Error",
 ]
@@ -572,17 +572,38 @@ def gemv_fused(mode: int, a: torch.Tensor, weights, *, norm_w=None, ss_in=None, 
     return outs
 
 
-def causal_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+def causal_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional[torch.Tensor] = None, *,
+                window: Optional[int] = None, sinks: int = 0, offset: int = 0) -> torch.Tensor:
     """Causal attention of a prompt: q [S, H, 128], k / v [S, Hkv, 128] (position-major, last two dims
-    contiguous) -> [S, H, 128]; position i attends positions 0..i (q40_attn_causal in include/q40b200.h)."""
-    dev = _need_cuda(q, k, v)
+    contiguous) -> [S, H, 128]; position i attends positions 0..i (q40_attn_causal in include/q40b200.h).
+
+    With `window` a position attends its last `window` positions, itself among them, and the first `sinks`.  With `offset` the queries
+    are positions offset .. offset + S - 1 of a longer prompt, whose first offset + S keys and values k and v hold
+    (q40_attn_causal_window)."""
+    dev = _need_cuda(q, k, v, out)
     S, H, D = q.shape
     Hkv = k.shape[1]
     for t in (q, k, v):
         if t.dtype != torch.float16 or t.stride(2) != 1 or t.stride(1) != D:
             raise Q40Error("causal_attn: fp16 tensors [S, heads, 128] with contiguous heads expected")
+    windowed = window is not None or sinks != 0 or offset != 0
+    if windowed:
+        if offset < 0 or sinks < 0 or (window is not None and window < 1):
+            raise Q40Error(f"causal_attn: window {window} below 1, sinks {sinks} or offset {offset} below 0")
+        if min(k.shape[0], v.shape[0]) < offset + S or v.shape[1:] != k.shape[1:] or k.shape[2] != D:
+            raise Q40Error(f"causal_attn: keys {tuple(k.shape)} and values {tuple(v.shape)} do not hold {offset + S} positions of [kv heads, {D}]")
+        if out is not None and (out.shape != q.shape or out.dtype != torch.float16 or out.stride(2) != 1 or out.stride(1) != D):
+            raise Q40Error("causal_attn: fp16 out like q with contiguous heads expected")
     if out is None:
         out = torch.empty((S, H, D), dtype=torch.float16, device=dev)
+    if windowed:
+        whole = offset + S
+        # (the stride of a dimension of one may be anything)
+        lds = [t.stride(0) if t.shape[0] > 1 else t.shape[1] * D for t in (q, k, v, out)]
+        check(lib.q40_attn_causal_window(q.data_ptr(), lds[0], k.data_ptr(), lds[1], v.data_ptr(), lds[2], out.data_ptr(), lds[3], S, H, Hkv, D,
+                                         offset, whole if window is None else min(window, max(whole, 1)), min(sinks, whole), _stream(dev)),
+              "q40_attn_causal_window")
+        return out
     check(lib.q40_attn_causal(q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
                               out.data_ptr(), out.stride(0), S, H, Hkv, D, _stream(dev)), "q40_attn_causal")
     return out
@@ -722,11 +743,16 @@ def _table(p: torch.Tensor):
     return p.to(torch.int32), 4
 
 
-def page_flash_attn(p, q, k, v, P, B, L, H, D, *, page_size: int = 1, seq_lens=None):
+def page_flash_attn(p, q, k, v, P, B, L, H, D, *, page_size: int = 1, seq_lens=None, window: Optional[int] = None, sinks: int = 0):
     """Paged decode attention; same call as the reference's page_flash_attn
     (triton_kernels.py:764-789): p [B,L] int16 token-slot table, k/v pools [H,P,D].
-    Extensions: page_size > 1 (p then lists page ids), int32 tables, per-branch seq_lens."""
+    Extensions: page_size > 1 (p then lists page ids), int32 tables, per-branch seq_lens; with `window`, a query, which is its branch's
+    last position, attends that many last keys and the first `sinks` alone."""
     dev = _need_cuda(p, q, k, v, seq_lens)
+    if window is not None or sinks != 0:
+        if k.dtype != torch.float16 or v.dtype != torch.float16 or q.shape != (B, H, D) or k.shape[1:] != (P, D) or v.shape != k.shape:
+            raise Q40Error(f"page_flash_attn: fp16 pools [kv heads, {P}, {D}] and queries [{B}, {H}, {D}] expected")
+        return _attn_pages("page_flash_attn", dev, p, q, k.contiguous(), v.contiguous(), None, None, L, page_size, seq_lens, window, sinks)
     p, idx_bytes = _table(p)
     if p.stride(-1) != 1:
         p = p.contiguous()
@@ -739,6 +765,135 @@ def page_flash_attn(p, q, k, v, P, B, L, H, D, *, page_size: int = 1, seq_lens=N
                              k.data_ptr(), v.data_ptr(), o.data_ptr(), P, B, L, H, Hkv, D, page_size,
                              _stream(dev)), "q40_attn_paged")
     return o
+
+
+_CACHE_TYPES = {torch.float16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}       # Q40_CACHE_*
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` [rows, heads, D] as the kernels read it: heads side by side, 16-byte rows at 16-byte addresses; a copy where it is not."""
+    n, D = t.shape[1], t.shape[2]
+    if t.stride(2) != 1 or (n > 1 and t.stride(1) != D) or (t.shape[0] > 1 and (t.stride(0) % 8 != 0 or t.stride(0) < n * D)):
+        t = t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 else t
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]          # (that of one row may be anything)
+
+
+def _need_pools(what: str, k, v, k_scale, v_scale, page_size: int) -> int:
+    """The Q40_CACHE_* of two pools [Hkv, P, 128], which have to lie as they are read, and be of one kind."""
+    kind = _CACHE_TYPES.get(k.dtype)
+    if kind is None or v.dtype != k.dtype:
+        raise Q40Error(f"{what}: pools of float16, int8 or float8_e4m3fn expected, got {k.dtype} and {v.dtype}")
+    if k.dim() != 3 or k.shape != v.shape or not (k.is_contiguous() and v.is_contiguous()):
+        raise Q40Error(f"{what}: contiguous pools [kv heads, slots, 128] of one shape expected, got {tuple(k.shape)} and {tuple(v.shape)}")
+    if page_size < 1:
+        raise Q40Error(f"{what}: page_size {page_size}")
+    if kind == 0:
+        if k_scale is not None or v_scale is not None:
+            raise Q40Error(f"{what}: fp16 pools have no scales")
+        return kind
+    want = (k.shape[0], k.shape[1] // page_size)
+    for s in (k_scale, v_scale):
+        if s is None or s.dtype != torch.float32 or tuple(s.shape) != want or not s.is_contiguous() or k.shape[1] % page_size:
+            raise Q40Error(f"{what}: 8-bit pools of whole pages and contiguous fp32 scales {want}, one for each kv head and page, expected")
+    return kind
+
+
+def _page_table(what: str, p: torch.Tensor, rows: int):
+    if p.dim() != 2 or p.shape[0] != rows or p.dtype.is_floating_point:
+        raise Q40Error(f"{what}: a table of {rows} rows of page ids expected, got {tuple(p.shape)} of {p.dtype}")
+    p, idx_bytes = _table(p)
+    if p.stride(1) != 1 and p.shape[1] > 1 or (rows > 1 and p.stride(0) < p.shape[1]):
+        p = p.contiguous()
+    return p, idx_bytes, p.stride(0) if rows > 1 else p.shape[1]
+
+
+def _attn_pages(what, dev, p, q, k, v, k_scale, v_scale, L, page_size, seq_lens, window, sinks):
+    kind = _need_pools(what, k, v, k_scale, v_scale, page_size)
+    if q.dim() != 3 or q.dtype != torch.float16 or q.shape[2] != k.shape[2]:
+        raise Q40Error(f"{what}: fp16 queries [sequences, heads, {k.shape[2]}] expected, got {tuple(q.shape)} of {q.dtype}")
+    if (window is not None and window < 1) or sinks < 0:
+        raise Q40Error(f"{what}: window {window} below 1 or sinks {sinks} below 0")
+    B, H, D = q.shape
+    p, idx_bytes, tbl_stride = _page_table(what, p, B)
+    if L > p.shape[1] * page_size:
+        raise Q40Error(f"{what}: {L} keys do not fit a table of {p.shape[1]} pages of {page_size}")
+    if seq_lens is not None:
+        if seq_lens.shape != (B,):
+            raise Q40Error(f"{what}: {B} lengths expected, got {tuple(seq_lens.shape)}")
+        seq_lens = seq_lens.to(torch.int32).contiguous()
+    q = _rows(q)
+    o = torch.empty((B, H, D), device=dev, dtype=torch.float16)
+    w, sinks = (0, 0) if window is None else (min(window, 1 << 30), min(sinks, 1 << 30))
+    nbytes = lib.q40_attn_pages_workspace_bytes(B, H, k.shape[0], L, w, sinks)
+    # of this call alone: calls on other streams and captured graphs that overlap it have their own
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    check(lib.q40_attn_pages(p.data_ptr(), idx_bytes, tbl_stride, _ptr(seq_lens), q.data_ptr(), _row_stride(q), k.data_ptr(), v.data_ptr(),
+                             _ptr(k_scale), _ptr(v_scale), kind, o.data_ptr(), k.shape[1], B, L, H, k.shape[0], D, page_size, w, sinks,
+                             _ptr(ws), nbytes, _stream(dev)), "q40_attn_pages")
+    return o
+
+
+def page_flash_attn_q8(p, q, k, v, k_scale, v_scale, *, page_size: int, seq_lens=None, window: Optional[int] = None, sinks: int = 0):
+    """page_flash_attn over a cache held in 8 bits: pools k / v [Hkv, P, 128] of int8 or float8_e4m3fn codes with one fp32 scale for each
+    page and kv head, k_scale / v_scale [Hkv, P / page_size] (element = code * scale), as page_append writes them.  q [B, H, 128] is
+    one query for each sequence, its last position; p [B, pages] lists page ids, seq_lens [B] the lengths (None: the table's whole width).
+    With `window` a query attends that many last keys and the first `sinks` alone (q40_attn_pages in include/q40b200.h)."""
+    dev = _need_cuda(p, q, k, v, k_scale, v_scale, seq_lens)
+    if k.dtype == torch.float16:
+        raise Q40Error("page_flash_attn_q8: 8-bit pools expected; page_flash_attn reads fp16 ones")
+    return _attn_pages("page_flash_attn_q8", dev, p, q, k, v, k_scale, v_scale, p.shape[-1] * page_size, page_size, seq_lens, window, sinks)
+
+
+def page_append(p, k, v, kpool, vpool, pos, *, page_size: int = 1, offsets=None, k_scale=None, v_scale=None, q=None, cos=None, sin=None):
+    """Append new tokens' keys and values to a paged cache (in place): pools [Hkv, P, 128] of float16, or of int8 or float8_e4m3fn codes with scales
+    [Hkv, P / page_size] fp32, as page_flash_attn and page_flash_attn_q8 read them through the table p [B, pages] of page ids.
+
+    k / v [T, Hkv, 128] fp16 (rows may be strided, like views of one projection's output).  Without `offsets`, T == B and row b is
+    sequence b's one new token, at position pos[b]; with offsets [B + 1], rows offsets[b] .. offsets[b + 1] - 1 are sequence b's, from position
+    pos[b] on.  With fp16 tables cos / sin [n_pos, 64] keys are rotated to their positions on the way, and q [T, H, 128], if given, is
+    returned rotated (zeros for rows of no sequence); a rotated value is rounded once, where rope_ keeps the reference's roundings.
+
+    Rows of no sequence and positions without a page are not written.  An 8-bit page's scale grows with what comes, and its earlier
+    rows are coded anew when it does.  Tokens of one call that share a slot, or in 8 bits sequences that append to one page, leave it undefined
+    (q40_page_append in include/q40b200.h)."""
+    dev = _need_cuda(p, k, v, kpool, vpool, pos, offsets, k_scale, v_scale, q, cos, sin)
+    kind = _need_pools("page_append", kpool, vpool, k_scale, v_scale, page_size)
+    Hkv, P, D = kpool.shape
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (Hkv, D) or k.dtype != torch.float16 or v.dtype != torch.float16:
+        raise Q40Error(f"page_append: fp16 keys and values [tokens, {Hkv}, {D}] expected, got {tuple(k.shape)} and {tuple(v.shape)}")
+    T, B = k.shape[0], pos.shape[0] if pos.dim() == 1 else -1
+    if B < 0 or (T != B if offsets is None else offsets.shape != (B + 1,)):
+        raise Q40Error(f"page_append: {T} tokens, positions {tuple(pos.shape)} and offsets "
+                       f"{None if offsets is None else tuple(offsets.shape)} do not go together")
+    if (cos is None) != (sin is None) or (q is not None and cos is None):
+        raise Q40Error("page_append: both tables, cos and sin, or neither; queries come to be rotated and need them")
+    if cos is not None and (cos.dtype != torch.float16 or sin.dtype != torch.float16 or cos.dim() != 2 or cos.shape[1] != D // 2 or sin.shape != cos.shape):
+        raise Q40Error(f"page_append: fp16 tables [positions, {D // 2}] expected, got {tuple(cos.shape)} and {tuple(sin.shape)}")
+    if q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[2] != D or q.dtype != torch.float16):
+        raise Q40Error(f"page_append: fp16 queries [{T}, heads, {D}] expected, got {tuple(q.shape)}")
+    p, idx_bytes, tbl_stride = _page_table("page_append", p, B)
+    pos = pos.to(torch.int32).contiguous()
+    if offsets is not None:
+        offsets = offsets.to(torch.int32).contiguous()
+    k, v = _rows(k), _rows(v)
+    q_out = None
+    if q is not None:
+        q, q_out = _rows(q), torch.empty(q.shape, device=dev, dtype=torch.float16)
+        if B == 0:
+            q_out.zero_()
+    if cos is not None:
+        cos, sin = (t.clone() if t.data_ptr() % 16 else t for t in (cos.contiguous(), sin.contiguous()))
+    check(lib.q40_page_append(p.data_ptr(), idx_bytes, tbl_stride, p.shape[1], pos.data_ptr(), _ptr(offsets), _ptr(q),
+                              _row_stride(q) if q is not None else 0, _ptr(q_out), k.data_ptr(), _row_stride(k), v.data_ptr(), _row_stride(v),
+                              _ptr(cos), _ptr(sin), cos.shape[0] if cos is not None else 0, kpool.data_ptr(), vpool.data_ptr(), _ptr(k_scale),
+                              _ptr(v_scale), kind, P, B, T, q.shape[1] if q is not None else 0, Hkv, D, page_size, _stream(dev)), "q40_page_append")
+    # writes that torch did not make itself: counted, as by quantize_q40_rows
+    torch.autograd.graph.increment_version([t for t in (kpool, vpool, k_scale, v_scale) if t is not None and not t.is_inference()])
+    return q_out
 
 
 def shared_prefix_attn(q, prefix_k, prefix_v, prefix_len, p, seq_lens, kpool, vpool, *,
