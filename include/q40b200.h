@@ -305,7 +305,7 @@ int q40_attn_paged(const void* page_tbl, int idx_bytes, int64_t tbl_stride, cons
  * (at q + b*q_stride elements, position seq_lens[b] - 1) attends its last `window` keys (0: all) and its first `sinks`.  cache_type
  * says what the pools [Hkv, P, D] hold: Q40_CACHE_F16, or signed 8-bit codes or e4m3 codes, element = code * scale with one fp32 scale >= 0 for
  * each page and kv head, k_scale / v_scale [Hkv, P / page_size] (P a multiple of page_size; NULL for fp16).  Table, lengths (NULL: Lmax each;
- * at most Lmax <= 2^30 count) and the order of tokens as in q40_attn_paged.  A sequence without keys gets zeros.  Keys that are not visible are not
+ * at most Lmax <= 2^29 count) and the order of tokens as in q40_attn_paged.  A sequence without keys gets zeros.  Keys that are not visible are not
  * read.  An element whose scale is NaN is NaN.  Results do not depend on Lmax.  Workspace: *_workspace_bytes bytes, 16-byte aligned, no
  * initialisation (0 bytes: may be NULL); calls that may overlap need one each.  No counterpart in the reference. */
 #define Q40_CACHE_F16 0

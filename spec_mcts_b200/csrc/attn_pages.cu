@@ -3,10 +3,10 @@
 //
 // The visible keys of a sequence are numbered through (first ones, then the window), so that a window costs nothing but the look-up of
 // a key's place, and masked keys are never read.  A unit is a sequence and up to eight query heads of one kv head, whose keys and values are
-// read once for all of them; its keys go to CTAs in chunks that begin at multiples of `chunk`, whatever the lengths, so that
+// read once for all of them; its keys go to CTAs in chunks, whose size goes by the number of keys and of units alone (chunk_of), so that
 // results do not depend on how long the tables are.  A unit of one chunk writes its output; the partial results of several meet in page_merge_kernel.
 //
-// A warp takes 16 keys at a time through a ring of its own (cp.async):
+// A warp takes 16 keys at a time, of 8-bit ones 32, through a ring of its own (cp.async):
 //   scores   A = 16 keys, B = the queries: columns 2i and 2i + 1 are head i's (of two heads, 4i .. 4i + 3; of one, all; of eight, one each)
 //   output   A = 16 values transposed, B = the weights, each as two fp16 parts (weight_parts): a head's two columns, or, of eight
 //            heads, two products
@@ -20,7 +20,9 @@
 namespace q40 {
 namespace pages {
 
-constexpr int KEYS = 16, NW = 4, THREADS = NW * 32;
+constexpr int NW = 4, THREADS = NW * 32;
+constexpr int CHUNK_MIN = 512, CHUNK_MAX = 8192;
+constexpr int64_t CHUNKS = 4800;
 
 struct Args {
   const __half* q;         // sequence b, head h at q + b * q_stride + h * 128
@@ -34,7 +36,8 @@ struct Args {
   int64_t P;
   int B, L, H, Hkv, window, sinks;
   int groups, heads;       // of a kv head's query heads; heads of a group (the last may have fewer)
-  int chunk, nchunks;
+  int64_t chunks_of_unit; // what a unit's keys are cut into, about (chunk_of)
+  int nchunks;             // most of a unit
   float* po;               // [units][nchunks][heads][128], not normalised
   float2* pml;             // ... maximum (log2) and sum
   float scale_log2;
@@ -43,7 +46,9 @@ struct Args {
 template <int T>
 constexpr int row_bytes = ATTN_D * cache_bytes<T>;
 template <int T>
-constexpr int stage_bytes = 2 * KEYS * row_bytes<T> + (T == CACHE_F16 ? 0 : 2 * KEYS * 4);
+constexpr int keys_of = T == CACHE_F16 ? 16 : 32;         // of a stage: 8 KB
+template <int T>
+constexpr int stage_bytes = 2 * keys_of<T> * row_bytes<T> + (T == CACHE_F16 ? 0 : 2 * keys_of<T> * 4);
 template <int T, int G, int S>
 constexpr int warp_bytes = S * stage_bytes<T> > G * ATTN_D * 4 ? S * stage_bytes<T> : G * ATTN_D * 4;
 
@@ -54,7 +59,7 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 }
 __device__ __forceinline__ float lg2(float x) {
   float y;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
@@ -70,6 +75,13 @@ __device__ __forceinline__ float lds32(uint32_t addr) {
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool pred) {
   const int sz = pred ? 4 : 0;
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(sz));
+}
+
+// Keys of a chunk for a unit of n keys, by its own length and the number of units alone
+__host__ __device__ __forceinline__ int chunk_of(int64_t n, int64_t chunks_of_unit) {
+  int chunk = CHUNK_MIN;
+  while (chunk < CHUNK_MAX && chunk * chunks_of_unit < n) chunk *= 2;
+  return chunk;
 }
 
 // Visible keys of a sequence: number n; key i of them is position i below `first`, then i + skip
@@ -91,22 +103,24 @@ __device__ __forceinline__ uint32_t weight_parts_of_one_sum(float p) {
   return h2_as_u32(__halves2half2(h, __hmax_nan(__float2half_rn(p - __half2float(h)), least)));
 }
 
-// Words of two codes each (bytes 0 and 1 of the word, and 2 and 3) as halves
+// Four codes as two pairs of halves
 template <int T>
-__device__ __forceinline__ uint32_t low_two(uint32_t w) {
-  return T == CACHE_I8 ? i8_to_h2(prmt(w, 0x64646464u, 0x4140)) : e4m3_to_h2(w & 0xffffu);
-}
-template <int T>
-__device__ __forceinline__ uint32_t high_two(uint32_t w) {
-  return T == CACHE_I8 ? i8_to_h2(prmt(w, 0x64646464u, 0x4342)) : e4m3_to_h2(w >> 16);
+__device__ __forceinline__ uint2 halves_of(uint32_t w) {
+  return T == CACHE_I8 ? make_uint2(i8_to_h2(prmt(w, 0x64646464u, 0x4140)), i8_to_h2(prmt(w, 0x64646464u, 0x4342))) : e4m3_to_h4(w);
 }
 template <int T>
 __device__ __forceinline__ uint32_t biased(uint32_t w) { return T == CACHE_I8 ? w ^ 0x80808080u : w; }
+// base + i * size in one instruction
+__device__ __forceinline__ const unsigned char* row_at(const unsigned char* base, int i, int size) {
+  const unsigned char* r;
+  asm("mad.wide.s32 %0, %1, %2, %3;" : "=l"(r) : "r"(i), "r"(size), "l"(base));
+  return r;
+}
 
 template <int T, int G, int S>
 __global__ void __launch_bounds__(THREADS)
 attn_pages_kernel(const Args a) {
-  constexpr int D = ATTN_D, RB = row_bytes<T>;
+  constexpr int D = ATTN_D, RB = row_bytes<T>, KEYS = keys_of<T>, MT = KEYS / 16;
   constexpr int GL = G == 4 ? 0 : G == 2 ? 1 : 2;        // up to four heads: lane t works for head t >> GL
   constexpr int HL = G == 8 ? 2 : 1;                     // heads of a lane
   constexpr int LPR = RB / 16, RPI = 32 / LPR;           // lanes that copy a row, rows a copy instruction
@@ -117,22 +131,23 @@ attn_pages_kernel(const Args a) {
   const int group = unit % a.groups, hk = unit / a.groups % a.Hkv, b = unit / a.groups / a.Hkv;
   const int rep = a.H / a.Hkv, h0 = hk * rep + group * a.heads, heads = min(a.heads, rep - group * a.heads);
   const Visible vis(a, b);
-  const int64_t begin64 = (int64_t)chunk * a.chunk;
+  const int size = chunk_of(vis.n, a.chunks_of_unit);
+  const int64_t begin64 = (int64_t)chunk * size;
   if (begin64 >= vis.n && chunk > 0) return;
-  const int begin = (int)begin64, end = (int)min((int64_t)vis.n, begin64 + a.chunk);
+  const int begin = (int)begin64, end = (int)min((int64_t)vis.n, begin64 + size);
 
   extern __shared__ __align__(128) unsigned char rings[];
   constexpr int WB = warp_bytes<T, G, S>;
   const uint32_t ring = smem_u32(rings + warp * WB);
   const unsigned char* const kb = reinterpret_cast<const unsigned char*>(a.k) + (int64_t)hk * a.P * RB + (lane % LPR) * 16;
   const unsigned char* const vb = reinterpret_cast<const unsigned char*>(a.v) + (int64_t)hk * a.P * RB + (lane % LPR) * 16;
-  const float* const scales = (lane < 16 ? a.ks : a.vs) + (int64_t)hk * a.pages;
+  const float *const ks = a.ks + (int64_t)hk * a.pages, *const vs = a.vs + (int64_t)hk * a.pages;
 
-  // place of the 16 keys from i0 in lanes 0 to 15 and again in 16 to 31, looked up one request ahead
+  // place of the keys from i0 on, one a lane (16 keys: again in lanes 16 to 31), looked up one request ahead
   struct Place { int page, slot; };
   const auto place_of = [&](int i0) {
     Place p = {0, 0};
-    const int i = i0 + (lane & 15);
+    const int i = i0 + (lane & (KEYS - 1));
     if (i < end) {
       const int pos = i < vis.first ? i : i + vis.skip, pg = a.tbl.page_of(pos);
       // a bad page id must not turn into a wild read: clamp into the pool
@@ -147,12 +162,17 @@ attn_pages_kernel(const Args a) {
     for (int j = 0; j < KEYS / RPI; ++j) {
       const int r = j * RPI + lane / LPR;
       const bool ok = i0 + r < end;
-      const int64_t off = (int64_t)__shfl_sync(0xffffffffu, p.slot, r) * RB;
+      const int slot = __shfl_sync(0xffffffffu, p.slot, r);
       const uint32_t at = r * RB + (((lane % LPR) ^ (r & 7)) << 4);
-      cp_async16(kt + at, kb + off, ok);
-      cp_async16(vt + at, vb + off, ok);
+      cp_async16(kt + at, row_at(kb, slot, RB), ok);
+      cp_async16(vt + at, row_at(vb, slot, RB), ok);
     }
-    if (T != CACHE_F16) cp_async4(vt + KEYS * RB + lane * 4, scales + p.page, i0 + (lane & 15) < end);
+    if (T != CACHE_F16) {
+      static_assert(T == CACHE_F16 || KEYS == 32, "a lane copies the scales of one key");
+      const bool ok = i0 + lane < end;
+      cp_async4(vt + KEYS * RB + lane * 4, ks + p.page, ok);
+      cp_async4(vt + KEYS * RB + KEYS * 4 + lane * 4, vs + p.page, ok);
+    }
   };
   constexpr int STEP = NW * KEYS;
   const int mine = begin + warp * KEYS;
@@ -171,14 +191,14 @@ attn_pages_kernel(const Args a) {
     const int head = min(G == 8 ? g : (g >> 1) >> GL, heads - 1);
     const __half* const q = a.q + b * a.q_stride + (int64_t)(h0 + head) * D;
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
+    for (int i = 0; i < 8; ++i) {
       if (T == CACHE_F16) {
-        qb[ks][0] = *reinterpret_cast<const uint32_t*>(q + 16 * ks + 2 * t);
-        qb[ks][1] = *reinterpret_cast<const uint32_t*>(q + 16 * ks + 8 + 2 * t);
+        qb[i][0] = *reinterpret_cast<const uint32_t*>(q + 16 * i + 2 * t);
+        qb[i][1] = *reinterpret_cast<const uint32_t*>(q + 16 * i + 8 + 2 * t);
       } else {
-        const uint2 w = *reinterpret_cast<const uint2*>(q + 32 * t + 4 * ks);
-        qb[ks][0] = w.x;
-        qb[ks][1] = w.y;
+        const uint2 w = *reinterpret_cast<const uint2*>(q + 32 * t + 4 * i);
+        qb[i][0] = w.x;
+        qb[i][1] = w.y;
       }
     }
   }
@@ -196,57 +216,65 @@ attn_pages_kernel(const Args a) {
     cp_async_wait<S - 1>();
     __syncwarp();
     const uint32_t kt = ring + stage * stage_bytes<T>, vt = kt + KEYS * RB;
-    float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (T == CACHE_F16) {
+    float x[MT][4], sc[2 * MT][HL], lv[2 * MT];    // scores, log2 of the values' scales of keys 8r + g
 #pragma unroll
-      for (int ks = 0; ks < 8; ks += 2) {
-        uint32_t x[4], y[4];
-        const int r = (lane & 7) + (mi & 1) * 8;
-        ldsm_x4(kt + tile_off(r, 2 * ks + (mi >> 1)), x[0], x[1], x[2], x[3]);
-        ldsm_x4(kt + tile_off(r, 2 * ks + 2 + (mi >> 1)), y[0], y[1], y[2], y[3]);
-        mma_f16(c0, x[0], x[1], x[2], x[3], qb[ks][0], qb[ks][1]);
-        mma_f16(c1, y[0], y[1], y[2], y[3], qb[ks + 1][0], qb[ks + 1][1]);
-      }
-    } else {
+    for (int mt = 0; mt < MT; ++mt) {
+      float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (T == CACHE_F16) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint4 x = lds128(kt + g * RB + (((2 * t + c) ^ g) << 4)), y = lds128(kt + (g + 8) * RB + (((2 * t + c) ^ g) << 4));
-        const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+        for (int i = 0; i < 8; i += 2) {
+          uint32_t y[4], z[4];
+          const int r = (lane & 7) + (mi & 1) * 8;
+          ldsm_x4(kt + tile_off(r, 2 * i + (mi >> 1)), y[0], y[1], y[2], y[3]);
+          ldsm_x4(kt + tile_off(r, 2 * i + 2 + (mi >> 1)), z[0], z[1], z[2], z[3]);
+          mma_f16(c0, y[0], y[1], y[2], y[3], qb[i][0], qb[i][1]);
+          mma_f16(c1, z[0], z[1], z[2], z[3], qb[i + 1][0], qb[i + 1][1]);
+        }
+      } else {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t u = biased<T>(xw[w]), z = biased<T>(yw[w]);
-          mma_f16(w & 1 ? c1 : c0, low_two<T>(u), low_two<T>(z), high_two<T>(u), high_two<T>(z), qb[4 * c + w][0], qb[4 * c + w][1]);
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t at = kt + (16 * mt + g) * RB + (((2 * t + c) ^ g) << 4);
+          const uint4 y4 = lds128(at), z4 = lds128(at + 8 * RB);
+          const uint32_t y[4] = {y4.x, y4.y, y4.z, y4.w}, z[4] = {z4.x, z4.y, z4.z, z4.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint2 u = halves_of<T>(biased<T>(y[w])), v = halves_of<T>(biased<T>(z[w]));
+            mma_f16(w & 1 ? c1 : c0, u.x, v.x, u.y, v.y, qb[4 * c + w][0], qb[4 * c + w][1]);
+          }
         }
       }
-    }
-    float lv[2] = {0.f, 0.f}, s[2][HL];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+      for (int j = 0; j < 4; ++j) x[mt][j] = c0[j] + c1[j];
+    }
+    bool above = false;
+#pragma unroll
+    for (int r = 0; r < 2 * MT; ++r) {
       float scale = a.scale_log2;
+      lv[r] = 0.f;
       if (T != CACHE_F16) {
         scale *= lds32(vt + KEYS * RB + (8 * r + g) * 4);
-        const float x = lg2(lds32(vt + KEYS * RB + 64 + (8 * r + g) * 4));
-        lv[r] = x < -60.f ? -60.f : x;           // a scale of 0: next to nothing.  NaN stays
+        const float y = lg2(lds32(vt + KEYS * RB + KEYS * 4 + (8 * r + g) * 4));
+        lv[r] = y < -60.f ? -60.f : y;           // a scale of 0: next to nothing.  NaN stays
       }
       const bool there = i0 + 8 * r + g < end;
 #pragma unroll
-      for (int j = 0; j < HL; ++j) s[r][j] = there ? (c0[2 * r + j] + c1[2 * r + j]) * scale : -CUDART_INF_F;
+      for (int j = 0; j < HL; ++j) {
+        sc[r][j] = there ? x[r >> 1][2 * (r & 1) + j] * scale : -CUDART_INF_F;
+        above |= sc[r][j] + lv[r] > m[j] + (WEIGHT_BITS + 1.f);
+      }
     }
-    float mnew[HL];
-    bool moved = false;
-#pragma unroll
-    for (int j = 0; j < HL; ++j) {
-      mnew[j] = fmaxf(m[j], fmaxf(s[0][j] + lv[0], s[1][j] + lv[1]) - WEIGHT_BITS);
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) mnew[j] = fmaxf(mnew[j], __shfl_xor_sync(0xffffffffu, mnew[j], o));
-      moved |= mnew[j] != m[j];
-    }
-    if (moved) {
+    // a maximum stays while no weight passes 2^(WEIGHT_BITS + 1), which fp16 holds
+    if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
       for (int j = 0; j < HL; ++j) {
-        const float corr = ex2(m[j] - mnew[j]);
+        float mnew = m[j];
+#pragma unroll
+        for (int r = 0; r < 2 * MT; ++r) mnew = fmaxf(mnew, sc[r][j] + lv[r] - WEIGHT_BITS);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) mnew = fmaxf(mnew, __shfl_xor_sync(0xffffffffu, mnew, o));
+        const float corr = ex2(m[j] - mnew);
         l[j] *= corr;
-        m[j] = mnew[j];
+        m[j] = mnew;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           acc[i][j] *= corr;
@@ -255,48 +283,47 @@ attn_pages_kernel(const Args a) {
         }
       }
     }
-    __syncwarp();                                // heads differ in whether theirs has moved
-    uint32_t pk[2][HL];                          // both parts of a weight
+    uint32_t bh[2 * MT], bl[2 * MT];             // B fragments of the weights' first and second parts
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int r = 0; r < 2 * MT; ++r) {
+      uint32_t pk[HL];                           // both parts of a weight
 #pragma unroll
       for (int j = 0; j < HL; ++j) {
-        const float w = ex2(s[r][j] + lv[r] - m[j]);
-        l[j] += T == CACHE_F16 ? w : ex2(s[r][j] - m[j]);
-        pk[r][j] = HL == 1 ? weight_parts(w) : weight_parts_of_one_sum(w);
+        const float w = ex2(sc[r][j] + lv[r] - m[j]);
+        l[j] += T == CACHE_F16 ? w : ex2(sc[r][j] - m[j]);
+        pk[j] = HL == 1 ? weight_parts(w) : weight_parts_of_one_sum(w);
       }
-    uint32_t bh[2], bl[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
       if (HL == 1) {
-        bh[r] = movmatrix(pk[r][0]);
+        bh[r] = movmatrix(pk[0]);
       } else {
-        bh[r] = movmatrix(prmt(pk[r][0], pk[r][HL - 1], 0x5410));
-        bl[r] = movmatrix(prmt(pk[r][0], pk[r][HL - 1], 0x7632));
+        bh[r] = movmatrix(prmt(pk[0], pk[HL - 1], 0x5410));
+        bl[r] = movmatrix(prmt(pk[0], pk[HL - 1], 0x7632));
       }
     }
-    if constexpr (T == CACHE_F16) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint32_t x[4];
-        ldsm_x4_t(vt + tile_off((lane & 7) + (mi >> 1) * 8, 2 * i + (mi & 1)), x[0], x[1], x[2], x[3]);
-        mma_f16(acc[i], x[0], x[1], x[2], x[3], bh[0], bh[1]);
-        if (HL == 2) mma_f16(acc[i], x[0], x[1], x[2], x[3], bl[0], bl[1]);
-      }
-    } else {
-      // keys 2t, 2t + 1 (x, y) and 2t + 8, 2t + 9 (z, u), dims 16 g ..: product i has dims 2i (rows g) and 2i + 1 (rows g + 8) of these
-      const auto values = [&](int key) { return lds128(vt + key * RB + ((g ^ (key & 7)) << 4)); };
-      const uint4 x4 = values(2 * t), y4 = values(2 * t + 1), z4 = values(2 * t + 8), u4 = values(2 * t + 9);
-      const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w}, z[4] = {z4.x, z4.y, z4.z, z4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
+    for (int mt = 0; mt < MT; ++mt) {
+      if constexpr (T == CACHE_F16) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t bx = biased<T>(x[w]), by = biased<T>(y[w]), bz = biased<T>(z[w]), bu = biased<T>(u[w]);
+        for (int i = 0; i < 8; ++i) {
+          uint32_t y[4];
+          ldsm_x4_t(vt + tile_off((lane & 7) + (mi >> 1) * 8, 2 * i + (mi & 1)), y[0], y[1], y[2], y[3]);
+          mma_f16(acc[i], y[0], y[1], y[2], y[3], bh[0], bh[1]);
+          if (HL == 2) mma_f16(acc[i], y[0], y[1], y[2], y[3], bl[0], bl[1]);
+        }
+      } else {
+        // keys 2t, 2t + 1 (y, z) and 2t + 8, 2t + 9 (u, v), dims 16 g ..: product i has dims 2i (rows g) and 2i + 1 (rows g + 8) of these
+        const auto values = [&](int key) { return lds128(vt + (16 * mt + key) * RB + ((g ^ (key & 7)) << 4)); };
+        const uint4 y4 = values(2 * t), z4 = values(2 * t + 1), u4 = values(2 * t + 8), v4 = values(2 * t + 9);
+        const uint32_t y[4] = {y4.x, y4.y, y4.z, y4.w}, z[4] = {z4.x, z4.y, z4.z, z4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t xy = prmt(bx, by, half ? 0x7362 : 0x5140), zu = prmt(bz, bu, half ? 0x7362 : 0x5140);
-          const uint32_t a0 = low_two<T>(xy), a1 = high_two<T>(xy), a2 = low_two<T>(zu), a3 = high_two<T>(zu);
-          mma_f16(acc[2 * w + half], a0, a1, a2, a3, bh[0], bh[1]);
-          if (HL == 2) mma_f16(acc[2 * w + half], a0, a1, a2, a3, bl[0], bl[1]);
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t by = biased<T>(y[w]), bz = biased<T>(z[w]), bu = biased<T>(u[w]), bv = biased<T>(v[w]);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint2 yz = halves_of<T>(prmt(by, bz, half ? 0x7362 : 0x5140)), uv = halves_of<T>(prmt(bu, bv, half ? 0x7362 : 0x5140));
+            mma_f16(acc[2 * w + half], yz.x, yz.y, uv.x, uv.y, bh[2 * mt], bh[2 * mt + 1]);
+            if (HL == 2) mma_f16(acc[2 * w + half], yz.x, yz.y, uv.x, uv.y, bl[2 * mt], bl[2 * mt + 1]);
+          }
         }
       }
     }
@@ -335,7 +362,7 @@ attn_pages_kernel(const Args a) {
     }
   }
   __syncthreads();
-  const bool alone = vis.n <= a.chunk;
+  const bool alone = vis.n <= size;
 #pragma unroll
   for (int j = 0; j < G; ++j) {
     if (j >= heads) break;
@@ -368,8 +395,9 @@ page_merge_kernel(const Args a) {
   const int rep = a.H / a.Hkv;
   if (j >= rep - group * a.heads) return;
   const Visible vis(a, b);
-  if (vis.n <= a.chunk) return;
-  const int n = (vis.n - 1) / a.chunk + 1;
+  const int size = chunk_of(vis.n, a.chunks_of_unit);
+  if (vis.n <= size) return;
+  const int n = (vis.n - 1) / size + 1;
   const int64_t first = (int64_t)unit * a.nchunks * a.heads + j;
   float M = NO_KEY;
   for (int c = tid & 31; c < n; c += 32) M = fmaxf(M, a.pml[first + (int64_t)c * a.heads].x);
@@ -386,7 +414,7 @@ page_merge_kernel(const Args a) {
   a.o[((int64_t)b * a.H + hk * rep + group * a.heads + j) * ATTN_D + tid] = __float2half_rn(Lsum != 0.f ? x / Lsum : 0.f);
 }
 
-struct Plan { int64_t units; int groups, heads, chunk, nchunks; };
+struct Plan { int64_t units, chunks_of_unit; int groups, heads, nchunks; };
 
 static Plan plan_of(int B, int H, int Hkv, int L, int window, int sinks) {
   Plan p;
@@ -394,17 +422,20 @@ static Plan plan_of(int B, int H, int Hkv, int L, int window, int sinks) {
   p.groups = (rep + 7) / 8;
   p.heads = (rep + p.groups - 1) / p.groups;
   p.units = (int64_t)B * Hkv * p.groups;
+  p.chunks_of_unit = std::max<int64_t>(1, CHUNKS / p.units);
   const int64_t most = window > 0 ? std::min<int64_t>(L, (int64_t)window + sinks) : L;      // visible keys
-  int64_t chunk = p.units <= 32 ? 256 : p.units <= 512 ? 512 : p.units <= 2048 ? 1024 : 2048;
-  while ((most + chunk - 1) / chunk > 65535) chunk *= 2;
-  p.chunk = (int)chunk;
-  p.nchunks = (int)std::max<int64_t>(1, (most + chunk - 1) / chunk);
+  int64_t n = 1;
+  for (int64_t chunk = CHUNK_MIN; chunk <= CHUNK_MAX; chunk *= 2) {
+    const int64_t longest = chunk < CHUNK_MAX ? std::min(most, chunk * p.chunks_of_unit) : most;      // of those cut into such
+    if (longest > 0 && chunk_of(longest, p.chunks_of_unit) == chunk) n = std::max(n, (longest + chunk - 1) / chunk);
+  }
+  p.nchunks = (int)std::min<int64_t>(n, 1 << 30);
   return p;
 }
 
 template <int T, int G>
 static cudaError_t launch(const Args& a, int64_t units, cudaStream_t st) {
-  constexpr int S = 3;
+  constexpr int S = T == CACHE_F16 ? 3 : 2;
   static std::atomic<uint64_t> ready;
   constexpr int BYTES = NW * warp_bytes<T, G, S>;
   const cudaError_t e = q40_allow_smem(ready, (const void*)attn_pages_kernel<T, G, S>, BYTES);
@@ -435,7 +466,7 @@ extern "C" int q40_attn_pages(const void* page_tbl, int idx_bytes, int64_t tbl_s
   if (!q || !o) return Q40_E_NULL;
   if (D != ATTN_D || (idx_bytes != 2 && idx_bytes != 4) || cache_type < CACHE_F16 || cache_type > CACHE_E4M3) return Q40_E_UNSUPPORTED;
   if (B < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || (int64_t)B * H > 0x7fffffffLL) return Q40_E_SHAPE;
-  if (Lmax < 0 || Lmax > (1 << 30) || P < 0 || P > 0x7fffffffLL || page_size <= 0 || window < 0 || sinks < 0 || q_stride < (int64_t)H * D) return Q40_E_SHAPE;
+  if (Lmax < 0 || Lmax > (1 << 29) || P < 0 || P > 0x7fffffffLL || page_size <= 0 || window < 0 || sinks < 0 || q_stride < (int64_t)H * D) return Q40_E_SHAPE;
   if (Lmax > 0 && (!page_tbl || !kpool || !vpool || P == 0 || (cache_type != CACHE_F16 && (!k_scale || !v_scale)))) return Q40_E_NULL;
   if (tbl_stride < ((int64_t)Lmax + page_size - 1) / page_size) return Q40_E_SHAPE;
   if (cache_type != CACHE_F16 && P % page_size != 0) return Q40_E_SHAPE;
@@ -445,7 +476,7 @@ extern "C" int q40_attn_pages(const void* page_tbl, int idx_bytes, int64_t tbl_s
     return Q40_E_ALIGN;
   const Plan p = plan_of(B, H, Hkv, Lmax, window, sinks);
   const int64_t parts = p.units * p.nchunks * p.heads;
-  if (parts > 0x7fffffffLL) return Q40_E_SHAPE;
+  if (parts > 0x7fffffffLL || p.nchunks > 65535) return Q40_E_SHAPE;
   if (p.nchunks > 1) {
     if (!workspace || workspace_bytes < (size_t)parts * (ATTN_D + 2) * sizeof(float)) return Q40_E_WORKSPACE;
     if (!q40_aligned(workspace, 16)) return Q40_E_ALIGN;
@@ -455,7 +486,7 @@ extern "C" int q40_attn_pages(const void* page_tbl, int idx_bytes, int64_t tbl_s
   a.tbl = {page_tbl, tbl_stride, idx_bytes == 4, page_size, page_shift_of(page_size)};
   a.seq_lens = seq_lens; a.P = P; a.last_page = P > 0 ? (int)((P - 1) / page_size) : 0; a.pages = (int)(P / page_size);
   a.B = B; a.L = Lmax; a.H = H; a.Hkv = Hkv; a.window = window; a.sinks = sinks;
-  a.groups = p.groups; a.heads = p.heads; a.chunk = p.chunk; a.nchunks = p.nchunks;
+  a.groups = p.groups; a.heads = p.heads; a.chunks_of_unit = p.chunks_of_unit; a.nchunks = p.nchunks;
   a.po = (float*)workspace; a.pml = (float2*)(a.po + parts * ATTN_D);
   a.scale_log2 = attn_scale_log2(D);
   const cudaStream_t st = (cudaStream_t)stream;

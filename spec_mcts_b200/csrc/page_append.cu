@@ -170,15 +170,14 @@ __device__ __forceinline__ uint2 recode8(uint2 c, float ratio) {
   float f[8];
   const uint32_t w[2] = {c.x, c.y};
 #pragma unroll
-  for (int j = 0; j < 8; j += 2) {
-    const uint32_t two = w[j >> 2] >> (8 * (j & 2));
+  for (int j = 0; j < 2; ++j) {
     if (T == CACHE_I8) {
-      f[j] = (float)(int8_t)two;
-      f[j + 1] = (float)(int8_t)(two >> 8);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[4 * j + i] = (float)(int8_t)(w[j] >> (8 * i));
     } else {
-      const float2 x = __half22float2(u32_as_h2(e4m3_to_h2(two & 0xffff)));
-      f[j] = x.x;
-      f[j + 1] = x.y;
+      const uint2 h = e4m3_to_h4(w[j]);
+      const float2 x = __half22float2(u32_as_h2(h.x)), y = __half22float2(u32_as_h2(h.y));
+      f[4 * j] = x.x; f[4 * j + 1] = x.y; f[4 * j + 2] = y.x; f[4 * j + 3] = y.y;
     }
   }
   return code8<T>(f, ratio);

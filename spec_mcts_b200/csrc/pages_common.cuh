@@ -38,10 +38,11 @@ static inline int page_shift_of(int page_size) {
   return s;
 }
 
-// Two e4m3 codes (bytes 0 and 1) as two halves: exact
-__device__ __forceinline__ uint32_t e4m3_to_h2(uint32_t two) {
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-  return (uint32_t)r.x | ((uint32_t)r.y << 16);
+// Four e4m3 codes as two pairs of halves: exact
+__device__ __forceinline__ uint2 e4m3_to_h4(uint32_t four) {
+  uint2 r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(r.x), "=r"(r.y) : "r"(four));
+  return r;
 }
 // Two signed bytes, which come + 128 with a byte 0x64 above each (the half 1024 + 128 + code), as two halves: exact
 __device__ __forceinline__ uint32_t i8_to_h2(uint32_t biased) {
