@@ -8,22 +8,12 @@
 // that are not finite are therefore taken out in shared memory, and added at the end to the queries that see their key: an infinity or NaN comes
 // out of a sum whatever its weight is.
 #include "attn_tile.cuh"
+#include "attn_window.cuh"
 
 namespace q40 {
 namespace window {
 
-struct Args {
-  const __half *q, *k, *v;    // position-major rows; heads side by side
-  __half* o;
-  int64_t ldq, ldk, ldv, ldo;
-  int S, H, Hkv;
-  int offset, window, sinks;
-  float scale_log2;
-};
-
 constexpr int NWARPS = 4, RB = NWARPS * 16, NT = NWARPS * 32;
-
-__device__ __forceinline__ bool not_finite(__half x) { return (__half_as_ushort(x) & 0x7c00) == 0x7c00; }
 
 __global__ void __launch_bounds__(NT)
 attn_window_kernel(const Args a) {
@@ -135,7 +125,8 @@ attn_window_kernel(const Args a) {
 }  // namespace q40
 
 extern "C" int q40_attn_causal_window(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* o,
-                                      int64_t ldo, int S, int H, int Hkv, int D, int offset, int window, int sinks, void* stream) {
+                                      int64_t ldo, int S, int H, int Hkv, int D, int offset, int window, int sinks, int* err,
+                                      void* stream) {
   using namespace q40;
   using namespace q40::window;
   if (!q || !k || !v || !o) return Q40_E_NULL;
@@ -152,6 +143,11 @@ extern "C" int q40_attn_causal_window(const void* q, int64_t ldq, const void* k,
   // positions end at offset + S: what is further back, or further on, than that sees or adds nothing more
   a.offset = offset; a.window = min(window, offset + S); a.sinks = min(sinks, offset + S);
   a.scale_log2 = attn_scale_log2(D);
+  a.wide_out = ldo % 8 == 0 && q40_aligned(o, 16);
+  if (err && S >= 256) {
+    const int rc = launch_tc(a, err, (cudaStream_t)stream);
+    if (rc != Q40_E_UNSUPPORTED) return rc;
+  }
   const size_t smem = RB * TILE_ROW_BYTES + 4 * TILE_BYTES;
   static std::atomic<uint64_t> ready;
   cudaError_t e = q40_allow_smem(ready, (const void*)attn_window_kernel, (int)smem);

@@ -1,0 +1,438 @@
+// q40_attn_causal_window's kernel for prompts with enough work: on tcgen05, 256 queries of one head a CTA.
+//
+// Two tiles of 128 queries take turns on the tensor cores: S = Q K^T of a tile of 128 keys into tensor memory, P = 2^(S - m) as fp16 over S's
+// place, O += P V with P as the A operand from tensor memory.  While the MMAs of one tile of queries run, the other's softmax does.
+//   warps 0 - 3, 4 - 7   softmax of the first and second tile of queries: a thread has a row; they write the output
+//   warp 8               issues the MMAs (one thread), in the order O += P V of a step, S of the next, tile by tile
+//   warp 9               requests tensor copies (one thread): Q, then keys and values, two stages of each
+//   warps 10, 11         look through the values that some query of a tile sees in part: see below
+// Tensor memory: S (and P) of the two tiles at columns 0 and 128, O at 256 and 384.
+//
+// A row's maximum stays while no score passes it by 8 (a weight is then at most 2^8, which fp16 holds), so that O is seldom rescaled; who
+// rescales finds no MMA of its O on the way, since S of a step is finished after O += P V of the step before.
+//
+// A masked key has a weight of 0, and 0 times a value that is not finite is no number: in tiles with masked places such values are taken out of
+// shared memory before the MMA, and added at the end to the rows that see them (as in attn_window_kernel).
+//
+// Every wait is bounded: on expiry the error word is set, what is left is skipped, the CTA's own copies and MMAs are waited for (bounded too),
+// and tensor memory is freed.
+#include <math_constants.h>
+
+#include "attn_window.cuh"
+#include "q40_tc_common.cuh"
+
+namespace q40 {
+namespace window {
+namespace tc {
+
+using ttc::elect_one;
+using ttc::mbar_arrive;
+using ttc::mbar_expect_tx;
+using ttc::mbar_init;
+using ttc::mbar_wait;
+
+constexpr int BQ = 128, BK = 128, THREADS = 384;
+constexpr uint32_t TILE = BK * ATTN_D * 2;               // 32 KB: two blocks of 64 dims, rows of 128 bytes
+constexpr uint32_t HALF = TILE / 2;
+constexpr uint32_t AT_Q = 0, AT_K = 2 * TILE, AT_V = 4 * TILE, AT_BARS = 6 * TILE;
+enum Bar { Q_FULL, K_FULL = Q_FULL + 2, K_EMPTY = K_FULL + 2, V_FULL = K_EMPTY + 2, V_READY = V_FULL + 2, V_EMPTY = V_READY + 2, S_FULL = V_EMPTY + 2,
+           P_FULL = S_FULL + 2, O_DONE = P_FULL + 2, ALL_DONE = O_DONE + 2, BARS };
+constexpr uint32_t SMEM = AT_BARS + 8 * BARS + 32 + 1024;       // (1024: the alignment)
+constexpr float STAY = 8.f;
+
+struct Maps { CUtensorMap q, k, v; };
+
+__device__ __forceinline__ void ld32(uint32_t taddr, float* x) {
+  uint32_t* const r = reinterpret_cast<uint32_t*>(x);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+      "%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+      "%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// ... of a whole warp, which goes on together or not at all
+__device__ __forceinline__ bool all_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+// D[tmem] (+)= A[smem] * B[smem]
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum) : "memory");
+}
+// The B operand [keys][dims] as it lies: dims contiguous, 64 a row of 128 swizzled bytes, blocks of 64 dims a half tile apart, groups
+// of eight keys 1024 bytes
+__device__ __forceinline__ uint64_t values_desc(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)(HALF >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(BK >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);       // fp16 in, fp32 out
+constexpr uint32_t VALUES_MAJOR = 1u << 16;                                                             // B lies dims first
+
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// What a CTA goes through, and who takes part in it
+struct Tiles {
+  int p_first, p_last;               // positions of the CTA's first and last query
+  int window, sinks, t_first, t_from, n;
+  __device__ __forceinline__ Tiles(const Args& a, int row0) {
+    p_first = a.offset + row0;
+    p_last = min(p_first + 2 * BQ, a.offset + a.S) - 1;
+    window = a.window;
+    sinks = a.sinks;
+    const int from = max(0, p_first - window + 1), first = min(sinks, from);
+    t_first = (first + BK - 1) / BK;
+    t_from = max(from / BK, t_first);
+    n = t_first + p_last / BK + 1 - t_from;
+  }
+  __device__ __forceinline__ int key0(int j) const { return (j < t_first ? j : j - t_first + t_from) * BK; }
+  // of tile i of the queries: its first position, whether it has any, sees some keys of the tile from key k, or all of them
+  __device__ __forceinline__ int first_of(int i) const { return p_first + i * BQ; }
+  __device__ __forceinline__ bool has(int i) const { return first_of(i) <= p_last; }
+  __device__ __forceinline__ bool sees(int i, int k) const {
+    return has(i) && k <= min(first_of(i) + BQ - 1, p_last) && (k + BK > first_of(i) - window + 1 || k < sinks);
+  }
+  __device__ __forceinline__ bool sees_all(int i, int k) const {
+    return k + BK <= first_of(i) + 1 && (k > min(first_of(i) + BQ - 1, p_last) - window || k + BK <= sinks);
+  }
+  __device__ __forceinline__ bool masked(int k) const { return (sees(0, k) && !sees_all(0, k)) || (sees(1, k) && !sees_all(1, k)); }
+};
+
+__global__ void __launch_bounds__(THREADS, 1)
+attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err) {
+  extern __shared__ unsigned char smem_raw[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t raw0 = ttc::smem_u32(smem_raw), base = (raw0 + 1023u) & ~1023u;
+  unsigned char* const gbase = smem_raw + (base - raw0);
+  const auto bar = [&](int which) { return base + AT_BARS + 8 * which; };
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gbase + AT_BARS + 8 * BARS);
+  volatile int* const s_failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* const s_taken_out = s_failed + 1;
+  volatile int* const s_copied = s_failed + 2;         // key and value tiles that were requested
+  const int blocks = (a.S + 2 * BQ - 1) / (2 * BQ);
+  const int blk = blocks - 1 - (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H), hk = h / (a.H / a.Hkv);
+  const int row0 = blk * 2 * BQ;
+  const Tiles tiles(a, row0);
+
+  if (tid == 0) {
+    *s_failed = 0;
+    *s_taken_out = 0;
+    s_copied[0] = s_copied[1] = 0;
+    for (int i = 0; i < BARS; ++i) {
+      const int count = i >= P_FULL && i < P_FULL + 2 ? 4 : (i >= V_READY && i < V_READY + 2) || (i >= V_EMPTY && i < V_EMPTY + 2) ? 2 : 1;
+      mbar_init(bar(i), count);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ttc::smem_u32(tmem_slot)), "n"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  bool failed = false;
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int i = warp >> 2, row = (warp & 3) * 32 + lane, p = tiles.first_of(i) + row;
+    const uint32_t quad = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + quad + 128 * i, o_at = s_at + 256;
+    float m = -3e38f, l = 0.f;
+    int n = 0;                                         // tiles of keys so far
+    for (int j = 0; j < tiles.n; ++j) {
+      const int key0 = tiles.key0(j);
+      if (!tiles.sees(i, key0)) continue;
+      if (!all_wait(bar(S_FULL + i), n & 1)) { failed = true; break; }
+      fence_after();
+      float s[BK];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) ld32(s_at + 32 * c, s + 32 * c);
+      wait_ld();
+      if (!tiles.sees_all(i, key0)) {
+        const int last = p - key0, from = p - a.window - key0, first = a.sinks - key0;      // places <= last that are > from or < first
+#pragma unroll
+        for (int c = 0; c < BK; ++c)
+          if (c > last || (c <= from && c >= first)) s[c] = -CUDART_INF_F;
+      }
+      float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int c = 4; c < BK; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+      const float most = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+      const bool passes = most > m + STAY;
+      if (__any_sync(0xffffffffu, passes)) {
+        const float now = passes ? most : m, corr = ex2(m - now);
+        m = now;
+        l *= corr;
+        if (n > 0) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float o[32];
+            ld32(o_at + 32 * c, o);
+            wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= corr;
+            st32(o_at + 32 * c, reinterpret_cast<const uint32_t*>(o));
+          }
+          wait_st();
+        }
+      }
+      const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), m2 = pack2(-m, -m);
+      uint64_t sum[2] = {pack2(l, 0.f), 0};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          float x, y;
+          unpack2(fma2(pack2(s[64 * c + 2 * e], s[64 * c + 2 * e + 1]), scale2, m2), x, y);
+          x = ex2(x);
+          y = ex2(y);
+          sum[e & 1] = add2(sum[e & 1], pack2(x, y));
+          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[e]) : "f"(y), "f"(x));
+        }
+        st32(s_at + 32 * c, pk);
+      }
+      float x, y;
+      unpack2(add2(sum[0], sum[1]), x, y);
+      l = x + y;
+      wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(P_FULL + i));
+      ++n;
+    }
+    if (!failed && tiles.has(i)) {
+      if (!all_wait(bar(O_DONE + i), 0)) failed = true;
+      fence_after();
+      if (!failed) {
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        const bool there = p <= tiles.p_last, taken_out = *s_taken_out;
+        __half* const out = a.o + (int64_t)(p - a.offset) * a.ldo + h * ATTN_D;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float o[32];
+          ld32(o_at + 32 * c, o);
+          wait_ld();
+          if (taken_out && there)                      // rare, and slow
+            for (int j = 0; j < tiles.n; ++j) {
+              const int key0 = tiles.key0(j);
+              if (!tiles.masked(key0)) continue;
+              for (int k = key0; k < min(key0 + BK, p + 1); ++k) {
+                if (p - k >= a.window && k >= a.sinks) continue;
+                const __half* const v = a.v + (int64_t)k * a.ldv + hk * ATTN_D + 32 * c;
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if (not_finite(v[e])) o[e] += __half2float(v[e]);
+              }
+            }
+          if (there) {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[e] = h2_as_u32(__floats2half2_rn(o[2 * e] * inv, o[2 * e + 1] * inv));
+            if (a.wide_out) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) reinterpret_cast<uint4*>(out + 32 * c)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) reinterpret_cast<uint32_t*>(out + 32 * c)[e] = w[e];
+            }
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 8) {
+      if (elect_one()) {
+        int pending[2] = {-1, -1}, steps[2] = {0, 0}, readied[2] = {0, 0};
+        // O += P V of tile i's step on the values of tile j
+        const auto product = [&](int i) {
+          const int j = pending[i], st = j & 1;
+          pending[i] = -1;
+          if (!mbar_wait(bar(P_FULL + i), (steps[i] - 1) & 1)) return false;
+          if (!mbar_wait(bar(V_FULL + st), (j >> 1) & 1)) return false;
+          if (tiles.masked(tiles.key0(j))) {
+            // (the second tile of queries to come here has the barrier's phase behind it; `readied` counts the phases of the stage)
+            if (!mbar_wait(bar(V_READY + st), readied[st] & 1)) return false;
+          }
+          fence_after();
+          const uint64_t b = values_desc(base + AT_V + st * TILE);
+#pragma unroll
+          for (int ks = 0; ks < BK / 16; ++ks)
+            ttc::mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * ks, b + (uint64_t)((ks * 2048) >> 4), IDESC | VALUES_MAJOR, steps[i] > 1 || ks > 0 ? 1u : 0u);
+          ttc::commit(bar(V_EMPTY + st));
+          return true;
+        };
+        // a tile's phase of V_READY is over when no product on it is pending
+        const auto finish = [&](int j) {
+          if (j >= 0 && tiles.masked(tiles.key0(j))) ++readied[j & 1];
+        };
+        bool q_there[2] = {false, false};
+        for (int j = 0; j < tiles.n && !failed; ++j) {
+          const int key0 = tiles.key0(j), st = j & 1;
+          if (!mbar_wait(bar(K_FULL + st), (j >> 1) & 1)) { failed = true; break; }
+          for (int i = 0; i < 2 && !failed; ++i) {
+            if (pending[i] >= 0 && !product(i)) { failed = true; break; }
+            if (!tiles.sees(i, key0)) {
+              // not a plain arrival: it would count for the stage's values before these while a product on them is on its way
+              ttc::commit(bar(V_EMPTY + st));
+              continue;
+            }
+            if (!q_there[i]) {
+              if (!mbar_wait(bar(Q_FULL + i), 0)) { failed = true; break; }
+              q_there[i] = true;
+            }
+            fence_after();
+            const uint64_t qd = ttc::kmajor_desc(base + AT_Q + i * TILE), kd = ttc::kmajor_desc(base + AT_K + st * TILE);
+#pragma unroll
+            for (int ks = 0; ks < ATTN_D / 16; ++ks) {
+              const uint64_t off = (uint64_t)(((ks >> 2) * HALF + (ks & 3) * 32) >> 4);
+              mma_ss(tmem + 128 * i, qd + off, kd + off, IDESC, ks > 0 ? 1u : 0u);
+            }
+            ttc::commit(bar(S_FULL + i));
+            pending[i] = j;
+            ++steps[i];
+          }
+          finish(j - 1);
+          ttc::commit(bar(K_EMPTY + st));
+        }
+        for (int i = 0; i < 2; ++i) {
+          if (!failed && pending[i] >= 0 && !product(i)) failed = true;
+          ttc::commit(bar(O_DONE + i));
+        }
+        ttc::commit(bar(ALL_DONE));
+      }
+      __syncwarp();
+    } else if (warp == 9) {
+      if (elect_one()) {
+        const auto copy = [&](const CUtensorMap* map, uint32_t dst, int head, int row, uint32_t full) {
+          mbar_expect_tx(full, TILE);
+          ttc::tma_2d(dst, map, head * ATTN_D, row, full);
+          ttc::tma_2d(dst + HALF, map, head * ATTN_D + 64, row, full);
+        };
+        for (int i = 0; i < 2; ++i)
+          if (tiles.has(i)) copy(&maps.q, base + AT_Q + i * TILE, h, row0 + i * BQ, bar(Q_FULL + i));
+        for (int j = 0; j < tiles.n; ++j) {
+          const int st = j & 1, key0 = tiles.key0(j);
+          if (j >= 2 && !mbar_wait(bar(K_EMPTY + st), ((j >> 1) - 1) & 1)) { failed = true; break; }
+          copy(&maps.k, base + AT_K + st * TILE, hk, key0, bar(K_FULL + st));
+          s_copied[0] = j + 1;
+          if (j >= 2 && !mbar_wait(bar(V_EMPTY + st), ((j >> 1) - 1) & 1)) { failed = true; break; }
+          copy(&maps.v, base + AT_V + st * TILE, hk, key0, bar(V_FULL + st));
+          s_copied[1] = j + 1;
+        }
+      }
+      __syncwarp();
+    } else {
+      const int at = (warp - 10) * 32 + lane;
+      for (int j = 0; j < tiles.n; ++j) {
+        const int st = j & 1;
+        // (for every tile: a wait tells only odd from even phases.  Of tiles that are not looked through these warps may be late, but at one that
+        // is, the MMAs are not ahead of them)
+        if (!all_wait(bar(V_FULL + st), (j >> 1) & 1)) { failed = true; break; }
+        if (!tiles.masked(tiles.key0(j))) continue;
+        uint4* const v = reinterpret_cast<uint4*>(gbase + AT_V + st * TILE);
+        bool found = false;
+#pragma unroll 8
+        for (int c = at; c < (int)TILE / 16; c += 64) {
+          const uint4 x = v[c];
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          bool here = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) here |= (w[e] & 0x7c00u) == 0x7c00u || (w[e] & 0x7c000000u) == 0x7c000000u;
+          found |= here;
+        }
+        if (__any_sync(0xffffffffu, found)) {
+          __half* const x = reinterpret_cast<__half*>(v);
+          for (int c = at; c < (int)TILE / 16; c += 64)
+            for (int e = 0; e < 8; ++e)
+              if (not_finite(x[8 * c + e])) x[8 * c + e] = __ushort_as_half(0);
+          *s_taken_out = 1;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(V_READY + st));
+      }
+    }
+  }
+  if (!mbar_wait(bar(ALL_DONE), 0) || failed) *s_failed = 1;
+  fence_before();
+  __syncthreads();
+  if (tid == 0 && *s_failed) {
+    q40_set_error(err);
+    for (int i = 0; i < 2; ++i)
+      if (tiles.has(i)) mbar_wait(bar(Q_FULL + i), 0);
+    for (int j = max(0, s_copied[0] - 2); j < s_copied[0]; ++j) mbar_wait(bar(K_FULL + (j & 1)), (j >> 1) & 1);
+    for (int j = max(0, s_copied[1] - 2); j < s_copied[1]; ++j) mbar_wait(bar(V_FULL + (j & 1)), (j >> 1) & 1);
+  }
+  __syncthreads();
+  if (warp == 8) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512));
+  }
+}
+
+}  // namespace tc
+
+int launch_tc(const Args& a, int* err, cudaStream_t st) {
+  using namespace tc;
+  EncodeTiledFn encode = ttc_encode_fn();
+  if (!encode) return Q40_E_UNSUPPORTED;
+  Maps maps;
+  const auto map = [&](CUtensorMap* m, const __half* x, int heads, int64_t rows, int64_t ld) {
+    const cuuint64_t dims[2] = {(cuuint64_t)heads * ATTN_D, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t box[2] = {64, BK}, one[2] = {1, 1};
+    return ttc_encode(encode, m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2u, (void*)x, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  const int64_t keys = (int64_t)a.offset + a.S;
+  if (map(&maps.q, a.q, a.H, a.S, a.ldq) != CUDA_SUCCESS || map(&maps.k, a.k, a.Hkv, keys, a.ldk) != CUDA_SUCCESS ||
+      map(&maps.v, a.v, a.Hkv, keys, a.ldv) != CUDA_SUCCESS)
+    return Q40_E_UNSUPPORTED;
+  static std::atomic<uint64_t> ready;
+  cudaError_t e = q40_allow_smem(ready, (const void*)attn_window_tc_kernel, (int)SMEM);
+  if (e != cudaSuccess) { (void)cudaGetLastError(); return Q40_E_UNSUPPORTED; }
+  const int64_t blocks = (int64_t)a.H * ((a.S + 2 * BQ - 1) / (2 * BQ));
+  if (blocks > 0x7fffffffLL) return Q40_E_SHAPE;
+  e = q40_launch_pdl(attn_window_tc_kernel, dim3((unsigned)blocks), dim3(THREADS), SMEM, st, a, maps, err);
+  return e == cudaSuccess ? Q40_OK : (int)e;
+}
+
+}  // namespace window
+}  // namespace q40

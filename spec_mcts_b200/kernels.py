@@ -473,7 +473,7 @@ def _tc_error_page(dev, st) -> torch.Tensor:
 
 
 def tc_error_flag(dev=None) -> int:
-    """1 if a tensor-core matmul launched through matmul_q40, linear_q40 or a prompt pass on the current stream of `dev` gave up
+    """1 if a tensor-core matmul launched through matmul_q40, linear_q40 or a prompt pass, or causal_attn with a window, on the current stream of `dev` gave up
     on one of its bounded waits since the workspace was created (synchronises the device).  Not reported: matmuls
     captured on a stream on which no call that needs a workspace was made outside of a capture before."""
     dev = _indexed(dev)
@@ -599,10 +599,11 @@ def causal_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional
     if windowed:
         whole = offset + S
         # (the stride of a dimension of one may be anything)
+        st = _stream(dev)
+        err = _tc_error_page(dev, st).data_ptr() + 4092
         lds = [t.stride(0) if t.shape[0] > 1 else t.shape[1] * D for t in (q, k, v, out)]
         check(lib.q40_attn_causal_window(q.data_ptr(), lds[0], k.data_ptr(), lds[1], v.data_ptr(), lds[2], out.data_ptr(), lds[3], S, H, Hkv, D,
-                                         offset, whole if window is None else min(window, max(whole, 1)), min(sinks, whole), _stream(dev)),
-              "q40_attn_causal_window")
+                                         offset, whole if window is None else min(window, max(whole, 1)), min(sinks, whole), err, st), "q40_attn_causal_window")
         return out
     check(lib.q40_attn_causal(q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
                               out.data_ptr(), out.stride(0), S, H, Hkv, D, _stream(dev)), "q40_attn_causal")

@@ -211,12 +211,14 @@ def check_prompt(got, want, size, v):
 
 @pytest.mark.parametrize("s,h,hkv,window,sinks,offset", [(1, 4, 4, 1, 0, 0), (1, 4, 2, 5, 2, 100), (16, 2, 1, 16, 0, 0), (63, 4, 2, 10, 1, 0), (64, 4, 2, 64, 64, 1), (65, 4, 1, 1, 0, 63),
                                                          (130, 8, 2, 40, 70, 200), (200, 2, 2, 1000, 5, 0), (200, 2, 2, 1000, 5, 777), (129, 3, 3, 128, 0, 128), (300, 4, 4, 65, 130, 450),
-                                                         (77, 32, 8, 50, 4, 0), (257, 8, 1, 200, 4, 1000), (513, 16, 2, 1, 3, 0), (700, 5, 1, 333, 1000, 90)])
+                                                         (77, 32, 8, 50, 4, 0), (257, 8, 1, 200, 4, 1000), (513, 16, 2, 1, 3, 0), (700, 5, 1, 333, 1000, 90),
+                                                         (1000, 4, 2, 129, 0, 300), (1500, 2, 2, 700, 200, 31), (2049, 1, 1, 1, 1, 0), (1280, 2, 1, 10000, 0, 2000), (999, 2, 1, 128, 300, 129)])
 def test_prompt(K, s, h, hkv, window, sinks, offset):
     g = generator(s + h)
     q, k, v = normal(g, s, h, D), normal(g, offset + s + 3, hkv, D), normal(g, offset + s + 3, hkv, D)
     k[offset + s:], v[offset + s:] = math.nan, math.nan                  # rows behind the last position
     got = K.causal_attn(q, k, v, window=window, sinks=sinks, offset=offset)
+    assert K.tc_error_flag() == 0
     check_prompt(got, *prompt_reference(q, k, v, window, sinks, offset), v)
 
 

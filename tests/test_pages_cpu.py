@@ -19,8 +19,8 @@ def append(tbl=A, idx=4, tstride=8, width=8, pos=A, off=None, q=A, qs=512, qo=A,
     return lib.q40_page_append(tbl, idx, tstride, width, pos, off, q, qs, qo, k, kst, v, vst, cos, sin, n_pos, kp, vp, ks, vs, kind, P, B, T, H, Hkv, D, ps, None)
 
 
-def window(q=A, ldq=512, k=A, ldk=256, v=A, ldv=256, o=A, ldo=512, S=4, H=4, Hkv=2, D=128, off=0, w=3, s=0):
-    return lib.q40_attn_causal_window(q, ldq, k, ldk, v, ldv, o, ldo, S, H, Hkv, D, off, w, s, None)
+def window(q=A, ldq=512, k=A, ldk=256, v=A, ldv=256, o=A, ldo=512, S=4, H=4, Hkv=2, D=128, off=0, w=3, s=0, err=A):
+    return lib.q40_attn_causal_window(q, ldq, k, ldk, v, ldv, o, ldo, S, H, Hkv, D, off, w, s, err, None)
 
 
 @pytest.mark.parametrize("status,bad", [(NULL, dict(q=None)), (NULL, dict(tbl=None)), (NULL, dict(ks=None)), (NULL, dict(P=0)), (SHAPE, dict(H=5)), (SHAPE, dict(tstride=7)), (SHAPE, dict(P=100)),
