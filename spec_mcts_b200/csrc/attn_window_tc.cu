@@ -36,7 +36,7 @@ constexpr uint32_t TILE = BK * ATTN_D * 2;               // 32 KB: two blocks of
 constexpr uint32_t HALF = TILE / 2;
 constexpr uint32_t AT_Q = 0, AT_K = 2 * TILE, AT_V = 4 * TILE, AT_BARS = 6 * TILE;
 enum Bar { Q_FULL, K_FULL = Q_FULL + 2, K_EMPTY = K_FULL + 2, V_FULL = K_EMPTY + 2, V_READY = V_FULL + 2, V_EMPTY = V_READY + 2, S_FULL = V_EMPTY + 2,
-           P_FULL = S_FULL + 2, O_DONE = P_FULL + 2, ALL_DONE = O_DONE + 2, BARS };
+           P_HALF = S_FULL + 2, P_FULL = P_HALF + 2, O_DONE = P_FULL + 2, ALL_DONE = O_DONE + 2, BARS };
 constexpr uint32_t SMEM = AT_BARS + 8 * BARS + 32 + 1024;       // (1024: the alignment)
 constexpr float STAY = 8.f;
 
@@ -103,6 +103,9 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// The lowest n bits, of any n
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+
 // What a CTA goes through, and who takes part in it
 struct Tiles {
   int p_first, p_last;               // positions of the CTA's first and last query
@@ -151,11 +154,15 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
     *s_taken_out = 0;
     s_copied[0] = s_copied[1] = 0;
     for (int i = 0; i < BARS; ++i) {
-      const int count = i >= P_FULL && i < P_FULL + 2 ? 4 : (i >= V_READY && i < V_READY + 2) || (i >= V_EMPTY && i < V_EMPTY + 2) ? 2 : 1;
+      const int count = i >= P_HALF && i < P_FULL + 2 ? 4 : (i >= V_READY && i < V_READY + 2) || (i >= V_EMPTY && i < V_EMPTY + 2) ? 2 : 1;
       mbar_init(bar(i), count);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 9 && lane < 3) {
+    const CUtensorMap* const map = lane == 0 ? &maps.q : lane == 1 ? &maps.k : &maps.v;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
   }
   if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ttc::smem_u32(tmem_slot)), "n"(512));
@@ -185,10 +192,14 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
       for (int c = 0; c < 4; ++c) ld32(s_at + 32 * c, s + 32 * c);
       wait_ld();
       if (!tiles.sees_all(i, key0)) {
-        const int last = p - key0, from = p - a.window - key0, first = a.sinks - key0;      // places <= last that are > from or < first
+        const int last = p - key0, from = p - a.window - key0, first = a.sinks - key0;      // seen: places <= last that are > from or < first
 #pragma unroll
-        for (int c = 0; c < BK; ++c)
-          if (c > last || (c <= from && c >= first)) s[c] = -CUDART_INF_F;
+        for (int c = 0; c < BK; c += 32) {
+          const uint32_t seen = below(last + 1 - c) & (~below(from + 1 - c) | below(first - c));
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!(seen & (1u << e))) s[c + e] = -CUDART_INF_F;
+        }
       }
       float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -227,14 +238,14 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
           asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[e]) : "f"(y), "f"(x));
         }
         st32(s_at + 32 * c, pk);
+        wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar((c ? P_FULL : P_HALF) + i));
       }
       float x, y;
       unpack2(add2(sum[0], sum[1]), x, y);
       l = x + y;
-      wait_st();
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(P_FULL + i));
       ++n;
     }
     if (!failed && tiles.has(i)) {
@@ -285,7 +296,7 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
         const auto product = [&](int i) {
           const int j = pending[i], st = j & 1;
           pending[i] = -1;
-          if (!mbar_wait(bar(P_FULL + i), (steps[i] - 1) & 1)) return false;
+          if (!mbar_wait(bar(P_HALF + i), (steps[i] - 1) & 1)) return false;
           if (!mbar_wait(bar(V_FULL + st), (j >> 1) & 1)) return false;
           if (tiles.masked(tiles.key0(j))) {
             // (the second tile of queries to come here has the barrier's phase behind it; `readied` counts the phases of the stage)
@@ -294,8 +305,13 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
           fence_after();
           const uint64_t b = values_desc(base + AT_V + st * TILE);
 #pragma unroll
-          for (int ks = 0; ks < BK / 16; ++ks)
+          for (int ks = 0; ks < BK / 32; ++ks)
             ttc::mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * ks, b + (uint64_t)((ks * 2048) >> 4), IDESC | VALUES_MAJOR, steps[i] > 1 || ks > 0 ? 1u : 0u);
+          if (!mbar_wait(bar(P_FULL + i), (steps[i] - 1) & 1)) return false;
+          fence_after();
+#pragma unroll
+          for (int ks = BK / 32; ks < BK / 16; ++ks)
+            ttc::mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * ks, b + (uint64_t)((ks * 2048) >> 4), IDESC | VALUES_MAJOR, 1u);
           ttc::commit(bar(V_EMPTY + st));
           return true;
         };
@@ -346,13 +362,13 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
           ttc::tma_2d(dst, map, head * ATTN_D, row, full);
           ttc::tma_2d(dst + HALF, map, head * ATTN_D + 64, row, full);
         };
-        for (int i = 0; i < 2; ++i)
-          if (tiles.has(i)) copy(&maps.q, base + AT_Q + i * TILE, h, row0 + i * BQ, bar(Q_FULL + i));
+        copy(&maps.q, base + AT_Q, h, row0, bar(Q_FULL));
         for (int j = 0; j < tiles.n; ++j) {
           const int st = j & 1, key0 = tiles.key0(j);
           if (j >= 2 && !mbar_wait(bar(K_EMPTY + st), ((j >> 1) - 1) & 1)) { failed = true; break; }
           copy(&maps.k, base + AT_K + st * TILE, hk, key0, bar(K_FULL + st));
           s_copied[0] = j + 1;
+          if (j == 0 && tiles.has(1)) copy(&maps.q, base + AT_Q + TILE, h, row0 + BQ, bar(Q_FULL + 1));
           if (j >= 2 && !mbar_wait(bar(V_EMPTY + st), ((j >> 1) - 1) & 1)) { failed = true; break; }
           copy(&maps.v, base + AT_V + st * TILE, hk, key0, bar(V_FULL + st));
           s_copied[1] = j + 1;
@@ -368,16 +384,15 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
         if (!all_wait(bar(V_FULL + st), (j >> 1) & 1)) { failed = true; break; }
         if (!tiles.masked(tiles.key0(j))) continue;
         uint4* const v = reinterpret_cast<uint4*>(gbase + AT_V + st * TILE);
-        bool found = false;
+        __half2 most[2] = {u32_as_h2(0), u32_as_h2(0)};              // magnitudes; what is not finite is above all that is, or stays
 #pragma unroll 8
         for (int c = at; c < (int)TILE / 16; c += 64) {
           const uint4 x = v[c];
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-          bool here = false;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) here |= (w[e] & 0x7c00u) == 0x7c00u || (w[e] & 0x7c000000u) == 0x7c000000u;
-          found |= here;
+          most[0] = __hmax2_nan(__hmax2_nan(most[0], __habs2(u32_as_h2(x.x))), __habs2(u32_as_h2(x.y)));
+          most[1] = __hmax2_nan(__hmax2_nan(most[1], __habs2(u32_as_h2(x.z))), __habs2(u32_as_h2(x.w)));
         }
+        const __half2 top = __hmax2_nan(most[0], most[1]);
+        const bool found = not_finite(__low2half(top)) || not_finite(__high2half(top));
         if (__any_sync(0xffffffffu, found)) {
           __half* const x = reinterpret_cast<__half*>(v);
           for (int c = at; c < (int)TILE / 16; c += 64)
