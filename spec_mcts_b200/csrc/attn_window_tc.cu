@@ -4,7 +4,7 @@
 // place, O += P V with P as the A operand from tensor memory.  While the MMAs of one tile of queries run, the other's softmax does.
 //   warps 0 - 3, 4 - 7   softmax of the first and second tile of queries: a thread has a row; they write the output
 //   warp 8               issues the MMAs (one thread), in the order O += P V of a step, S of the next, tile by tile
-//   warp 9               requests tensor copies (one thread): Q, then keys and values, two stages of each
+//   warp 9               requests tensor copies (one thread): Q, then keys and values in turn through a ring of five tiles
 //   warps 10, 11         look through the values that some query of a tile sees in part: see below
 // Tensor memory: S (and P) of the two tiles at columns 0 and 128, O at 256 and 384.
 //
@@ -34,10 +34,12 @@ using ttc::mbar_wait;
 constexpr int BQ = 128, BK = 128, THREADS = 384;
 constexpr uint32_t TILE = BK * ATTN_D * 2;               // 32 KB: two blocks of 64 dims, rows of 128 bytes
 constexpr uint32_t HALF = TILE / 2;
-constexpr uint32_t AT_Q = 0, AT_K = 2 * TILE, AT_V = 4 * TILE, AT_BARS = 6 * TILE;
-enum Bar { Q_FULL, K_FULL = Q_FULL + 2, K_EMPTY = K_FULL + 2, V_FULL = K_EMPTY + 2, V_READY = V_FULL + 2, V_EMPTY = V_READY + 2, S_FULL = V_EMPTY + 2,
+constexpr int SLOTS = 5;                        // of the ring that keys and values go through in turn
+constexpr int LOOKED = 4;                       // barriers of values that are looked through: at most three of them are in the ring
+constexpr uint32_t AT_Q = 0, AT_RING = 2 * TILE, AT_BARS = AT_RING + SLOTS * TILE;
+enum Bar { Q_FULL, FULL = Q_FULL + 2, EMPTY = FULL + SLOTS, LOOK = EMPTY + SLOTS, READY = LOOK + LOOKED, S_FULL = READY + LOOKED,
            P_HALF = S_FULL + 2, P_FULL = P_HALF + 2, O_DONE = P_FULL + 2, ALL_DONE = O_DONE + 2, BARS };
-constexpr uint32_t SMEM = AT_BARS + 8 * BARS + 32 + 1024;       // (1024: the alignment)
+constexpr uint32_t SMEM = AT_BARS + 8 * BARS + 48 + 1024;       // (1024: the alignment)
 constexpr float STAY = 8.f;
 
 struct Maps { CUtensorMap q, k, v; };
@@ -143,7 +145,7 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gbase + AT_BARS + 8 * BARS);
   volatile int* const s_failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* const s_taken_out = s_failed + 1;
-  volatile int* const s_copied = s_failed + 2;         // key and value tiles that were requested
+  volatile uint32_t* const s_requested = tmem_slot + 3;          // of each slot: the barrier of its last copy, and 1 + the phase
   const int blocks = (a.S + 2 * BQ - 1) / (2 * BQ);
   const int blk = blocks - 1 - (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H), hk = h / (a.H / a.Hkv);
   const int row0 = blk * 2 * BQ;
@@ -152,9 +154,9 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
   if (tid == 0) {
     *s_failed = 0;
     *s_taken_out = 0;
-    s_copied[0] = s_copied[1] = 0;
+    for (int i = 0; i < SLOTS; ++i) s_requested[i] = 0;
     for (int i = 0; i < BARS; ++i) {
-      const int count = i >= P_HALF && i < P_FULL + 2 ? 4 : (i >= V_READY && i < V_READY + 2) || (i >= V_EMPTY && i < V_EMPTY + 2) ? 2 : 1;
+      const int count = i >= P_HALF && i < P_FULL + 2 ? 4 : (i >= READY && i < READY + LOOKED) || (i >= EMPTY && i < EMPTY + SLOTS) ? 2 : 1;
       mbar_init(bar(i), count);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -291,19 +293,21 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8) {
       if (elect_one()) {
-        int pending[2] = {-1, -1}, steps[2] = {0, 0}, readied[2] = {0, 0};
-        // O += P V of tile i's step on the values of tile j
+        bool pending[2] = {false, false}, q_there[2] = {false, false};      // O += P V of the tile before is still to come
+        int steps[2] = {0, 0}, slot = 0, looked = 0, v_slot = 0;
+        bool v_masked = false;                         // ... whose values are in v_slot, the looked-th to be looked through
+        uint32_t phases = 0;                           // of FULL, a bit a slot
+        const auto full = [&](int at) { return mbar_wait(bar(FULL + at), (phases >> at) & 1); };
         const auto product = [&](int i) {
-          const int j = pending[i], st = j & 1;
-          pending[i] = -1;
+          pending[i] = false;
           if (!mbar_wait(bar(P_HALF + i), (steps[i] - 1) & 1)) return false;
-          if (!mbar_wait(bar(V_FULL + st), (j >> 1) & 1)) return false;
-          if (tiles.masked(tiles.key0(j))) {
-            // (the second tile of queries to come here has the barrier's phase behind it; `readied` counts the phases of the stage)
-            if (!mbar_wait(bar(V_READY + st), readied[st] & 1)) return false;
+          if (v_masked) {
+            if (!mbar_wait(bar(LOOK + looked % LOOKED), (looked / LOOKED) & 1) || !mbar_wait(bar(READY + looked % LOOKED), (looked / LOOKED) & 1)) return false;
+          } else if (!full(v_slot)) {
+            return false;
           }
           fence_after();
-          const uint64_t b = values_desc(base + AT_V + st * TILE);
+          const uint64_t b = values_desc(base + AT_RING + v_slot * TILE);
 #pragma unroll
           for (int ks = 0; ks < BK / 32; ++ks)
             ttc::mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * ks, b + (uint64_t)((ks * 2048) >> 4), IDESC | VALUES_MAJOR, steps[i] > 1 || ks > 0 ? 1u : 0u);
@@ -312,44 +316,44 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
 #pragma unroll
           for (int ks = BK / 32; ks < BK / 16; ++ks)
             ttc::mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * ks, b + (uint64_t)((ks * 2048) >> 4), IDESC | VALUES_MAJOR, 1u);
-          ttc::commit(bar(V_EMPTY + st));
+          ttc::commit(bar(EMPTY + v_slot));
           return true;
         };
-        // a tile's phase of V_READY is over when no product on it is pending
-        const auto finish = [&](int j) {
-          if (j >= 0 && tiles.masked(tiles.key0(j))) ++readied[j & 1];
-        };
-        bool q_there[2] = {false, false};
         for (int j = 0; j < tiles.n && !failed; ++j) {
-          const int key0 = tiles.key0(j), st = j & 1;
-          if (!mbar_wait(bar(K_FULL + st), (j >> 1) & 1)) { failed = true; break; }
+          const int key0 = tiles.key0(j), next = slot + 1 == SLOTS ? 0 : slot + 1;       // keys in `slot`, values in the next
+          if (!full(slot)) { failed = true; break; }
           for (int i = 0; i < 2 && !failed; ++i) {
-            if (pending[i] >= 0 && !product(i)) { failed = true; break; }
-            if (!tiles.sees(i, key0)) {
-              // not a plain arrival: it would count for the stage's values before these while a product on them is on its way
-              ttc::commit(bar(V_EMPTY + st));
-              continue;
-            }
-            if (!q_there[i]) {
-              if (!mbar_wait(bar(Q_FULL + i), 0)) { failed = true; break; }
-              q_there[i] = true;
-            }
-            fence_after();
-            const uint64_t qd = ttc::kmajor_desc(base + AT_Q + i * TILE), kd = ttc::kmajor_desc(base + AT_K + st * TILE);
+            if (pending[i] && !product(i)) { failed = true; break; }
+            if (tiles.sees(i, key0)) {
+              if (!q_there[i]) {
+                if (!mbar_wait(bar(Q_FULL + i), 0)) { failed = true; break; }
+                q_there[i] = true;
+              }
+              fence_after();
+              const uint64_t qd = ttc::kmajor_desc(base + AT_Q + i * TILE), kd = ttc::kmajor_desc(base + AT_RING + slot * TILE);
 #pragma unroll
-            for (int ks = 0; ks < ATTN_D / 16; ++ks) {
-              const uint64_t off = (uint64_t)(((ks >> 2) * HALF + (ks & 3) * 32) >> 4);
-              mma_ss(tmem + 128 * i, qd + off, kd + off, IDESC, ks > 0 ? 1u : 0u);
+              for (int ks = 0; ks < ATTN_D / 16; ++ks) {
+                const uint64_t off = (uint64_t)(((ks >> 2) * HALF + (ks & 3) * 32) >> 4);
+                mma_ss(tmem + 128 * i, qd + off, kd + off, IDESC, ks > 0 ? 1u : 0u);
+              }
+              ttc::commit(bar(S_FULL + i));
+              pending[i] = true;
+              ++steps[i];
+            } else {
+              // not a plain arrival: it would count for what was in the slot before while a product on that is on its way
+              ttc::commit(bar(EMPTY + next));
             }
-            ttc::commit(bar(S_FULL + i));
-            pending[i] = j;
-            ++steps[i];
+            ttc::commit(bar(EMPTY + slot));
           }
-          finish(j - 1);
-          ttc::commit(bar(K_EMPTY + st));
+          if (v_masked) ++looked;
+          else if (j > 0) phases ^= 1u << v_slot;
+          phases ^= 1u << slot;
+          v_slot = next;
+          v_masked = tiles.masked(key0);
+          slot = next + 1 == SLOTS ? 0 : next + 1;
         }
         for (int i = 0; i < 2; ++i) {
-          if (!failed && pending[i] >= 0 && !product(i)) failed = true;
+          if (!failed && pending[i] && !product(i)) failed = true;
           ttc::commit(bar(O_DONE + i));
         }
         ttc::commit(bar(ALL_DONE));
@@ -363,27 +367,31 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
           ttc::tma_2d(dst + HALF, map, head * ATTN_D + 64, row, full);
         };
         copy(&maps.q, base + AT_Q, h, row0, bar(Q_FULL));
-        for (int j = 0; j < tiles.n; ++j) {
-          const int st = j & 1, key0 = tiles.key0(j);
-          if (j >= 2 && !mbar_wait(bar(K_EMPTY + st), ((j >> 1) - 1) & 1)) { failed = true; break; }
-          copy(&maps.k, base + AT_K + st * TILE, hk, key0, bar(K_FULL + st));
-          s_copied[0] = j + 1;
-          if (j == 0 && tiles.has(1)) copy(&maps.q, base + AT_Q + TILE, h, row0 + BQ, bar(Q_FULL + 1));
-          if (j >= 2 && !mbar_wait(bar(V_EMPTY + st), ((j >> 1) - 1) & 1)) { failed = true; break; }
-          copy(&maps.v, base + AT_V + st * TILE, hk, key0, bar(V_FULL + st));
-          s_copied[1] = j + 1;
+        int slot = 0, looked = 0;
+        uint32_t full = 0;                             // phases of FULL, a bit a slot
+        for (int x = 0; x < 2 * tiles.n; ++x) {        // keys of tile x / 2, or its values
+          const int key0 = tiles.key0(x >> 1);
+          if (x >= SLOTS && !mbar_wait(bar(EMPTY + slot), (x / SLOTS - 1) & 1)) { failed = true; break; }
+          const bool look = (x & 1) && tiles.masked(key0);
+          const int which = look ? LOOK + looked % LOOKED : FULL + slot;
+          s_requested[slot] = 2 * which + 1 + (look ? (looked / LOOKED) & 1 : (full >> slot) & 1);
+          copy(x & 1 ? &maps.v : &maps.k, base + AT_RING + slot * TILE, hk, key0, bar(which));
+          if (look) ++looked;
+          else full ^= 1u << slot;
+          if (x == 0 && tiles.has(1)) copy(&maps.q, base + AT_Q + TILE, h, row0 + BQ, bar(Q_FULL + 1));
+          if (++slot == SLOTS) slot = 0;
         }
       }
       __syncwarp();
     } else {
       const int at = (warp - 10) * 32 + lane;
+      int looked = 0;
       for (int j = 0; j < tiles.n; ++j) {
-        const int st = j & 1;
-        // (for every tile: a wait tells only odd from even phases.  Of tiles that are not looked through these warps may be late, but at one that
-        // is, the MMAs are not ahead of them)
-        if (!all_wait(bar(V_FULL + st), (j >> 1) & 1)) { failed = true; break; }
         if (!tiles.masked(tiles.key0(j))) continue;
-        uint4* const v = reinterpret_cast<uint4*>(gbase + AT_V + st * TILE);
+        const int which = looked % LOOKED;
+        if (!all_wait(bar(LOOK + which), (looked / LOOKED) & 1)) { failed = true; break; }
+        ++looked;
+        uint4* const v = reinterpret_cast<uint4*>(gbase + AT_RING + (2 * j + 1) % SLOTS * TILE);
         __half2 most[2] = {u32_as_h2(0), u32_as_h2(0)};              // magnitudes; what is not finite is above all that is, or stays
 #pragma unroll 8
         for (int c = at; c < (int)TILE / 16; c += 64) {
@@ -402,7 +410,7 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(V_READY + st));
+        if (lane == 0) mbar_arrive(bar(READY + which));
       }
     }
   }
@@ -413,8 +421,8 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
     q40_set_error(err);
     for (int i = 0; i < 2; ++i)
       if (tiles.has(i)) mbar_wait(bar(Q_FULL + i), 0);
-    for (int j = max(0, s_copied[0] - 2); j < s_copied[0]; ++j) mbar_wait(bar(K_FULL + (j & 1)), (j >> 1) & 1);
-    for (int j = max(0, s_copied[1] - 2); j < s_copied[1]; ++j) mbar_wait(bar(V_FULL + (j & 1)), (j >> 1) & 1);
+    for (int i = 0; i < SLOTS; ++i)
+      if (const uint32_t r = s_requested[i]) mbar_wait(bar((int)(r - 1) >> 1), (r - 1) & 1);
   }
   __syncthreads();
   if (warp == 8) {
