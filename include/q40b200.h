@@ -473,9 +473,13 @@ int q40_attn_causal(const void* q, int64_t ldq, const void* k, int64_t ldk, cons
 
 /* q40_attn_causal for a prompt's positions offset .. offset + S - 1, whose keys and values are rows 0 .. offset + S - 1 of k and v, with a
  * window: the query at position p attends the keys j <= p with p - j < window or j < sinks.  offset + S <= 2^30.
- * `err` is a device int that a kernel on tcgen05, for longer prompts, sets to 1 if one of its bounded waits expires (NULL: that kernel is not used). */
+ * `err` is a device int that a kernel on tcgen05, for longer prompts, sets to 1 if one of its bounded waits expires (NULL: that kernel is not used).
+ * With *_workspace_bytes bytes of workspace (16-byte aligned, no initialisation; calls that may overlap need one each) CTAs share the keys where
+ * queries are few; without (NULL) they do not. */
+size_t q40_attn_causal_window_workspace_bytes(int S, int H, int Hkv, int D, int offset, int window, int sinks);
 int q40_attn_causal_window(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* o, int64_t ldo,
-                           int S, int H, int Hkv, int D, int offset, int window, int sinks, int* err, void* stream);
+                           int S, int H, int Hkv, int D, int offset, int window, int sinks, void* workspace, size_t workspace_bytes, int* err,
+                           void* stream);
 
 /* The layers of a prompt pass, enqueued by one call: per layer q40_rmsnorm (adding the previous layer's output), q40_gemm_tiled_tc_multi
  * for wq, wk and wv (keys and values into the prompt cache), q40_rope_qk, q40_attn_causal, wo, q40_rmsnorm, q40_gemm_tiled_tc_ws with the SiLU

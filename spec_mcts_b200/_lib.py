@@ -48,7 +48,8 @@ SIGNATURES = {
     "q40_gemm_kn_tc_multi": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                      c_int, c_int, c_void_p, c_int, c_void_p]),
     "q40_attn_causal_window": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64] + [c_int] * 7 +
-                               [c_void_p, c_void_p]),
+                               [c_void_p, c_size_t, c_void_p, c_void_p]),
+    "q40_attn_causal_window_workspace_bytes": (c_size_t, [c_int] * 7),
     "q40_attn_causal": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int,
                                 c_int, c_int, c_int, c_void_p]),
     "q40_tp_layout": (c_int, [c_int, c_int, c_int, c_void_p]),

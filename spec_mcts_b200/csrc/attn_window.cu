@@ -124,29 +124,66 @@ attn_window_kernel(const Args a) {
 }  // namespace window
 }  // namespace q40
 
+namespace q40 {
+namespace window {
+
+static Args args_of(int S, int H, int Hkv, int offset, int window, int sinks) {
+  Args a{};
+  a.S = S; a.H = H; a.Hkv = Hkv;
+  // positions end at offset + S: what is further back, or further on, than that sees or adds nothing more
+  a.offset = offset; a.window = min(window, offset + S); a.sinks = min(sinks, offset + S);
+  a.scale_log2 = attn_scale_log2(ATTN_D);
+  a.splits = 1;
+  return a;
+}
+// Whether the kernel on tcgen05 takes the call
+static bool wide(const Args& a) { return a.S > 64 || min(a.offset, a.window - 1) + a.S + a.sinks > 128; }
+static bool fits(int S, int H, int Hkv, int D, int offset, int window, int sinks) {
+  return S >= 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && offset >= 0 && window > 0 && sinks >= 0 && (int64_t)S + offset <= (1 << 30) && D == ATTN_D;
+}
+static size_t part_bytes(const Args& a) { return (size_t)a.splits * a.S * a.H * (ATTN_D + 2) * sizeof(float); }
+
+}  // namespace window
+}  // namespace q40
+
+extern "C" size_t q40_attn_causal_window_workspace_bytes(int S, int H, int Hkv, int D, int offset, int window, int sinks) {
+  using namespace q40::window;
+  if (!fits(S, H, Hkv, D, offset, window, sinks) || S == 0) return 0;
+  Args a = args_of(S, H, Hkv, offset, window, sinks);
+  if (!wide(a)) return 0;
+  a.splits = splits_tc(a);
+  return a.splits == 1 ? 0 : part_bytes(a);
+}
+
 extern "C" int q40_attn_causal_window(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* o,
-                                      int64_t ldo, int S, int H, int Hkv, int D, int offset, int window, int sinks, int* err,
-                                      void* stream) {
+                                      int64_t ldo, int S, int H, int Hkv, int D, int offset, int window, int sinks, void* workspace,
+                                      size_t workspace_bytes, int* err, void* stream) {
   using namespace q40;
   using namespace q40::window;
   if (!q || !k || !v || !o) return Q40_E_NULL;
   if (D != ATTN_D) return Q40_E_UNSUPPORTED;
-  if (S < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || offset < 0 || window <= 0 || sinks < 0) return Q40_E_SHAPE;
-  if ((int64_t)S + offset > (1 << 30)) return Q40_E_SHAPE;
+  if (!fits(S, H, Hkv, D, offset, window, sinks)) return Q40_E_SHAPE;
   if (ldq < (int64_t)H * D || ldo < (int64_t)H * D || ldk < (int64_t)Hkv * D || ldv < (int64_t)Hkv * D) return Q40_E_SHAPE;
   if (ldq % 8 != 0 || ldk % 8 != 0 || ldv % 8 != 0 || ldo % 2 != 0) return Q40_E_ALIGN;
   if (!q40_aligned(q, 16) || !q40_aligned(k, 16) || !q40_aligned(v, 16) || !q40_aligned(o, 4)) return Q40_E_ALIGN;
   if (S == 0) return Q40_OK;
-  Args a{};
+  Args a = args_of(S, H, Hkv, offset, window, sinks);
   a.q = (const __half*)q; a.k = (const __half*)k; a.v = (const __half*)v; a.o = (__half*)o;
-  a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo; a.S = S; a.H = H; a.Hkv = Hkv;
-  // positions end at offset + S: what is further back, or further on, than that sees or adds nothing more
-  a.offset = offset; a.window = min(window, offset + S); a.sinks = min(sinks, offset + S);
-  a.scale_log2 = attn_scale_log2(D);
+  a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo;
   a.wide_out = ldo % 8 == 0 && q40_aligned(o, 16);
-  if (err && S >= 256) {
+  if (err && wide(a)) {
+    if (!q40_aligned(err, 4)) return Q40_E_ALIGN;
+    const int splits = splits_tc(a);
+    if (splits > 1 && workspace) {
+      a.splits = splits;
+      if (workspace_bytes < part_bytes(a)) return Q40_E_WORKSPACE;
+      if (!q40_aligned(workspace, 16)) return Q40_E_ALIGN;
+      a.po = (float*)workspace;
+      a.pml = (float2*)(a.po + (size_t)splits * S * H * ATTN_D);
+    }
     const int rc = launch_tc(a, err, (cudaStream_t)stream);
     if (rc != Q40_E_UNSUPPORTED) return rc;
+    a.splits = 1;
   }
   const size_t smem = RB * TILE_ROW_BYTES + 4 * TILE_BYTES;
   static std::atomic<uint64_t> ready;

@@ -18,6 +18,8 @@
 // and tensor memory is freed.
 #include <math_constants.h>
 
+#include <algorithm>
+
 #include "attn_window.cuh"
 #include "q40_tc_common.cuh"
 
@@ -111,18 +113,21 @@ __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0
 // What a CTA goes through, and who takes part in it
 struct Tiles {
   int p_first, p_last;               // positions of the CTA's first and last query
-  int window, sinks, t_first, t_from, n;
-  __device__ __forceinline__ Tiles(const Args& a, int row0) {
+  int window, sinks, t_first, t_from;
+  int j0, n;                         // this CTA's tiles of the block's
+  __host__ __device__ __forceinline__ Tiles(const Args& a, int row0, int split) {
     p_first = a.offset + row0;
-    p_last = min(p_first + 2 * BQ, a.offset + a.S) - 1;
+    p_last = (p_first + 2 * BQ < a.offset + a.S ? p_first + 2 * BQ : a.offset + a.S) - 1;
     window = a.window;
     sinks = a.sinks;
-    const int from = max(0, p_first - window + 1), first = min(sinks, from);
+    const int from = p_first - window + 1 > 0 ? p_first - window + 1 : 0, first = sinks < from ? sinks : from;
     t_first = (first + BK - 1) / BK;
-    t_from = max(from / BK, t_first);
-    n = t_first + p_last / BK + 1 - t_from;
+    t_from = from / BK > t_first ? from / BK : t_first;
+    const int all = t_first + p_last / BK + 1 - t_from;
+    j0 = (int)((int64_t)all * split / a.splits);
+    n = (int)((int64_t)all * (split + 1) / a.splits) - j0;
   }
-  __device__ __forceinline__ int key0(int j) const { return (j < t_first ? j : j - t_first + t_from) * BK; }
+  __device__ __forceinline__ int key0(int j) const { return (j + j0 < t_first ? j + j0 : j + j0 - t_first + t_from) * BK; }
   // of tile i of the queries: its first position, whether it has any, sees some keys of the tile from key k, or all of them
   __device__ __forceinline__ int first_of(int i) const { return p_first + i * BQ; }
   __device__ __forceinline__ bool has(int i) const { return first_of(i) <= p_last; }
@@ -149,7 +154,7 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
   const int blocks = (a.S + 2 * BQ - 1) / (2 * BQ);
   const int blk = blocks - 1 - (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H), hk = h / (a.H / a.Hkv);
   const int row0 = blk * 2 * BQ;
-  const Tiles tiles(a, row0);
+  const Tiles tiles(a, row0, blockIdx.y);
 
   if (tid == 0) {
     *s_failed = 0;
@@ -256,12 +261,18 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
       if (!failed) {
         const float inv = l != 0.f ? 1.f / l : 0.f;
         const bool there = p <= tiles.p_last, taken_out = *s_taken_out;
+        // (rows by way of shared memory, 256 bytes of one at a time: no faster)
         __half* const out = a.o + (int64_t)(p - a.offset) * a.ldo + h * ATTN_D;
+        const int64_t part_at = ((int64_t)blockIdx.y * a.S + (p - a.offset)) * a.H + h;
+        if (a.splits > 1 && there) a.pml[part_at] = make_float2(m, l);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float o[32];
           ld32(o_at + 32 * c, o);
           wait_ld();
+          if (n == 0)                                  // none of the split's keys: nothing has been written there
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0.f;
           if (taken_out && there)                      // rare, and slow
             for (int j = 0; j < tiles.n; ++j) {
               const int key0 = tiles.key0(j);
@@ -274,7 +285,11 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
                   if (not_finite(v[e])) o[e] += __half2float(v[e]);
               }
             }
-          if (there) {
+          if (there && a.splits > 1) {
+            float4* const part = reinterpret_cast<float4*>(a.po + part_at * ATTN_D + 32 * c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) part[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          } else if (there) {
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) w[e] = h2_as_u32(__floats2half2_rn(o[2 * e] * inv, o[2 * e + 1] * inv));
@@ -431,7 +446,51 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
   }
 }
 
+// Partial results of a row, in the splits' order: a warp has one, a lane four dims
+__global__ void __launch_bounds__(128)
+attn_window_merge_kernel(const Args a, int64_t rows) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  float M = -3e38f;
+  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.pml[s * rows + row].x);
+  float x[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 ml = a.pml[s * rows + row];
+    const float4 o = reinterpret_cast<const float4*>(a.po + (s * rows + row) * ATTN_D)[lane];
+    const float f = ex2(ml.x - M), y[4] = {o.x, o.y, o.z, o.w};
+    l = fmaf(ml.y, f, l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = fabsf(y[e]) <= 3.402823466e38f ? fmaf(y[e], f, x[e]) : x[e] + y[e];       // not 0 times infinity
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  __half* const out = a.o + row / a.H * a.ldo + row % a.H * ATTN_D + 4 * lane;
+  reinterpret_cast<__half2*>(out)[0] = __floats2half2_rn(x[0] * inv, x[1] * inv);
+  reinterpret_cast<__half2*>(out)[1] = __floats2half2_rn(x[2] * inv, x[3] * inv);
+}
+
 }  // namespace tc
+
+int splits_tc(const Args& a) {
+  using namespace tc;
+  const int64_t blocks = (int64_t)a.H * ((a.S + 2 * BQ - 1) / (2 * BQ));
+  Args one = a;
+  one.splits = 1;
+  const int tiles = Tiles(one, (a.S - 1) / (2 * BQ) * 2 * BQ, 0).n;          // of the last block, which has most
+  // Least of what a CTA takes for its tiles and what sharing them costs: another launch, and the partial results' way out and back
+  // (us; measured: 256 queries x 32 heads, 11 tiles 27.5 alone, 20 in four splits; 512 queries, four tiles 12.7 alone, 19 in two)
+  const double tile = a.S > BQ ? 2.1 : 1.4, part = 0.35e-6 * a.S * a.H * (ATTN_D + 2) * sizeof(float);
+  int best = 1;
+  double least = tile * tiles;
+  for (int s = 2; s <= 16 && s * blocks <= 148 && 2 * s <= tiles; ++s) {
+    const double t = tile * ((tiles + s - 1) / s) + 3.5 + part * s;
+    if (t < least) { least = t; best = s; }
+  }
+  return best;
+}
 
 int launch_tc(const Args& a, int* err, cudaStream_t st) {
   using namespace tc;
@@ -453,7 +512,9 @@ int launch_tc(const Args& a, int* err, cudaStream_t st) {
   if (e != cudaSuccess) { (void)cudaGetLastError(); return Q40_E_UNSUPPORTED; }
   const int64_t blocks = (int64_t)a.H * ((a.S + 2 * BQ - 1) / (2 * BQ));
   if (blocks > 0x7fffffffLL) return Q40_E_SHAPE;
-  e = q40_launch_pdl(attn_window_tc_kernel, dim3((unsigned)blocks), dim3(THREADS), SMEM, st, a, maps, err);
+  e = q40_launch_pdl(attn_window_tc_kernel, dim3((unsigned)blocks, a.splits), dim3(THREADS), SMEM, st, a, maps, err);
+  const int64_t rows = (int64_t)a.S * a.H;
+  if (e == cudaSuccess && a.splits > 1) e = q40_launch_pdl(tc::attn_window_merge_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, a, rows);
   return e == cudaSuccess ? Q40_OK : (int)e;
 }
 

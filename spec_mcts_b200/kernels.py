@@ -602,8 +602,11 @@ def causal_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional
         st = _stream(dev)
         err = _tc_error_page(dev, st).data_ptr() + 4092
         lds = [t.stride(0) if t.shape[0] > 1 else t.shape[1] * D for t in (q, k, v, out)]
+        w, sinks = whole if window is None else min(window, max(whole, 1)), min(sinks, whole)
+        nbytes = lib.q40_attn_causal_window_workspace_bytes(S, H, Hkv, D, offset, max(w, 1), sinks)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None           # of this call alone, as in _attn_pages
         check(lib.q40_attn_causal_window(q.data_ptr(), lds[0], k.data_ptr(), lds[1], v.data_ptr(), lds[2], out.data_ptr(), lds[3], S, H, Hkv, D,
-                                         offset, whole if window is None else min(window, max(whole, 1)), min(sinks, whole), err, st), "q40_attn_causal_window")
+                                         offset, max(w, 1), sinks, _ptr(ws), nbytes, err, st), "q40_attn_causal_window")
         return out
     check(lib.q40_attn_causal(q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
                               out.data_ptr(), out.stride(0), S, H, Hkv, D, _stream(dev)), "q40_attn_causal")

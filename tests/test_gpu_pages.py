@@ -212,7 +212,8 @@ def check_prompt(got, want, size, v):
 @pytest.mark.parametrize("s,h,hkv,window,sinks,offset", [(1, 4, 4, 1, 0, 0), (1, 4, 2, 5, 2, 100), (16, 2, 1, 16, 0, 0), (63, 4, 2, 10, 1, 0), (64, 4, 2, 64, 64, 1), (65, 4, 1, 1, 0, 63),
                                                          (130, 8, 2, 40, 70, 200), (200, 2, 2, 1000, 5, 0), (200, 2, 2, 1000, 5, 777), (129, 3, 3, 128, 0, 128), (300, 4, 4, 65, 130, 450),
                                                          (77, 32, 8, 50, 4, 0), (257, 8, 1, 200, 4, 1000), (513, 16, 2, 1, 3, 0), (700, 5, 1, 333, 1000, 90),
-                                                         (1000, 4, 2, 129, 0, 300), (1500, 2, 2, 700, 200, 31), (2049, 1, 1, 1, 1, 0), (1280, 2, 1, 10000, 0, 2000), (999, 2, 1, 128, 300, 129)])
+                                                         (1000, 4, 2, 129, 0, 300), (1500, 2, 2, 700, 200, 31), (2049, 1, 1, 1, 1, 0), (1280, 2, 1, 10000, 0, 2000), (999, 2, 1, 128, 300, 129),
+                                                         (1, 2, 1, 5000, 0, 4500), (7, 1, 1, 1000, 500, 6000), (100, 8, 2, 900, 4, 2000), (257, 4, 4, 300, 1, 3000), (300, 1, 1, 4000, 130, 3777)])
 def test_prompt(K, s, h, hkv, window, sinks, offset):
     g = generator(s + h)
     q, k, v = normal(g, s, h, D), normal(g, offset + s + 3, hkv, D), normal(g, offset + s + 3, hkv, D)
@@ -232,18 +233,19 @@ def test_prompt_strided_into_out(K):
     assert (out[:, 0] == 7).all() and (out[:, 5] == 7).all()
 
 
-@pytest.mark.parametrize("s", [150, 700])
-def test_prompt_values_that_are_not_finite(K, s):
+@pytest.mark.parametrize("s,window", [(60, 30), (150, 30), (700, 30), (700, 650)])
+def test_prompt_values_that_are_not_finite(K, s, window):
     """They reach the queries that see them, and no other; keys that are not finite reach nobody behind a mask."""
     g = generator(12)
-    window, sinks = 30, 3
+    sinks = 3
     q, k, v = normal(g, s, 4, D), normal(g, s, 2, D), normal(g, s, 2, D)
     want, size = prompt_reference(q, k, v, window, sinks, 0)
     i = torch.arange(s, device="cuda")
     sees = lambda j: (i >= j) & ((i - j < window) | (j < sinks))
-    v[70, 0, 5], v[70, 0, 6], v[100, 0, 6], v[s - 20, 1, 7] = math.inf, math.inf, -math.inf, math.nan
+    x, y, z = s // 3, s // 3 + 20, s - 20
+    v[x, 0, 5], v[x, 0, 6], v[y, 0, 6], v[z, 1, 7] = math.inf, math.inf, -math.inf, math.nan
     got = K.causal_attn(q, k, v, window=window, sinks=sinks)
-    a, b, c = sees(70)[:, None], sees(100)[:, None], sees(s - 20)[:, None]
+    a, b, c = sees(x)[:, None], sees(y)[:, None], sees(z)[:, None]
     first, second = got[:, :2], got[:, 2:]
     assert ((first[..., 5] == math.inf) == a).all()
     assert ((first[..., 6] == math.inf) == (a & ~b)).all() and ((first[..., 6] == -math.inf) == (b & ~a)).all() and (first[..., 6].isnan() == (a & b)).all()
@@ -251,9 +253,9 @@ def test_prompt_values_that_are_not_finite(K, s):
     rest = torch.ones_like(got, dtype=torch.bool)
     rest[:, :2, 5:7], rest[:, 2:, 7] = False, False
     check_prompt(torch.where(rest, got, 0), torch.where(rest, want, 0), size, v)
-    k[90] = math.nan                                     # every query that sees it, and no other
+    k[s // 2] = math.nan                                 # every query that sees it, and no other
     got = K.causal_attn(q, k, v, window=window, sinks=sinks)
-    assert (got[..., 0].isnan() == sees(90)[:, None]).all()
+    assert (got[..., 0].isnan() == sees(s // 2)[:, None]).all()
 
 
 # ---- append --------------------------------------------------------------------------------------------------------

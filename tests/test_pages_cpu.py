@@ -19,8 +19,8 @@ def append(tbl=A, idx=4, tstride=8, width=8, pos=A, off=None, q=A, qs=512, qo=A,
     return lib.q40_page_append(tbl, idx, tstride, width, pos, off, q, qs, qo, k, kst, v, vst, cos, sin, n_pos, kp, vp, ks, vs, kind, P, B, T, H, Hkv, D, ps, None)
 
 
-def window(q=A, ldq=512, k=A, ldk=256, v=A, ldv=256, o=A, ldo=512, S=4, H=4, Hkv=2, D=128, off=0, w=3, s=0, err=A):
-    return lib.q40_attn_causal_window(q, ldq, k, ldk, v, ldv, o, ldo, S, H, Hkv, D, off, w, s, err, None)
+def window(q=A, ldq=512, k=A, ldk=256, v=A, ldv=256, o=A, ldo=512, S=4, H=4, Hkv=2, D=128, off=0, w=3, s=0, ws=None, n=0, err=A):
+    return lib.q40_attn_causal_window(q, ldq, k, ldk, v, ldv, o, ldo, S, H, Hkv, D, off, w, s, ws, n, err, None)
 
 
 @pytest.mark.parametrize("status,bad", [(NULL, dict(q=None)), (NULL, dict(tbl=None)), (NULL, dict(ks=None)), (NULL, dict(P=0)), (SHAPE, dict(H=5)), (SHAPE, dict(tstride=7)), (SHAPE, dict(P=100)),
@@ -51,6 +51,17 @@ def test_append_refuses(status, bad):
 
 
 @pytest.mark.parametrize("status,bad", [(NULL, dict(o=None)), (UNSUPPORTED, dict(D=64)), (SHAPE, dict(H=5)), (SHAPE, dict(w=0)), (SHAPE, dict(s=-1)), (SHAPE, dict(off=-1)), (SHAPE, dict(off=1 << 30)),
-                                        (SHAPE, dict(ldq=511)), (ALIGN, dict(ldk=260)), (ALIGN, dict(v=A + 8)), (ALIGN, dict(o=A + 2)), (0, dict(S=0))])
+                                        (SHAPE, dict(ldq=511)), (ALIGN, dict(ldk=260)), (ALIGN, dict(v=A + 8)), (ALIGN, dict(o=A + 2)), (0, dict(S=0)),
+                                        (WORKSPACE, dict(S=100, off=4000, w=4000, ws=A, n=64)), (ALIGN, dict(S=100, off=4000, w=4000, ws=A + 4, n=1 << 30)), (ALIGN, dict(S=100, err=A + 2))])
 def test_window_refuses(status, bad):
     assert window(**bad) == status
+
+
+def test_window_workspace():
+    need = lambda S, H, off, w, s=0: lib.q40_attn_causal_window_workspace_bytes(S, H, H, 128, off, w, s)
+    row = 130 * 4
+    assert need(1, 32, 0, 1) == need(100, 32, 0, 100) == need(0, 32, 5000, 5000) == need(100, 32, 5000, 0) == 0
+    assert need(100, 32, 5000, 4096) == 4 * 100 * 32 * row                 # as many as leave each SM a CTA, for many tiles
+    assert need(100, 32, 1000, 200) == 0                                   # few tiles
+    assert need(100, 1, 1 << 20, 1 << 20) == 16 * 100 * row                # and 16 at most
+    assert need(5000, 32, 5000, 4096) == need(512, 32, 0, 512) == 0
