@@ -20,9 +20,11 @@
 namespace q40 {
 namespace pages {
 
-constexpr int NW = 4, THREADS = NW * 32;
+constexpr int MERGE_THREADS = 128;
+constexpr int FEW = 148;                   // units
 constexpr int CHUNK_MIN = 512, CHUNK_MAX = 8192;
-constexpr int64_t CHUNKS = 4800;
+constexpr int CHUNK_WAVE = 2048;
+constexpr int64_t WAVE = 296, CTAS = 1200; // CTAs that a call is cut into, about: one wave of them, where that leaves chunks of up to CHUNK_WAVE
 
 struct Args {
   const __half* q;         // sequence b, head h at q + b * q_stride + h * 128
@@ -36,7 +38,7 @@ struct Args {
   int64_t P;
   int B, L, H, Hkv, window, sinks;
   int groups, heads;       // of a kv head's query heads; heads of a group (the last may have fewer)
-  int64_t chunks_of_unit; // what a unit's keys are cut into, about (chunk_of)
+  int64_t units;
   int nchunks;             // most of a unit
   float* po;               // [units][nchunks][heads][128], not normalised
   float2* pml;             // ... maximum (log2) and sum
@@ -78,9 +80,13 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool pr
 }
 
 // Keys of a chunk for a unit of n keys, by its own length and the number of units alone
-__host__ __device__ __forceinline__ int chunk_of(int64_t n, int64_t chunks_of_unit) {
+__host__ __device__ __forceinline__ int chunk_of(int64_t n, int64_t units) {
   int chunk = CHUNK_MIN;
-  while (chunk < CHUNK_MAX && chunk * chunks_of_unit < n) chunk *= 2;
+  const int64_t wave = WAVE / units, all = CTAS > units ? CTAS / units : 1;
+  while (chunk < CHUNK_WAVE && chunk * wave < n) chunk *= 2;
+  if (wave > 1 && chunk * wave >= n) return chunk;
+  chunk = CHUNK_MIN;
+  while (chunk < CHUNK_MAX && chunk * all < n) chunk *= 2;
   return chunk;
 }
 
@@ -117,21 +123,20 @@ __device__ __forceinline__ const unsigned char* row_at(const unsigned char* base
   return r;
 }
 
-template <int T, int G, int S>
-__global__ void __launch_bounds__(THREADS)
+template <int T, int G, int S, int NW>
+__global__ void __launch_bounds__(NW * 32)
 attn_pages_kernel(const Args a) {
   constexpr int D = ATTN_D, RB = row_bytes<T>, KEYS = keys_of<T>, MT = KEYS / 16;
   constexpr int GL = G == 4 ? 0 : G == 2 ? 1 : 2;        // up to four heads: lane t works for head t >> GL
   constexpr int HL = G == 8 ? 2 : 1;                     // heads of a lane
   constexpr int LPR = RB / 16, RPI = 32 / LPR;           // lanes that copy a row, rows a copy instruction
-  asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, mi = lane >> 3;
   const int unit = blockIdx.x, chunk = blockIdx.y;
   const int group = unit % a.groups, hk = unit / a.groups % a.Hkv, b = unit / a.groups / a.Hkv;
   const int rep = a.H / a.Hkv, h0 = hk * rep + group * a.heads, heads = min(a.heads, rep - group * a.heads);
   const Visible vis(a, b);
-  const int size = chunk_of(vis.n, a.chunks_of_unit);
+  const int size = chunk_of(vis.n, a.units);
   const int64_t begin64 = (int64_t)chunk * size;
   if (begin64 >= vis.n && chunk > 0) return;
   const int begin = (int)begin64, end = (int)min((int64_t)vis.n, begin64 + size);
@@ -272,7 +277,7 @@ attn_pages_kernel(const Args a) {
         for (int r = 0; r < 2 * MT; ++r) mnew = fmaxf(mnew, sc[r][j] + lv[r] - WEIGHT_BITS);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) mnew = fmaxf(mnew, __shfl_xor_sync(0xffffffffu, mnew, o));
-        const float corr = ex2(m[j] - mnew);
+        const float corr = ex2_some(m[j] - mnew);
         l[j] *= corr;
         m[j] = mnew;
 #pragma unroll
@@ -338,6 +343,8 @@ attn_pages_kernel(const Args a) {
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], o);
 
+  // behind the wait: see page_merge_kernel; and not before most of the work, since the next launch's CTAs take room from what is left of this one
+  asm volatile("griddepcontrol.launch_dependents;");
   // the ring, which is empty, takes the warp's outputs
   __shared__ float sm_m[G][NW], sm_l[G][NW];
   float* const out = reinterpret_cast<float*>(rings + warp * WB);
@@ -363,58 +370,72 @@ attn_pages_kernel(const Args a) {
   }
   __syncthreads();
   const bool alone = vis.n <= size;
-#pragma unroll
-  for (int j = 0; j < G; ++j) {
-    if (j >= heads) break;
+  const auto write = [&](int j, int d, float M, float Lsum, float x) {
+    if (alone) {
+      a.o[((int64_t)b * a.H + h0 + j) * D + d] = __float2half_rn(Lsum != 0.f ? x / Lsum : 0.f);
+    } else {
+      const int64_t at = ((int64_t)unit * a.nchunks + chunk) * a.heads + j;
+      a.po[at * D + d] = x;
+      if (d == 0) a.pml[at] = make_float2(M, Lsum);
+    }
+  };
+  for (int i = tid; i < heads * D; i += NW * 32) {
+    const int j = i / D;
     float M = NO_KEY, Lsum = 0.f, x = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) M = fmaxf(M, sm_m[j][w]);
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float f = ex2(sm_m[j][w] - M);
+      const float f = ex2_some(sm_m[j][w] - M);
       Lsum = fmaf(sm_l[j][w], f, Lsum);
-      x = fmaf(reinterpret_cast<const float*>(rings + w * WB)[j * D + tid], f, x);
+      x = fmaf(reinterpret_cast<const float*>(rings + w * WB)[i], f, x);
     }
-    if (alone) {
-      a.o[((int64_t)b * a.H + h0 + j) * D + tid] = __float2half_rn(Lsum != 0.f ? x / Lsum : 0.f);
-    } else {
-      const int64_t at = ((int64_t)unit * a.nchunks + chunk) * a.heads + j;
-      a.po[at * D + tid] = x;
-      if (tid == 0) a.pml[at] = make_float2(M, Lsum);
-    }
+    write(j, i % D, M, Lsum, x);
   }
 }
 
-// The partial results of units of several chunks, in the chunks' order; a CTA has a unit and one of its heads, a thread a dim
-__global__ void __launch_bounds__(THREADS)
+// The partial results of units of several chunks, in the chunks' order; a CTA has a unit and one of its heads, a thread a dim.  The launch in
+// front starts this one when what it waited for is there, so that lengths can be read before its results are
+__global__ void __launch_bounds__(MERGE_THREADS)
 page_merge_kernel(const Args a) {
-  asm volatile("griddepcontrol.launch_dependents;");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr int BATCH = 8;                       // chunks whose results are requested together
   const int unit = blockIdx.x / a.heads, j = blockIdx.x % a.heads, tid = threadIdx.x;
   const int group = unit % a.groups, hk = unit / a.groups % a.Hkv, b = unit / a.groups / a.Hkv;
   const int rep = a.H / a.Hkv;
-  if (j >= rep - group * a.heads) return;
   const Visible vis(a, b);
-  const int size = chunk_of(vis.n, a.chunks_of_unit);
-  if (vis.n <= size) return;
-  const int n = (vis.n - 1) / size + 1;
+  const int size = chunk_of(vis.n, a.units), n = (vis.n - 1) / size + 1;
   const int64_t first = (int64_t)unit * a.nchunks * a.heads + j;
-  float M = NO_KEY;
-  for (int c = tid & 31; c < n; c += 32) M = fmaxf(M, a.pml[first + (int64_t)c * a.heads].x);
-  M = warp_max(M);
-  float x = 0.f, Lsum = 0.f;
-#pragma unroll 8
-  for (int c = 0; c < n; ++c) {
-    const int64_t at = first + (int64_t)c * a.heads;
-    const float2 ml = a.pml[at];
-    const float f = ex2(ml.x - M);
-    Lsum = fmaf(ml.y, f, Lsum);
-    x = fmaf(a.po[at * ATTN_D + tid], f, x);
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (vis.n <= size || j >= rep - group * a.heads) return;
+  float M = NO_KEY, x = 0.f, Lsum = 0.f;
+  for (int c0 = 0; c0 < n; c0 += BATCH) {
+    float2 ml[BATCH];
+    float y[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int64_t at = first + (int64_t)(c0 + i) * a.heads;
+      ml[i] = c0 + i < n ? a.pml[at] : make_float2(NO_KEY, 0.f);
+      y[i] = c0 + i < n ? a.po[at * ATTN_D + tid] : 0.f;
+    }
+    float now = M;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) now = fmaxf(now, ml[i].x);
+    const float corr = ex2_some(M - now);
+    x *= corr;
+    Lsum *= corr;
+    M = now;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const float f = ex2_some(ml[i].x - M);
+      Lsum = fmaf(ml[i].y, f, Lsum);
+      x = fmaf(y[i], f, x);
+    }
   }
   a.o[((int64_t)b * a.H + hk * rep + group * a.heads + j) * ATTN_D + tid] = __float2half_rn(Lsum != 0.f ? x / Lsum : 0.f);
 }
 
-struct Plan { int64_t units, chunks_of_unit; int groups, heads, nchunks; };
+struct Plan { int64_t units; int groups, heads, nchunks; };
 
 static Plan plan_of(int B, int H, int Hkv, int L, int window, int sinks) {
   Plan p;
@@ -422,29 +443,40 @@ static Plan plan_of(int B, int H, int Hkv, int L, int window, int sinks) {
   p.groups = (rep + 7) / 8;
   p.heads = (rep + p.groups - 1) / p.groups;
   p.units = (int64_t)B * Hkv * p.groups;
-  p.chunks_of_unit = std::max<int64_t>(1, CHUNKS / p.units);
   const int64_t most = window > 0 ? std::min<int64_t>(L, (int64_t)window + sinks) : L;      // visible keys
+  // The most chunks that a unit of up to that many keys has.  While chunks are of one size, longer units have more of them; the size changes
+  // behind multiples of one (chunk_of): there, or at the end
   int64_t n = 1;
+  const auto at = [&](int64_t keys) {
+    keys = std::min(keys, most);
+    if (keys > 0) n = std::max(n, (keys + chunk_of(keys, p.units) - 1) / chunk_of(keys, p.units));
+  };
+  at(most);
   for (int64_t chunk = CHUNK_MIN; chunk <= CHUNK_MAX; chunk *= 2) {
-    const int64_t longest = chunk < CHUNK_MAX ? std::min(most, chunk * p.chunks_of_unit) : most;      // of those cut into such
-    if (longest > 0 && chunk_of(longest, p.chunks_of_unit) == chunk) n = std::max(n, (longest + chunk - 1) / chunk);
+    at(chunk * (WAVE / p.units));
+    at(chunk * std::max<int64_t>(1, CTAS / p.units));
   }
   p.nchunks = (int)std::min<int64_t>(n, 1 << 30);
   return p;
 }
 
-template <int T, int G>
+template <int T, int G, int S, int NW>
 static cudaError_t launch(const Args& a, int64_t units, cudaStream_t st) {
-  constexpr int S = T == CACHE_F16 ? 3 : 2;
   static std::atomic<uint64_t> ready;
   constexpr int BYTES = NW * warp_bytes<T, G, S>;
-  const cudaError_t e = q40_allow_smem(ready, (const void*)attn_pages_kernel<T, G, S>, BYTES);
+  const cudaError_t e = q40_allow_smem(ready, (const void*)attn_pages_kernel<T, G, S, NW>, BYTES);
   if (e != cudaSuccess) return e;
-  return q40_launch_pdl(attn_pages_kernel<T, G, S>, dim3((unsigned)units, (unsigned)a.nchunks), dim3(THREADS), BYTES, st, a);
+  return q40_launch_pdl(attn_pages_kernel<T, G, S, NW>, dim3((unsigned)units, (unsigned)a.nchunks), dim3(NW * 32), BYTES, st, a);
+}
+template <int T, int G>
+static cudaError_t launch_warps(const Args& a, int64_t units, cudaStream_t st) {
+  if (units <= FEW) return launch<T, G, 1, 8>(a, units, st);
+  return launch<T, G, T == CACHE_F16 ? 3 : 2, 4>(a, units, st);
 }
 template <int T>
 static cudaError_t launch_heads(const Args& a, int64_t units, cudaStream_t st) {
-  return a.heads > 4 ? launch<T, 8>(a, units, st) : a.heads > 2 ? launch<T, 4>(a, units, st) : a.heads > 1 ? launch<T, 2>(a, units, st) : launch<T, 1>(a, units, st);
+  return a.heads > 4 ? launch_warps<T, 8>(a, units, st) : a.heads > 2 ? launch_warps<T, 4>(a, units, st)
+         : a.heads > 1 ? launch_warps<T, 2>(a, units, st) : launch_warps<T, 1>(a, units, st);
 }
 
 }  // namespace pages
@@ -486,12 +518,12 @@ extern "C" int q40_attn_pages(const void* page_tbl, int idx_bytes, int64_t tbl_s
   a.tbl = {page_tbl, tbl_stride, idx_bytes == 4, page_size, page_shift_of(page_size)};
   a.seq_lens = seq_lens; a.P = P; a.last_page = P > 0 ? (int)((P - 1) / page_size) : 0; a.pages = (int)(P / page_size);
   a.B = B; a.L = Lmax; a.H = H; a.Hkv = Hkv; a.window = window; a.sinks = sinks;
-  a.groups = p.groups; a.heads = p.heads; a.chunks_of_unit = p.chunks_of_unit; a.nchunks = p.nchunks;
+  a.groups = p.groups; a.heads = p.heads; a.units = p.units; a.nchunks = p.nchunks;
   a.po = (float*)workspace; a.pml = (float2*)(a.po + parts * ATTN_D);
   a.scale_log2 = attn_scale_log2(D);
   const cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e = cache_type == CACHE_F16 ? launch_heads<CACHE_F16>(a, p.units, st)
                   : cache_type == CACHE_I8 ? launch_heads<CACHE_I8>(a, p.units, st) : launch_heads<CACHE_E4M3>(a, p.units, st);
-  if (e == cudaSuccess && p.nchunks > 1) e = q40_launch_pdl(page_merge_kernel, dim3((unsigned)(p.units * p.heads)), dim3(THREADS), 0, st, a);
+  if (e == cudaSuccess && p.nchunks > 1) e = q40_launch_pdl(page_merge_kernel, dim3((unsigned)(p.units * p.heads)), dim3(MERGE_THREADS), 0, st, a);
   return e == cudaSuccess ? Q40_OK : (int)e;
 }

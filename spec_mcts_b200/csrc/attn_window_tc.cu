@@ -214,7 +214,7 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
       const float most = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
       const bool passes = most > m + STAY;
       if (__any_sync(0xffffffffu, passes)) {
-        const float now = passes ? most : m, corr = ex2(m - now);
+        const float now = passes ? most : m, corr = fmaxf(ex2(m - now), 1.17549435e-38f);      // (never 0: infinities stay)
         m = now;
         l *= corr;
         if (n > 0) {
@@ -461,10 +461,10 @@ attn_window_merge_kernel(const Args a, int64_t rows) {
   for (int s = 0; s < a.splits; ++s) {
     const float2 ml = a.pml[s * rows + row];
     const float4 o = reinterpret_cast<const float4*>(a.po + (s * rows + row) * ATTN_D)[lane];
-    const float f = ex2(ml.x - M), y[4] = {o.x, o.y, o.z, o.w};
+    const float f = fmaxf(ex2(ml.x - M), 1.17549435e-38f), y[4] = {o.x, o.y, o.z, o.w};
     l = fmaf(ml.y, f, l);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = fabsf(y[e]) <= 3.402823466e38f ? fmaf(y[e], f, x[e]) : x[e] + y[e];       // not 0 times infinity
+    for (int e = 0; e < 4; ++e) x[e] = fmaf(y[e], f, x[e]);
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;
   __half* const out = a.o + row / a.H * a.ldo + row % a.H * ATTN_D + 4 * lane;

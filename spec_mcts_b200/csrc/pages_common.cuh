@@ -49,4 +49,7 @@ __device__ __forceinline__ uint32_t i8_to_h2(uint32_t biased) {
   return h2_as_u32(__hsub2(u32_as_h2(biased), u32_as_h2(0x64806480u)));
 }
 
+// 2^x of what is scaled down, never 0: an infinite value stays one
+__device__ __forceinline__ float ex2_some(float x) { return fmaxf(ex2(x), 1.17549435e-38f); }
+
 }  // namespace q40

@@ -109,7 +109,8 @@ def test_decode_edges(K, kind, h, hkv, ps, window, sinks, idx):
 # units of one and of several chunks in each of the rule's ranges
 @pytest.mark.parametrize("kind", ["f16", "int8", "e4m3"])
 @pytest.mark.parametrize("b,h,hkv,keys,window,sinks", [(1, 1, 1, 1, 4096, 0), (1, 8, 1, 20001, None, 0), (2, 32, 8, 3000, 2500, 4), (10, 32, 8, 1030, None, 0),
-                                                       (17, 32, 32, 1500, 1100, 64), (70, 32, 32, 2100, None, 0)])
+                                                       (17, 32, 32, 1500, 1100, 64), (70, 32, 32, 2100, None, 0), (1, 8, 8, 70000, None, 0),
+                                                          (3, 32, 8, 40000, None, 0), (2, 16, 8, 129, 129, 0), (5, 8, 8, 1100, 1000, 30), (30, 16, 2, 3000, None, 0)])
 def test_decode_long(K, kind, b, h, hkv, keys, window, sinks):
     if kind == "f16" and window is None:
         window, sinks = keys - 1, 1
@@ -167,17 +168,19 @@ def test_decode_masked_places_hold_anything(K, kind, h):
 
 
 @pytest.mark.parametrize("h", [2, 8])
-def test_decode_infinite_and_nan_values(K, h):
+@pytest.mark.parametrize("far", [9, 20, 40, 63, 600])     # in the same product, warp, CTA and another one
+def test_decode_infinite_and_nan_values(K, h, far):
     """fp16: an infinite value comes out, whatever its weight is; 8 bits: a NaN scale does."""
     g = generator(8)
-    lens = torch.full((2,), 64, dtype=torch.int32, device="cuda")
-    run, *_, (p, q, kp, vp, ks, vs, _, slots) = decode(K, "f16", g, 2, h, 1, 16, 64, lens, 64, 0)
+    n = 1000 if far > 63 else 64
+    lens = torch.full((2,), n, dtype=torch.int32, device="cuda")
+    run, *_, (p, q, kp, vp, ks, vs, _, slots) = decode(K, "f16", g, 2, h, 1, 16, n, lens, n, 0)
     q[..., 0] = 8.0
-    kp[0, slots[0, 5], 0], kp[0, slots[0, 9], 0] = -400.0, 40.0         # its score is far below another's
+    kp[0, slots[0, 5], 0], kp[0, slots[0, far], 0] = -400.0, 40.0       # its score is far below another's
     vp[0, slots[0, 5], 3], vp[0, slots[0, 5], 70] = math.inf, -math.inf
     got = run()
     assert (got[0, :, 3] == math.inf).all() and (got[0, :, 70] == -math.inf).all() and got[0].isfinite().sum() == h * (D - 2) and got[1].isfinite().all()
-    run, *_, (p, q, kp, vp, ks, vs, _, slots) = decode(K, "int8", g, 2, h, 1, 16, 64, lens, None, 0)
+    run, *_, (p, q, kp, vp, ks, vs, _, slots) = decode(K, "int8", g, 2, h, 1, 16, n, lens, None, 0)
     vs[0, p[1, 2].item()] = math.nan
     got = run()
     assert got[0].isfinite().all() and got[1].isnan().all()

@@ -27,14 +27,14 @@ def window(q=A, ldq=512, k=A, ldk=256, v=A, ldv=256, o=A, ldo=512, S=4, H=4, Hkv
                                         (SHAPE, dict(w=-1)), (SHAPE, dict(s=-1)), (SHAPE, dict(ps=0)), (SHAPE, dict(qs=511)), (SHAPE, dict(L=(1 << 30) + 1, tstride=1 << 40)),
                                         (ALIGN, dict(q=A + 8)), (ALIGN, dict(qs=516)), (ALIGN, dict(k=A + 8)), (ALIGN, dict(vs=A + 2)), (ALIGN, dict(lens=A + 2)), (ALIGN, dict(tbl=A + 2)),
                                         (UNSUPPORTED, dict(D=64)), (UNSUPPORTED, dict(idx=8)), (UNSUPPORTED, dict(kind=3)), (0, dict(B=0)),
-                                        (WORKSPACE, dict(L=4096, tstride=256)), (WORKSPACE, dict(L=4096, tstride=256, ws=A, n=64)), (ALIGN, dict(L=4096, tstride=256, ws=A + 4, n=1 << 30))])
+                                        (WORKSPACE, dict(L=1 << 20, tstride=1 << 16)), (WORKSPACE, dict(L=1 << 20, tstride=1 << 16, ws=A, n=64)), (ALIGN, dict(L=1 << 20, tstride=1 << 16, ws=A + 4, n=1 << 30))])
 def test_attention_refuses(status, bad):
     assert attn(**bad) == status
 
 
 def test_attention_workspace():
     need = lambda *a: lib.q40_attn_pages_workspace_bytes(*a)
-    assert need(1, 4, 4, 200, 0, 0) == 0 and need(0, 4, 4, 1 << 20, 0, 0) == 0 and need(2, 5, 4, 1 << 20, 0, 0) == 0
+    assert need(1, 4, 4, 500, 0, 0) == 0 and need(0, 4, 4, 1 << 20, 0, 0) == 0 and need(2, 5, 4, 1 << 20, 0, 0) == 0
     one = need(4, 32, 8, 1 << 16, 0, 0)
     assert one > 0 and need(8, 32, 8, 1 << 16, 0, 0) >= one
     assert need(4, 32, 8, 1 << 16, 100, 4) == 0               # what a window leaves fits one chunk
