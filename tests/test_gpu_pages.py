@@ -121,6 +121,15 @@ def test_decode_long(K, kind, b, h, hkv, keys, window, sinks):
     check_decode(run(), want, size)
 
 
+@pytest.mark.parametrize("lens", [[18944, 18945, 37888, 37889], [75776, 75777, 76800, 76801], [511, 512, 513, 1]])
+def test_decode_where_chunks_get_larger(K, lens):
+    """Eight units: chunks double behind 37 of 512 and of 1024 keys, and are of 512 again behind 37 of 2048, up to 150 of them."""
+    g = generator(lens[0])
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    run, want, size, _ = decode(K, "int8", g, 4, 4, 2, 64, max(lens), n, None, 0)
+    check_decode(run(), want, size)
+
+
 @pytest.mark.parametrize("kind", ["f16", "int8"])
 def test_decode_does_not_depend_on_the_tables_width(K, kind):
     """Nor on what its entries behind the lengths are."""
