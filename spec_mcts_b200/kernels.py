@@ -27,9 +27,12 @@ def _load_host_calls():
         from . import _host_calls as m
     except Exception as e:
         import warnings
-        warnings.warn(f"calls of matmul_q40 and linear_q40 take longer without {_build.HOST}: {e}")
+        warnings.warn(f"calls of matmul_q40, linear_q40 and of the paged cache take longer without {_build.HOST}: {e}")
         return None
-    m.init(*[ctypes.cast(f, ctypes.c_void_p).value for f in (lib.q40_matmul_tiled, lib.q40_gemm_nk)])
+    address = lambda f: ctypes.cast(f, ctypes.c_void_p).value
+    m.init(*[address(f) for f in (lib.q40_matmul_tiled, lib.q40_gemm_nk)])
+    m.init_pages(*[address(f) for f in (lib.q40_attn_pages, lib.q40_attn_pages_workspace_bytes, lib.q40_page_append, lib.q40_attn_causal_window,
+                                        lib.q40_attn_causal_window_workspace_bytes)])
     return m
 
 
@@ -580,6 +583,10 @@ def causal_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional
     With `window` a position attends its last `window` positions, itself among them, and the first `sinks`.  With `offset` the queries
     are positions offset .. offset + S - 1 of a longer prompt, whose first offset + S keys and values k and v hold
     (q40_attn_causal_window)."""
+    if out is None and (window is not None or sinks != 0 or offset != 0) and _host_calls is not None:
+        o = _host_calls.causal_window(q, k, v, window, sinks, offset, _workspaces)      # None: not a plain call
+        if o is not None:
+            return o
     dev = _need_cuda(q, k, v, out)
     S, H, D = q.shape
     Hkv = k.shape[1]
@@ -752,8 +759,13 @@ def page_flash_attn(p, q, k, v, P, B, L, H, D, *, page_size: int = 1, seq_lens=N
     (triton_kernels.py:764-789): p [B,L] int16 token-slot table, k/v pools [H,P,D].
     Extensions: page_size > 1 (p then lists page ids), int32 tables, per-branch seq_lens; with `window`, a query, which is its branch's
     last position, attends that many last keys and the first `sinks` alone."""
+    windowed = window is not None or sinks != 0
+    if windowed and D == 128 and _host_calls is not None and q.shape == (B, H, D) and k.dtype == torch.float16 and k.shape[1:] == (P, D):
+        o = _host_calls.attn_pages(p, q, k, v, None, None, L, page_size, seq_lens, window, sinks)      # None: not a plain call
+        if o is not None:
+            return o
     dev = _need_cuda(p, q, k, v, seq_lens)
-    if window is not None or sinks != 0:
+    if windowed:
         if k.dtype != torch.float16 or v.dtype != torch.float16 or q.shape != (B, H, D) or k.shape[1:] != (P, D) or v.shape != k.shape:
             raise Q40Error(f"page_flash_attn: fp16 pools [kv heads, {P}, {D}] and queries [{B}, {H}, {D}] expected")
         return _attn_pages("page_flash_attn", dev, p, q, k.contiguous(), v.contiguous(), None, None, L, page_size, seq_lens, window, sinks)
@@ -846,6 +858,10 @@ def page_flash_attn_q8(p, q, k, v, k_scale, v_scale, *, page_size: int, seq_lens
     page and kv head, k_scale / v_scale [Hkv, P / page_size] (element = code * scale), as page_append writes them.  q [B, H, 128] is
     one query for each sequence, its last position; p [B, pages] lists page ids, seq_lens [B] the lengths (None: the table's whole width).
     With `window` a query attends that many last keys and the first `sinks` alone (q40_attn_pages in include/q40b200.h)."""
+    if _host_calls is not None and k.dtype != torch.float16:
+        o = _host_calls.attn_pages(p, q, k, v, k_scale, v_scale, p.shape[-1] * page_size, page_size, seq_lens, window, sinks)      # None: not a plain call
+        if o is not None:
+            return o
     dev = _need_cuda(p, q, k, v, k_scale, v_scale, seq_lens)
     if k.dtype == torch.float16:
         raise Q40Error("page_flash_attn_q8: 8-bit pools expected; page_flash_attn reads fp16 ones")
@@ -864,6 +880,10 @@ def page_append(p, k, v, kpool, vpool, pos, *, page_size: int = 1, offsets=None,
     Rows of no sequence and positions without a page are not written.  An 8-bit page's scale grows with what comes, and its earlier
     rows are coded anew when it does.  Tokens of one call that share a slot, or in 8 bits sequences that append to one page, leave it undefined
     (q40_page_append in include/q40b200.h)."""
+    if _host_calls is not None:
+        done = _host_calls.page_append(p, k, v, kpool, vpool, pos, page_size, offsets, k_scale, v_scale, q, cos, sin)     # None: not a plain call
+        if done is not None:
+            return done[0]
     dev = _need_cuda(p, k, v, kpool, vpool, pos, offsets, k_scale, v_scale, q, cos, sin)
     kind = _need_pools("page_append", kpool, vpool, k_scale, v_scale, page_size)
     Hkv, P, D = kpool.shape
