@@ -471,7 +471,7 @@ static cudaError_t launch(const Args& a, int64_t units, cudaStream_t st) {
 template <int T, int G>
 static cudaError_t launch_warps(const Args& a, int64_t units, cudaStream_t st) {
   if (units <= FEW) return launch<T, G, 1, 8>(a, units, st);
-  return launch<T, G, T == CACHE_F16 ? 3 : 2, 4>(a, units, st);
+  return launch<T, G, 2, 4>(a, units, st);
 }
 template <int T>
 static cudaError_t launch_heads(const Args& a, int64_t units, cudaStream_t st) {

@@ -28,10 +28,12 @@ struct Args {
   float *k_scale, *v_scale;
   int64_t P;
   int B, T, H, Hkv;
-  unsigned q_blocks;       // of the 8-bit launch: blocks in front that rotate queries
+  unsigned page_blocks;    // of the 8-bit launch: blocks in front that have a page; the others rotate queries
 };
 
 constexpr int THREADS = 128;
+constexpr int EACH = 4;                   // heads of a lane group in large calls
+constexpr int64_t MANY = 32768;           // ... of more rows than these
 constexpr int UNITS = THREADS / 8;        // rows of 128 values of a block's pass, eight lanes each
 
 // The last i of [0, n) whose first(i) is not above x (0 where there is none)
@@ -89,35 +91,102 @@ __device__ __forceinline__ Row load_row(const __half* x, int i) {
   unpack8(*reinterpret_cast<const uint4*>(x + 64 + 8 * i), r.hi);
   return r;
 }
-__device__ __forceinline__ void rotate(Row& r, const Args& a, int64_t at, int i) {
+struct Turn { float c[8], s[8]; };        // of a position, lane i's
+__device__ __forceinline__ Turn turn_of(const Args& a, int64_t at, int i) {
   const int64_t p = at < a.n_pos ? at : a.n_pos - 1;
-  float c[8], s[8];
-  unpack8(*reinterpret_cast<const uint4*>(a.cos_tbl + p * 64 + 8 * i), c);
-  unpack8(*reinterpret_cast<const uint4*>(a.sin_tbl + p * 64 + 8 * i), s);
+  Turn t;
+  unpack8(*reinterpret_cast<const uint4*>(a.cos_tbl + p * 64 + 8 * i), t.c);
+  unpack8(*reinterpret_cast<const uint4*>(a.sin_tbl + p * 64 + 8 * i), t.s);
+  return t;
+}
+__device__ __forceinline__ void rotate(Row& r, const Turn& t) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float x = r.lo[j], y = r.hi[j];
-    r.lo[j] = fmaf(x, c[j], -(y * s[j]));
-    r.hi[j] = fmaf(y, c[j], x * s[j]);
+    r.lo[j] = fmaf(x, t.c[j], -(y * t.s[j]));
+    r.hi[j] = fmaf(y, t.c[j], x * t.s[j]);
   }
 }
 
-__device__ __forceinline__ void rotate_query(const Args& a, int t, int h, int i) {
-  __half* const out = a.q_out + ((int64_t)t * a.H + h) * ATTN_D;
+// Heads [h, end) of token t's queries.  Several, so that a token's place and tables are looked up once for them: 8191 tokens of 64 heads
+// 83 us with one, 60 with four, 61 with eight
+template <int E>
+__device__ __forceinline__ void rotate_queries(const Args& a, int t, int h, int end, int i) {
+  const __half* const x = a.q + t * a.q_stride + 8 * i;
+  __half* const out = a.q_out + (int64_t)t * a.H * ATTN_D + 8 * i;
+  constexpr int U = E < 4 ? E : 4;
   int seq;
   int64_t at;
-  uint4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};                     // a row of no sequence
-  if (token_of(a, t, seq, at)) {
-    Row r = load_row(a.q + t * a.q_stride + h * ATTN_D, i);
-    rotate(r, a, at, i);
-    lo = pack8(r.lo);
-    hi = pack8(r.hi);
+  const bool there = token_of(a, t, seq, at);                     // else zeros
+  const Turn turn = turn_of(a, there ? at : 0, i);
+#pragma unroll 1
+  for (int h0 = h; h0 < end; h0 += U) {
+    uint4 lo[U], hi[U];
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const int at_h = min(h0 + e, end - 1) * ATTN_D;
+      lo[e] = *reinterpret_cast<const uint4*>(x + at_h);
+      hi[e] = *reinterpret_cast<const uint4*>(x + at_h + 64);
+    }
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      if (h0 + e >= end) break;
+      Row r;
+      unpack8(lo[e], r.lo);
+      unpack8(hi[e], r.hi);
+      rotate(r, turn);
+      *reinterpret_cast<uint4*>(out + (h0 + e) * ATTN_D) = there ? pack8(r.lo) : make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(out + (h0 + e) * ATTN_D + 64) = there ? pack8(r.hi) : make_uint4(0, 0, 0, 0);
+    }
   }
-  *reinterpret_cast<uint4*>(out + 8 * i) = lo;
-  *reinterpret_cast<uint4*>(out + 64 + 8 * i) = hi;
 }
 
-// fp16 pools.  Eight lanes a row: of queries, keys, values of a token in turn
+// Heads [h, end) of token t's keys, then values, into fp16 pools
+template <int E>
+__device__ __forceinline__ void append_heads(const Args& a, int t, int h, int end, int i) {
+  int seq;
+  int64_t at;
+  if (!token_of(a, t, seq, at)) return;
+  const int64_t page = at / a.tbl.page_size;
+  const int id = page_id(a, seq, page);
+  if (id < 0) return;
+  const int64_t slot = (int64_t)id * a.tbl.page_size + (at - page * a.tbl.page_size);
+  if (slot >= a.P) return;                                        // a pool may end inside its last page
+  Turn turn = {};
+  if (a.cos_tbl && h < a.Hkv) turn = turn_of(a, at, i);
+  constexpr int U = E < 4 ? E : 4;
+#pragma unroll 1
+  for (int h0 = h; h0 < end; h0 += U) {
+    uint4 lo[U], hi[U];
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const int he = min(h0 + e, end - 1);
+      const __half* const x = (he < a.Hkv ? a.k + t * a.k_stride + he * ATTN_D : a.v + t * a.v_stride + (he - a.Hkv) * ATTN_D) + 8 * i;
+      lo[e] = *reinterpret_cast<const uint4*>(x);
+      hi[e] = *reinterpret_cast<const uint4*>(x + 64);
+    }
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const int he = h0 + e;
+      if (he >= end) break;
+      const bool is_k = he < a.Hkv;
+      if (is_k && a.cos_tbl) {
+        Row r;
+        unpack8(lo[e], r.lo);
+        unpack8(hi[e], r.hi);
+        rotate(r, turn);
+        lo[e] = pack8(r.lo);
+        hi[e] = pack8(r.hi);
+      }
+      __half* const out = reinterpret_cast<__half*>(is_k ? a.kpool : a.vpool) + ((int64_t)(is_k ? he : he - a.Hkv) * a.P + slot) * ATTN_D + 8 * i;
+      *reinterpret_cast<uint4*>(out) = lo[e];
+      *reinterpret_cast<uint4*>(out + 64) = hi[e];
+    }
+  }
+}
+
+// fp16 pools.  Eight lanes take E heads of a token: of its queries, or of its keys and values
+template <int E>
 __global__ void __launch_bounds__(THREADS)
 page_append_kernel(const Args a, int64_t units) {
   asm volatile("griddepcontrol.launch_dependents;");
@@ -125,26 +194,9 @@ page_append_kernel(const Args a, int64_t units) {
   const int64_t unit = (int64_t)blockIdx.x * UNITS + (threadIdx.x >> 3);
   const int i = threadIdx.x & 7;
   if (unit >= units) return;
-  const int heads = a.H + 2 * a.Hkv, t = (int)(unit / heads);
-  int h = (int)(unit - (int64_t)t * heads);
-  if (h < a.H) return rotate_query(a, t, h, i);
-  h -= a.H;
-  const bool is_k = h < a.Hkv;
-  if (!is_k) h -= a.Hkv;
-  const __half* const x = is_k ? a.k + t * a.k_stride : a.v + t * a.v_stride;
-  Row r = load_row(x + h * ATTN_D, i);
-  int seq;
-  int64_t at;
-  if (!token_of(a, t, seq, at)) return;
-  const int64_t page = at / a.tbl.page_size;
-  const int id = page_id(a, seq, page);
-  if (id < 0) return;
-  if (is_k && a.cos_tbl) rotate(r, a, at, i);
-  const int64_t slot = (int64_t)id * a.tbl.page_size + (at - page * a.tbl.page_size);
-  if (slot >= a.P) return;                                        // a pool may end inside its last page
-  __half* const out = reinterpret_cast<__half*>(is_k ? a.kpool : a.vpool) + ((int64_t)h * a.P + slot) * ATTN_D;
-  *reinterpret_cast<uint4*>(out + 8 * i) = pack8(r.lo);
-  *reinterpret_cast<uint4*>(out + 64 + 8 * i) = pack8(r.hi);
+  const int nq = (a.H + E - 1) / E, n = nq + (2 * a.Hkv + E - 1) / E, t = (int)(unit / n), part = (int)(unit - (int64_t)t * n);
+  if (part < nq) rotate_queries<E>(a, t, part * E, min((part + 1) * E, a.H), i);
+  else append_heads<E>(a, t, (part - nq) * E, min((part - nq + 1) * E, 2 * a.Hkv), i);
 }
 
 // Eight values as codes of scale 1 / inv
@@ -183,21 +235,22 @@ __device__ __forceinline__ uint2 recode8(uint2 c, float ratio) {
   return code8<T>(f, ratio);
 }
 
-// 8-bit pools.  Blocks from q_blocks on have a page of a sequence and a kv head each: the first two warps its keys, the others its
+// 8-bit pools.  The first blocks, which take longest, have a page of a sequence and a kv head each: the first two warps its keys, the others its
 // values.  A sequence whose new rows are [o, e) touches at most (e - o) / page_size + 2 pages, so that its blocks can begin at
 // o / page_size + 2 * sequence, and nobody counts pages.
-template <int T>
-__global__ void __launch_bounds__(THREADS)
+template <int T, int E>
+__global__ void __launch_bounds__(THREADS, E > 1 ? 8 : 7)
 page_append_8bit_kernel(const Args a) {
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int i = threadIdx.x & 7;
-  if (blockIdx.x < a.q_blocks) {
-    const int64_t unit = (int64_t)blockIdx.x * UNITS + (threadIdx.x >> 3);
-    if (unit < (int64_t)a.T * a.H) rotate_query(a, (int)(unit / a.H), (int)(unit % a.H), i);
+  if (blockIdx.x >= a.page_blocks) {
+    const int64_t unit = (int64_t)(blockIdx.x - a.page_blocks) * UNITS + (threadIdx.x >> 3);
+    const int nq = (a.H + E - 1) / E, part = (int)(unit % nq);
+    if (unit < (int64_t)a.T * nq) rotate_queries<E>(a, (int)(unit / nq), part * E, min((part + 1) * E, a.H), i);
     return;
   }
-  const unsigned block = blockIdx.x - a.q_blocks;
+  const unsigned block = blockIdx.x;
   const int h = (int)(block % a.Hkv), ps = a.tbl.page_size;
   const int64_t unit = block / a.Hkv;
   int seq, first, end;                     // the sequence's new rows
@@ -229,7 +282,7 @@ page_append_8bit_kernel(const Args a) {
 
   const auto value = [&](int j) {
     Row r = load_row(x + j * ld, i);
-    if (is_k && a.cos_tbl) rotate(r, a, from_at + j, i);
+    if (is_k && a.cos_tbl) rotate(r, turn_of(a, from_at + j, i));
     return r;
   };
   unsigned most = 0;                       // bits of the largest magnitude; what is not finite is above all that is
@@ -307,17 +360,21 @@ extern "C" int q40_page_append(const void* page_tbl, int idx_bytes, int64_t tbl_
   a.B = B; a.T = T; a.H = H; a.Hkv = Hkv;
   const cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
+  // one head a lane group while that leaves few of them: a decode step is over when its longest chain of loads is
+  const bool many = (int64_t)T * (H + 2 * Hkv) > MANY;
+  const int each = many ? EACH : 1, nq = (H + each - 1) / each;
   if (cache_type == CACHE_F16) {
-    const int64_t units = (int64_t)T * (H + 2 * Hkv), blocks = (units + UNITS - 1) / UNITS;
+    const int64_t units = (int64_t)T * (nq + (2 * Hkv + each - 1) / each), blocks = (units + UNITS - 1) / UNITS;
     if (blocks > 0x7fffffffLL) return Q40_E_SHAPE;
-    e = q40_launch_pdl(page_append_kernel, dim3((unsigned)blocks), dim3(THREADS), 0, st, a, units);
+    e = q40_launch_pdl(many ? page_append_kernel<EACH> : page_append_kernel<1>, dim3((unsigned)blocks), dim3(THREADS), 0, st, a, units);
   } else {
-    const int64_t qb = ((int64_t)T * H + UNITS - 1) / UNITS, units = offsets ? T / page_size + 2 * (int64_t)B : B;
+    const int64_t qb = ((int64_t)T * nq + UNITS - 1) / UNITS, units = offsets ? T / page_size + 2 * (int64_t)B : B;
     if (qb + units * Hkv > 0x7fffffffLL) return Q40_E_SHAPE;
-    a.q_blocks = (unsigned)qb;
+    a.page_blocks = (unsigned)(units * Hkv);
     const dim3 grid((unsigned)(qb + units * Hkv));
-    e = cache_type == CACHE_I8 ? q40_launch_pdl(page_append_8bit_kernel<CACHE_I8>, grid, dim3(THREADS), 0, st, a)
-                               : q40_launch_pdl(page_append_8bit_kernel<CACHE_E4M3>, grid, dim3(THREADS), 0, st, a);
+    const auto kernel = cache_type == CACHE_I8 ? (many ? page_append_8bit_kernel<CACHE_I8, EACH> : page_append_8bit_kernel<CACHE_I8, 1>)
+                                               : (many ? page_append_8bit_kernel<CACHE_E4M3, EACH> : page_append_8bit_kernel<CACHE_E4M3, 1>);
+    e = q40_launch_pdl(kernel, grid, dim3(THREADS), 0, st, a);
   }
   return e == cudaSuccess ? Q40_OK : (int)e;
 }
