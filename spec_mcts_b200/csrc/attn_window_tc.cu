@@ -107,37 +107,51 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // The lowest n bits, of any n
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
 
-// What a CTA goes through, and who takes part in it
+// Which tiles of keys (by number: keys BK t ..) a tile of queries sees some keys of, and all of them.  (Comparisons of numbers that are made once: the
+// thread that issues MMAs asks for every tile, and a few hundred cycles of it were a tenth of the time)
+struct Sees {
+  int last, from, sinks, all_last, all_from, all_sinks;
+  // queries at positions first .. end, none if end < first
+  __host__ __device__ __forceinline__ Sees(int first, int end, int window, int n_sinks) {
+    last = end >= first ? end / BK : -1;
+    from = first - window + 1 > 0 ? (first - window + 1) / BK : 0;
+    sinks = (n_sinks + BK - 1) / BK;
+    all_last = (first + 1) / BK - 1;
+    all_from = end - window + 1 > 0 ? (end - window + BK) / BK : 0;
+    all_sinks = n_sinks / BK;
+  }
+  __host__ __device__ __forceinline__ bool some(int t) const { return t <= last && (t >= from || t < sinks); }
+  __host__ __device__ __forceinline__ bool all(int t) const { return t <= all_last && (t >= all_from || t < all_sinks); }
+  __host__ __device__ __forceinline__ bool part(int t) const { return some(t) && !all(t); }
+};
+
+// The tiles of keys that a CTA goes through, tile(0) to tile(n - 1): those that one of its queries sees, or a split's share of them
 struct Tiles {
   int p_first, p_last;               // positions of the CTA's first and last query
-  int window, sinks, t_first, t_from;
-  int j0, n;                         // this CTA's tiles of the block's
+  int t_first, t_from, j0, n;
   __host__ __device__ __forceinline__ Tiles(const Args& a, int row0, int split) {
     p_first = a.offset + row0;
     p_last = (p_first + 2 * BQ < a.offset + a.S ? p_first + 2 * BQ : a.offset + a.S) - 1;
-    window = a.window;
-    sinks = a.sinks;
-    const int from = p_first - window + 1 > 0 ? p_first - window + 1 : 0, first = sinks < from ? sinks : from;
+    const int from = p_first - a.window + 1 > 0 ? p_first - a.window + 1 : 0, first = a.sinks < from ? a.sinks : from;
     t_first = (first + BK - 1) / BK;
     t_from = from / BK > t_first ? from / BK : t_first;
     const int all = t_first + p_last / BK + 1 - t_from;
     j0 = (int)((int64_t)all * split / a.splits);
     n = (int)((int64_t)all * (split + 1) / a.splits) - j0;
   }
-  __device__ __forceinline__ int key0(int j) const { return (j + j0 < t_first ? j + j0 : j + j0 - t_first + t_from) * BK; }
-  // of tile i of the queries: its first position, whether it has any, sees some keys of the tile from key k, or all of them
+  __device__ __forceinline__ int tile(int j) const { return j + j0 < t_first ? j + j0 : j + j0 - t_first + t_from; }
+  // the CTA's tile i of queries
   __device__ __forceinline__ int first_of(int i) const { return p_first + i * BQ; }
   __device__ __forceinline__ bool has(int i) const { return first_of(i) <= p_last; }
-  __device__ __forceinline__ bool sees(int i, int k) const {
-    return has(i) && k <= min(first_of(i) + BQ - 1, p_last) && (k + BK > first_of(i) - window + 1 || k < sinks);
-  }
-  __device__ __forceinline__ bool sees_all(int i, int k) const {
-    return k + BK <= first_of(i) + 1 && (k > min(first_of(i) + BQ - 1, p_last) - window || k + BK <= sinks);
-  }
-  __device__ __forceinline__ bool masked(int k) const { return (sees(0, k) && !sees_all(0, k)) || (sees(1, k) && !sees_all(1, k)); }
+  __device__ __forceinline__ Sees sees(int i, const Args& a) const { return Sees(first_of(i), min(first_of(i) + BQ - 1, p_last), a.window, a.sinks); }
 };
 
 __global__ void __launch_bounds__(THREADS, 1)
@@ -155,13 +169,14 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
   const int blk = blocks - 1 - (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H), hk = h / (a.H / a.Hkv);
   const int row0 = blk * 2 * BQ;
   const Tiles tiles(a, row0, blockIdx.y);
+  const Sees sees[2] = {tiles.sees(0, a), tiles.sees(1, a)};       // (in front of the waits)
 
   if (tid == 0) {
     *s_failed = 0;
     *s_taken_out = 0;
     for (int i = 0; i < SLOTS; ++i) s_requested[i] = 0;
     for (int i = 0; i < BARS; ++i) {
-      const int count = i >= P_HALF && i < P_FULL + 2 ? 4 : (i >= READY && i < READY + LOOKED) || (i >= EMPTY && i < EMPTY + SLOTS) ? 2 : 1;
+      const int count = i >= P_HALF && i < P_FULL + 2 ? 4 : i >= READY && i < READY + LOOKED ? 2 : 1;
       mbar_init(bar(i), count);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -184,21 +199,22 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
 
   bool failed = false;
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int i = warp >> 2, row = (warp & 3) * 32 + lane, p = tiles.first_of(i) + row;
     const uint32_t quad = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + quad + 128 * i, o_at = s_at + 256;
+    const Sees mine = i ? sees[1] : sees[0];
     float m = -3e38f, l = 0.f;
     int n = 0;                                         // tiles of keys so far
     for (int j = 0; j < tiles.n; ++j) {
-      const int key0 = tiles.key0(j);
-      if (!tiles.sees(i, key0)) continue;
+      const int tile = tiles.tile(j), key0 = tile * BK;
+      if (!mine.some(tile)) continue;
       if (!all_wait(bar(S_FULL + i), n & 1)) { failed = true; break; }
       fence_after();
       float s[BK];
 #pragma unroll
       for (int c = 0; c < 4; ++c) ld32(s_at + 32 * c, s + 32 * c);
       wait_ld();
-      if (!tiles.sees_all(i, key0)) {
+      if (!mine.all(tile)) {
         const int last = p - key0, from = p - a.window - key0, first = a.sinks - key0;      // seen: places <= last that are > from or < first
 #pragma unroll
         for (int c = 0; c < BK; c += 32) {
@@ -210,8 +226,12 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
       }
       float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int c = 4; c < BK; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-      const float most = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+      for (int c = 4; c < BK - 4; c += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[BK - 4 + e]);
+      const float most = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * a.scale_log2;
       const bool passes = most > m + STAY;
       if (__any_sync(0xffffffffu, passes)) {
         const float now = passes ? most : m, corr = fmaxf(ex2(m - now), 1.17549435e-38f);      // (never 0: infinities stay)
@@ -275,8 +295,8 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
             for (int e = 0; e < 32; ++e) o[e] = 0.f;
           if (taken_out && there)                      // rare, and slow
             for (int j = 0; j < tiles.n; ++j) {
-              const int key0 = tiles.key0(j);
-              if (!tiles.masked(key0)) continue;
+              const int tile = tiles.tile(j), key0 = tile * BK;
+              if (!sees[0].part(tile) && !sees[1].part(tile)) continue;
               for (int k = key0; k < min(key0 + BK, p + 1); ++k) {
                 if (p - k >= a.window && k >= a.sinks) continue;
                 const __half* const v = a.v + (int64_t)k * a.ldv + hk * ATTN_D + 32 * c;
@@ -305,22 +325,23 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 8) {
       if (elect_one()) {
         bool pending[2] = {false, false}, q_there[2] = {false, false};      // O += P V of the tile before is still to come
         int steps[2] = {0, 0}, slot = 0, looked = 0, v_slot = 0;
-        bool v_masked = false;                         // ... whose values are in v_slot, the looked-th to be looked through
+        bool v_masked = false, v_there = false;        // the values are in v_slot, the looked-th to be looked through; they have been waited for
         uint32_t phases = 0;                           // of FULL, a bit a slot
         const auto full = [&](int at) { return mbar_wait(bar(FULL + at), (phases >> at) & 1); };
+        const auto values_there = [&]() {
+          if (v_there) return true;
+          v_there = true;
+          if (!v_masked) return full(v_slot);
+          return mbar_wait(bar(LOOK + looked % LOOKED), (looked / LOOKED) & 1) && mbar_wait(bar(READY + looked % LOOKED), (looked / LOOKED) & 1);
+        };
         const auto product = [&](int i) {
           pending[i] = false;
-          if (!mbar_wait(bar(P_HALF + i), (steps[i] - 1) & 1)) return false;
-          if (v_masked) {
-            if (!mbar_wait(bar(LOOK + looked % LOOKED), (looked / LOOKED) & 1) || !mbar_wait(bar(READY + looked % LOOKED), (looked / LOOKED) & 1)) return false;
-          } else if (!full(v_slot)) {
-            return false;
-          }
+          if (!values_there() || !mbar_wait(bar(P_HALF + i), (steps[i] - 1) & 1)) return false;
           fence_after();
           const uint64_t b = values_desc(base + AT_RING + v_slot * TILE);
 #pragma unroll
@@ -331,40 +352,40 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
 #pragma unroll
           for (int ks = BK / 32; ks < BK / 16; ++ks)
             ttc::mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * ks, b + (uint64_t)((ks * 2048) >> 4), IDESC | VALUES_MAJOR, 1u);
-          ttc::commit(bar(EMPTY + v_slot));
           return true;
         };
         for (int j = 0; j < tiles.n && !failed; ++j) {
-          const int key0 = tiles.key0(j), next = slot + 1 == SLOTS ? 0 : slot + 1;       // keys in `slot`, values in the next
+          const int tile = tiles.tile(j), next = slot + 1 == SLOTS ? 0 : slot + 1;       // keys in `slot`, values in the next
           if (!full(slot)) { failed = true; break; }
-          for (int i = 0; i < 2 && !failed; ++i) {
-            if (pending[i] && !product(i)) { failed = true; break; }
-            if (tiles.sees(i, key0)) {
-              if (!q_there[i]) {
-                if (!mbar_wait(bar(Q_FULL + i), 0)) { failed = true; break; }
-                q_there[i] = true;
-              }
-              fence_after();
-              const uint64_t qd = ttc::kmajor_desc(base + AT_Q + i * TILE), kd = ttc::kmajor_desc(base + AT_RING + slot * TILE);
 #pragma unroll
-              for (int ks = 0; ks < ATTN_D / 16; ++ks) {
-                const uint64_t off = (uint64_t)(((ks >> 2) * HALF + (ks & 3) * 32) >> 4);
-                mma_ss(tmem + 128 * i, qd + off, kd + off, IDESC, ks > 0 ? 1u : 0u);
-              }
-              ttc::commit(bar(S_FULL + i));
-              pending[i] = true;
-              ++steps[i];
-            } else {
-              // not a plain arrival: it would count for what was in the slot before while a product on that is on its way
-              ttc::commit(bar(EMPTY + next));
+          for (int i = 0; i < 2; ++i) {
+            if (failed) break;
+            if (pending[i] && !product(i)) { failed = true; break; }
+            if (i == 1 && j > 0) ttc::commit(bar(EMPTY + v_slot));
+            if (!sees[i].some(tile)) continue;
+            if (!q_there[i]) {
+              if (!mbar_wait(bar(Q_FULL + i), 0)) { failed = true; break; }
+              q_there[i] = true;
             }
-            ttc::commit(bar(EMPTY + slot));
+            fence_after();
+            const uint64_t qd = ttc::kmajor_desc(base + AT_Q + i * TILE), kd = ttc::kmajor_desc(base + AT_RING + slot * TILE);
+#pragma unroll
+            for (int ks = 0; ks < ATTN_D / 16; ++ks) {
+              const uint64_t off = (uint64_t)(((ks >> 2) * HALF + (ks & 3) * 32) >> 4);
+              mma_ss(tmem + 128 * i, qd + off, kd + off, IDESC, ks > 0 ? 1u : 0u);
+            }
+            ttc::commit(bar(S_FULL + i));
+            pending[i] = true;
+            ++steps[i];
           }
+          if (failed) break;
+          ttc::commit(bar(EMPTY + slot));
           if (v_masked) ++looked;
           else if (j > 0) phases ^= 1u << v_slot;
           phases ^= 1u << slot;
           v_slot = next;
-          v_masked = tiles.masked(key0);
+          v_masked = sees[0].part(tile) || sees[1].part(tile);
+          v_there = false;
           slot = next + 1 == SLOTS ? 0 : next + 1;
         }
         for (int i = 0; i < 2; ++i) {
@@ -385,12 +406,12 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
         int slot = 0, looked = 0;
         uint32_t full = 0;                             // phases of FULL, a bit a slot
         for (int x = 0; x < 2 * tiles.n; ++x) {        // keys of tile x / 2, or its values
-          const int key0 = tiles.key0(x >> 1);
+          const int tile = tiles.tile(x >> 1);
           if (x >= SLOTS && !mbar_wait(bar(EMPTY + slot), (x / SLOTS - 1) & 1)) { failed = true; break; }
-          const bool look = (x & 1) && tiles.masked(key0);
+          const bool look = (x & 1) && (sees[0].part(tile) || sees[1].part(tile));
           const int which = look ? LOOK + looked % LOOKED : FULL + slot;
           s_requested[slot] = 2 * which + 1 + (look ? (looked / LOOKED) & 1 : (full >> slot) & 1);
-          copy(x & 1 ? &maps.v : &maps.k, base + AT_RING + slot * TILE, hk, key0, bar(which));
+          copy(x & 1 ? &maps.v : &maps.k, base + AT_RING + slot * TILE, hk, tile * BK, bar(which));
           if (look) ++looked;
           else full ^= 1u << slot;
           if (x == 0 && tiles.has(1)) copy(&maps.q, base + AT_Q + TILE, h, row0 + BQ, bar(Q_FULL + 1));
@@ -402,7 +423,8 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
       const int at = (warp - 10) * 32 + lane;
       int looked = 0;
       for (int j = 0; j < tiles.n; ++j) {
-        if (!tiles.masked(tiles.key0(j))) continue;
+        const int tile = tiles.tile(j);
+        if (!sees[0].part(tile) && !sees[1].part(tile)) continue;
         const int which = looked % LOOKED;
         if (!all_wait(bar(LOOK + which), (looked / LOOKED) & 1)) { failed = true; break; }
         ++looked;
