@@ -33,15 +33,9 @@ using ttc::mbar_expect_tx;
 using ttc::mbar_init;
 using ttc::mbar_wait;
 
-constexpr int BQ = 128, BK = 128, THREADS = 384;
+constexpr int BQ = 128, BK = 128, THREADS = 384;            // queries of a CTA's tile, keys of a tile
 constexpr uint32_t TILE = BK * ATTN_D * 2;               // 32 KB: two blocks of 64 dims, rows of 128 bytes
 constexpr uint32_t HALF = TILE / 2;
-constexpr int SLOTS = 5;                        // of the ring that keys and values go through in turn
-constexpr int LOOKED = 4;                       // barriers of values that are looked through: at most three of them are in the ring
-constexpr uint32_t AT_Q = 0, AT_RING = 2 * TILE, AT_BARS = AT_RING + SLOTS * TILE;
-enum Bar { Q_FULL, FULL = Q_FULL + 2, EMPTY = FULL + SLOTS, LOOK = EMPTY + SLOTS, READY = LOOK + LOOKED, S_FULL = READY + LOOKED,
-           P_HALF = S_FULL + 2, P_FULL = P_HALF + 2, O_DONE = P_FULL + 2, ALL_DONE = O_DONE + 2, BARS };
-constexpr uint32_t SMEM = AT_BARS + 8 * BARS + 48 + 1024;       // (1024: the alignment)
 constexpr float STAY = 8.f;
 
 struct Maps { CUtensorMap q, k, v; };
@@ -137,9 +131,10 @@ struct Sees {
 struct Tiles {
   int p_first, p_last;               // positions of the CTA's first and last query
   int t_first, t_from, j0, n;
-  __host__ __device__ __forceinline__ Tiles(const Args& a, int row0, int split) {
+  // `rows` queries from row0 on
+  __host__ __device__ __forceinline__ Tiles(const Args& a, int row0, int rows, int split) {
     p_first = a.offset + row0;
-    p_last = (p_first + 2 * BQ < a.offset + a.S ? p_first + 2 * BQ : a.offset + a.S) - 1;
+    p_last = (p_first + rows < a.offset + a.S ? p_first + rows : a.offset + a.S) - 1;
     const int from = p_first - a.window + 1 > 0 ? p_first - a.window + 1 : 0, first = a.sinks < from ? a.sinks : from;
     t_first = (first + BK - 1) / BK;
     t_from = from / BK > t_first ? from / BK : t_first;
@@ -148,11 +143,160 @@ struct Tiles {
     n = (int)((int64_t)all * (split + 1) / a.splits) - j0;
   }
   __device__ __forceinline__ int tile(int j) const { return j + j0 < t_first ? j + j0 : j + j0 - t_first + t_from; }
-  // the CTA's tile i of queries
-  __device__ __forceinline__ int first_of(int i) const { return p_first + i * BQ; }
-  __device__ __forceinline__ bool has(int i) const { return first_of(i) <= p_last; }
-  __device__ __forceinline__ Sees sees(int i, const Args& a) const { return Sees(first_of(i), min(first_of(i) + BQ - 1, p_last), a.window, a.sinks); }
+  // `count` queries from the first-th on
+  __host__ __device__ __forceinline__ Sees sees(int first, int count, const Args& a) const {
+    const int end = p_first + first + count - 1;
+    return Sees(p_first + first, end < p_last ? end : p_last, a.window, a.sinks);
+  }
 };
+
+// A row's maximum, log2, and sum so far, and its step: the scores of 128 keys from key0 on, at s_at, become weights over their place, in two halves, each of
+// which arrive() tells of; O, at o_at, is scaled where the maximum moves
+struct Row {
+  float m = -3e38f, l = 0.f;
+  int n = 0;                         // tiles of keys so far
+  template <class Arrive>
+  __device__ __forceinline__ void step(const Args& a, uint32_t s_at, uint32_t o_at, int p, int key0, bool masked, int lane, Arrive arrive) {
+    float s[BK];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) ld32(s_at + 32 * c, s + 32 * c);
+    wait_ld();
+    if (masked) {
+      const int last = p - key0, from = p - a.window - key0, first = a.sinks - key0;      // seen: places <= last that are > from or < first
+#pragma unroll
+      for (int c = 0; c < BK; c += 32) {
+        const uint32_t seen = below(last + 1 - c) & (~below(from + 1 - c) | below(first - c));
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (!(seen & (1u << e))) s[c + e] = -CUDART_INF_F;
+      }
+    }
+    float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+    for (int c = 4; c < BK - 4; c += 8)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[BK - 4 + e]);
+    const float most = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * a.scale_log2;
+    const bool passes = most > m + STAY;
+    if (__any_sync(0xffffffffu, passes)) {
+      const float now = passes ? most : m, corr = fmaxf(ex2(m - now), 1.17549435e-38f);      // (never 0: infinities stay)
+      m = now;
+      l *= corr;
+      if (n > 0) {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float o[32];
+          ld32(o_at + 32 * c, o);
+          wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= corr;
+          st32(o_at + 32 * c, reinterpret_cast<const uint32_t*>(o));
+        }
+        wait_st();
+      }
+    }
+    const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), m2 = pack2(-m, -m);
+    uint64_t sum[2] = {pack2(l, 0.f), 0};
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      uint32_t pk[32];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        float x, y;
+        unpack2(fma2(pack2(s[64 * c + 2 * e], s[64 * c + 2 * e + 1]), scale2, m2), x, y);
+        x = ex2(x);
+        y = ex2(y);
+        sum[e & 1] = add2(sum[e & 1], pack2(x, y));
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[e]) : "f"(y), "f"(x));
+      }
+      st32(s_at + 32 * c, pk);
+      wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) arrive(c);
+    }
+    float x, y;
+    unpack2(add2(sum[0], sum[1]), x, y);
+    l = x + y;
+    ++n;
+  }
+  // ... and its output, or a split's partial result.  taken_out: values that are not finite were taken out of tiles that `sees` say are seen in part
+  __device__ __forceinline__ void write(const Args& a, uint32_t o_at, int p, int h, int hk, const Tiles& tiles, const Sees (&sees)[2], bool taken_out) const {
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    const bool there = p <= tiles.p_last;
+    // (rows by way of shared memory, 256 bytes of one at a time: no faster)
+    __half* const out = a.o + (int64_t)(p - a.offset) * a.ldo + h * ATTN_D;
+    const int64_t part_at = ((int64_t)blockIdx.y * a.S + (p - a.offset)) * a.H + h;
+    if (a.splits > 1 && there) a.pml[part_at] = make_float2(m, l);
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+      float o[32];
+      ld32(o_at + 32 * c, o);
+      wait_ld();
+      if (n == 0)                                  // none of the split's keys: nothing has been written there
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+      if (taken_out && there)                      // rare, and slow
+        for (int j = 0; j < tiles.n; ++j) {
+          const int tile = tiles.tile(j), key0 = tile * BK;
+          if (!sees[0].part(tile) && !sees[1].part(tile)) continue;
+          for (int k = key0; k < min(key0 + BK, p + 1); ++k) {
+            if (p - k >= a.window && k >= a.sinks) continue;
+            const __half* const v = a.v + (int64_t)k * a.ldv + hk * ATTN_D + 32 * c;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (not_finite(v[e])) o[e] += __half2float(v[e]);
+          }
+        }
+      if (there && a.splits > 1) {
+        float4* const part = reinterpret_cast<float4*>(a.po + part_at * ATTN_D + 32 * c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+      } else if (there) {
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = h2_as_u32(__floats2half2_rn(o[2 * e] * inv, o[2 * e + 1] * inv));
+        if (a.wide_out) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) reinterpret_cast<uint4*>(out + 32 * c)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) reinterpret_cast<uint32_t*>(out + 32 * c)[e] = w[e];
+        }
+      }
+    }
+  }
+};
+
+// Values that are not finite, among `n` pieces of 16 bytes, become zeros, by 64 threads at 0 .. 63 of two warps; whether this warp found any.  (64 bytes of eight
+// values a thread and step: magnitudes by maxima of pairs, above all of which is what is not finite)
+__device__ __forceinline__ bool take_out(uint4* v, int n, int at) {
+  __half2 most[2] = {u32_as_h2(0), u32_as_h2(0)};
+#pragma unroll 8
+  for (int c = at; c < n; c += 64) {
+    const uint4 x = v[c];
+    most[0] = __hmax2_nan(__hmax2_nan(most[0], __habs2(u32_as_h2(x.x))), __habs2(u32_as_h2(x.y)));
+    most[1] = __hmax2_nan(__hmax2_nan(most[1], __habs2(u32_as_h2(x.z))), __habs2(u32_as_h2(x.w)));
+  }
+  const __half2 top = __hmax2_nan(most[0], most[1]);
+  if (!__any_sync(0xffffffffu, not_finite(__low2half(top)) || not_finite(__high2half(top)))) return false;
+  __half* const x = reinterpret_cast<__half*>(v);
+  for (int c = at; c < n; c += 64)
+    for (int e = 0; e < 8; ++e)
+      if (not_finite(x[8 * c + e])) x[8 * c + e] = __ushort_as_half(0);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");           // the MMA reads them
+  return true;
+}
+
+constexpr int SLOTS = 5;                        // of the ring that keys and values go through in turn
+constexpr int LOOKED = 4;                       // barriers of values that are looked through: at most three of them are in the ring
+constexpr uint32_t AT_Q = 0, AT_RING = 2 * TILE, AT_BARS = AT_RING + SLOTS * TILE;
+enum Bar { Q_FULL, FULL = Q_FULL + 2, EMPTY = FULL + SLOTS, LOOK = EMPTY + SLOTS, READY = LOOK + LOOKED, S_FULL = READY + LOOKED,
+           P_HALF = S_FULL + 2, P_FULL = P_HALF + 2, O_DONE = P_FULL + 2, ALL_DONE = O_DONE + 2, BARS };
+static_assert(BARS <= 32, "a lane makes a barrier");
+constexpr uint32_t SMEM = AT_BARS + 8 * BARS + 48 + 1024;       // (1024: the alignment)
 
 __global__ void __launch_bounds__(THREADS, 1)
 attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err) {
@@ -168,23 +312,30 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
   const int blocks = (a.S + 2 * BQ - 1) / (2 * BQ);
   const int blk = blocks - 1 - (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H), hk = h / (a.H / a.Hkv);
   const int row0 = blk * 2 * BQ;
-  const Tiles tiles(a, row0, blockIdx.y);
-  const Sees sees[2] = {tiles.sees(0, a), tiles.sees(1, a)};       // (in front of the waits)
+  const Tiles tiles(a, row0, 2 * BQ, blockIdx.y);
+  const Sees sees[2] = {tiles.sees(0, BQ, a), tiles.sees(BQ, BQ, a)};       // (in front of the waits)
 
-  if (tid == 0) {
-    *s_failed = 0;
-    *s_taken_out = 0;
-    for (int i = 0; i < SLOTS; ++i) s_requested[i] = 0;
-    for (int i = 0; i < BARS; ++i) {
-      const int count = i >= P_HALF && i < P_FULL + 2 ? 4 : i >= READY && i < READY + LOOKED ? 2 : 1;
-      mbar_init(bar(i), count);
-    }
+  const auto copy = [&](const CUtensorMap* map, uint32_t dst, int head, int row, uint32_t full) {
+    mbar_expect_tx(full, TILE);
+    ttc::tma_2d(dst, map, head * ATTN_D, row, full);
+    ttc::tma_2d(dst + HALF, map, head * ATTN_D + 64, row, full);
+  };
+  if (warp == 9) {
+    if (lane < BARS) mbar_init(bar(lane), lane >= P_HALF && lane < P_FULL + 2 ? 4 : lane >= READY && lane < READY + LOOKED ? 2 : 1);
+    if (lane < SLOTS) s_requested[lane] = 0;
+    if (lane == 0) *s_failed = *s_taken_out = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
-  if (warp == 9 && lane < 3) {
-    const CUtensorMap* const map = lane == 0 ? &maps.q : lane == 1 ? &maps.k : &maps.v;
-    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+    __syncwarp();
+    // the first queries and keys are on their way while the others meet
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (elect_one() && tiles.n > 0) {
+      copy(&maps.q, base + AT_Q, h, row0, bar(Q_FULL));
+      s_requested[0] = 2 * FULL + 1;
+      copy(&maps.k, base + AT_RING, hk, tiles.tile(0) * BK, bar(FULL));
+      if (sees[1].last >= 0) copy(&maps.q, base + AT_Q + TILE, h, row0 + BQ, bar(Q_FULL + 1));
+    }
+    __syncwarp();
   }
   if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ttc::smem_u32(tmem_slot)), "n"(512));
@@ -200,129 +351,21 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
   bool failed = false;
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int i = warp >> 2, row = (warp & 3) * 32 + lane, p = tiles.first_of(i) + row;
+    const int i = warp >> 2, p = tiles.p_first + i * BQ + (warp & 3) * 32 + lane;
     const uint32_t quad = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + quad + 128 * i, o_at = s_at + 256;
     const Sees mine = i ? sees[1] : sees[0];
-    float m = -3e38f, l = 0.f;
-    int n = 0;                                         // tiles of keys so far
+    Row row;
     for (int j = 0; j < tiles.n; ++j) {
-      const int tile = tiles.tile(j), key0 = tile * BK;
+      const int tile = tiles.tile(j);
       if (!mine.some(tile)) continue;
-      if (!all_wait(bar(S_FULL + i), n & 1)) { failed = true; break; }
+      if (!all_wait(bar(S_FULL + i), row.n & 1)) { failed = true; break; }
       fence_after();
-      float s[BK];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) ld32(s_at + 32 * c, s + 32 * c);
-      wait_ld();
-      if (!mine.all(tile)) {
-        const int last = p - key0, from = p - a.window - key0, first = a.sinks - key0;      // seen: places <= last that are > from or < first
-#pragma unroll
-        for (int c = 0; c < BK; c += 32) {
-          const uint32_t seen = below(last + 1 - c) & (~below(from + 1 - c) | below(first - c));
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!(seen & (1u << e))) s[c + e] = -CUDART_INF_F;
-        }
-      }
-      float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-      for (int c = 4; c < BK - 4; c += 8)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[BK - 4 + e]);
-      const float most = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * a.scale_log2;
-      const bool passes = most > m + STAY;
-      if (__any_sync(0xffffffffu, passes)) {
-        const float now = passes ? most : m, corr = fmaxf(ex2(m - now), 1.17549435e-38f);      // (never 0: infinities stay)
-        m = now;
-        l *= corr;
-        if (n > 0) {
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            float o[32];
-            ld32(o_at + 32 * c, o);
-            wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= corr;
-            st32(o_at + 32 * c, reinterpret_cast<const uint32_t*>(o));
-          }
-          wait_st();
-        }
-      }
-      const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), m2 = pack2(-m, -m);
-      uint64_t sum[2] = {pack2(l, 0.f), 0};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float x, y;
-          unpack2(fma2(pack2(s[64 * c + 2 * e], s[64 * c + 2 * e + 1]), scale2, m2), x, y);
-          x = ex2(x);
-          y = ex2(y);
-          sum[e & 1] = add2(sum[e & 1], pack2(x, y));
-          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[e]) : "f"(y), "f"(x));
-        }
-        st32(s_at + 32 * c, pk);
-        wait_st();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar((c ? P_FULL : P_HALF) + i));
-      }
-      float x, y;
-      unpack2(add2(sum[0], sum[1]), x, y);
-      l = x + y;
-      ++n;
+      row.step(a, s_at, o_at, p, tile * BK, !mine.all(tile), lane, [&](int half) { mbar_arrive(bar((half ? P_FULL : P_HALF) + i)); });
     }
-    if (!failed && tiles.has(i)) {
+    if (!failed && mine.last >= 0) {
       if (!all_wait(bar(O_DONE + i), 0)) failed = true;
       fence_after();
-      if (!failed) {
-        const float inv = l != 0.f ? 1.f / l : 0.f;
-        const bool there = p <= tiles.p_last, taken_out = *s_taken_out;
-        // (rows by way of shared memory, 256 bytes of one at a time: no faster)
-        __half* const out = a.o + (int64_t)(p - a.offset) * a.ldo + h * ATTN_D;
-        const int64_t part_at = ((int64_t)blockIdx.y * a.S + (p - a.offset)) * a.H + h;
-        if (a.splits > 1 && there) a.pml[part_at] = make_float2(m, l);
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float o[32];
-          ld32(o_at + 32 * c, o);
-          wait_ld();
-          if (n == 0)                                  // none of the split's keys: nothing has been written there
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0.f;
-          if (taken_out && there)                      // rare, and slow
-            for (int j = 0; j < tiles.n; ++j) {
-              const int tile = tiles.tile(j), key0 = tile * BK;
-              if (!sees[0].part(tile) && !sees[1].part(tile)) continue;
-              for (int k = key0; k < min(key0 + BK, p + 1); ++k) {
-                if (p - k >= a.window && k >= a.sinks) continue;
-                const __half* const v = a.v + (int64_t)k * a.ldv + hk * ATTN_D + 32 * c;
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (not_finite(v[e])) o[e] += __half2float(v[e]);
-              }
-            }
-          if (there && a.splits > 1) {
-            float4* const part = reinterpret_cast<float4*>(a.po + part_at * ATTN_D + 32 * c);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) part[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-          } else if (there) {
-            uint32_t w[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) w[e] = h2_as_u32(__floats2half2_rn(o[2 * e] * inv, o[2 * e + 1] * inv));
-            if (a.wide_out) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) reinterpret_cast<uint4*>(out + 32 * c)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) reinterpret_cast<uint32_t*>(out + 32 * c)[e] = w[e];
-            }
-          }
-        }
-      }
+      if (!failed) row.write(a, o_at, p, h, hk, tiles, sees, *s_taken_out);
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
@@ -397,15 +440,9 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
       __syncwarp();
     } else if (warp == 9) {
       if (elect_one()) {
-        const auto copy = [&](const CUtensorMap* map, uint32_t dst, int head, int row, uint32_t full) {
-          mbar_expect_tx(full, TILE);
-          ttc::tma_2d(dst, map, head * ATTN_D, row, full);
-          ttc::tma_2d(dst + HALF, map, head * ATTN_D + 64, row, full);
-        };
-        copy(&maps.q, base + AT_Q, h, row0, bar(Q_FULL));
-        int slot = 0, looked = 0;
-        uint32_t full = 0;                             // phases of FULL, a bit a slot
-        for (int x = 0; x < 2 * tiles.n; ++x) {        // keys of tile x / 2, or its values
+        int slot = 1, looked = 0;
+        uint32_t full = 1;                             // phases of FULL, a bit a slot
+        for (int x = 1; x < 2 * tiles.n; ++x) {        // keys of tile x / 2, or its values; the first are requested
           const int tile = tiles.tile(x >> 1);
           if (x >= SLOTS && !mbar_wait(bar(EMPTY + slot), (x / SLOTS - 1) & 1)) { failed = true; break; }
           const bool look = (x & 1) && (sees[0].part(tile) || sees[1].part(tile));
@@ -414,9 +451,11 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
           copy(x & 1 ? &maps.v : &maps.k, base + AT_RING + slot * TILE, hk, tile * BK, bar(which));
           if (look) ++looked;
           else full ^= 1u << slot;
-          if (x == 0 && tiles.has(1)) copy(&maps.q, base + AT_Q + TILE, h, row0 + BQ, bar(Q_FULL + 1));
           if (++slot == SLOTS) slot = 0;
         }
+        // queries that see none of a split's keys are waited for by nobody else
+        for (int i = 0; i < 2; ++i)
+          if (tiles.n > 0 && sees[i].last >= 0 && !mbar_wait(bar(Q_FULL + i), 0)) failed = true;
       }
       __syncwarp();
     } else {
@@ -429,23 +468,7 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
         if (!all_wait(bar(LOOK + which), (looked / LOOKED) & 1)) { failed = true; break; }
         ++looked;
         uint4* const v = reinterpret_cast<uint4*>(gbase + AT_RING + (2 * j + 1) % SLOTS * TILE);
-        __half2 most[2] = {u32_as_h2(0), u32_as_h2(0)};              // magnitudes; what is not finite is above all that is, or stays
-#pragma unroll 8
-        for (int c = at; c < (int)TILE / 16; c += 64) {
-          const uint4 x = v[c];
-          most[0] = __hmax2_nan(__hmax2_nan(most[0], __habs2(u32_as_h2(x.x))), __habs2(u32_as_h2(x.y)));
-          most[1] = __hmax2_nan(__hmax2_nan(most[1], __habs2(u32_as_h2(x.z))), __habs2(u32_as_h2(x.w)));
-        }
-        const __half2 top = __hmax2_nan(most[0], most[1]);
-        const bool found = not_finite(__low2half(top)) || not_finite(__high2half(top));
-        if (__any_sync(0xffffffffu, found)) {
-          __half* const x = reinterpret_cast<__half*>(v);
-          for (int c = at; c < (int)TILE / 16; c += 64)
-            for (int e = 0; e < 8; ++e)
-              if (not_finite(x[8 * c + e])) x[8 * c + e] = __ushort_as_half(0);
-          *s_taken_out = 1;
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
+        if (take_out(v, (int)TILE / 16, at)) *s_taken_out = 1;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(READY + which));
       }
@@ -457,7 +480,7 @@ attn_window_tc_kernel(const Args a, const __grid_constant__ Maps maps, int* err)
   if (tid == 0 && *s_failed) {
     q40_set_error(err);
     for (int i = 0; i < 2; ++i)
-      if (tiles.has(i)) mbar_wait(bar(Q_FULL + i), 0);
+      if (tiles.n > 0 && sees[i].last >= 0) mbar_wait(bar(Q_FULL + i), 0);
     for (int i = 0; i < SLOTS; ++i)
       if (const uint32_t r = s_requested[i]) mbar_wait(bar((int)(r - 1) >> 1), (r - 1) & 1);
   }
@@ -501,7 +524,7 @@ int splits_tc(const Args& a) {
   const int64_t blocks = (int64_t)a.H * ((a.S + 2 * BQ - 1) / (2 * BQ));
   Args one = a;
   one.splits = 1;
-  const int tiles = Tiles(one, (a.S - 1) / (2 * BQ) * 2 * BQ, 0).n;          // of the last block, which has most
+  const int tiles = Tiles(one, (a.S - 1) / (2 * BQ) * 2 * BQ, 2 * BQ, 0).n;          // of the last block, which has most
   // Least of what a CTA takes for its tiles and what sharing them costs: another launch, and the partial results' way out and back
   // (us; measured: 256 queries x 32 heads, 11 tiles 27.5 alone, 20 in four splits; 512 queries, four tiles 12.7 alone, 19 in two)
   const double tile = a.S > BQ ? 2.1 : 1.4, part = 0.35e-6 * a.S * a.H * (ATTN_D + 2) * sizeof(float);
@@ -514,20 +537,21 @@ int splits_tc(const Args& a) {
   return best;
 }
 
+// Copies of `box` rows of 64 dims out of rows of heads
+static bool make_map(CUtensorMap* m, const __half* x, int heads, int64_t rows, int64_t ld, int box) {
+  EncodeTiledFn encode = ttc_encode_fn();
+  if (!encode) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)heads * ATTN_D, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t boxes[2] = {64, (cuuint32_t)box}, one[2] = {1, 1};
+  return ttc_encode(encode, m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2u, (void*)x, dims, strides, boxes, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int launch_tc(const Args& a, int* err, cudaStream_t st) {
   using namespace tc;
-  EncodeTiledFn encode = ttc_encode_fn();
-  if (!encode) return Q40_E_UNSUPPORTED;
   Maps maps;
-  const auto map = [&](CUtensorMap* m, const __half* x, int heads, int64_t rows, int64_t ld) {
-    const cuuint64_t dims[2] = {(cuuint64_t)heads * ATTN_D, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
-    const cuuint32_t box[2] = {64, BK}, one[2] = {1, 1};
-    return ttc_encode(encode, m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2u, (void*)x, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  };
   const int64_t keys = (int64_t)a.offset + a.S;
-  if (map(&maps.q, a.q, a.H, a.S, a.ldq) != CUDA_SUCCESS || map(&maps.k, a.k, a.Hkv, keys, a.ldk) != CUDA_SUCCESS ||
-      map(&maps.v, a.v, a.Hkv, keys, a.ldv) != CUDA_SUCCESS)
+  if (!make_map(&maps.q, a.q, a.H, a.S, a.ldq, BQ) || !make_map(&maps.k, a.k, a.Hkv, keys, a.ldk, BK) || !make_map(&maps.v, a.v, a.Hkv, keys, a.ldv, BK))
     return Q40_E_UNSUPPORTED;
   static std::atomic<uint64_t> ready;
   cudaError_t e = q40_allow_smem(ready, (const void*)attn_window_tc_kernel, (int)SMEM);
