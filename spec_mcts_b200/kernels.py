@@ -606,14 +606,17 @@ def causal_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional
     if windowed:
         whole = offset + S
         # (the stride of a dimension of one may be anything)
+        if S == 0:
+            return out
         st = _stream(dev)
-        err = _tc_error_page(dev, st).data_ptr() + 4092
+        page = _tc_error_page(dev, st)
+        err = page.data_ptr() + 4092
         lds = [t.stride(0) if t.shape[0] > 1 else t.shape[1] * D for t in (q, k, v, out)]
-        w, sinks = whole if window is None else min(window, max(whole, 1)), min(sinks, whole)
-        nbytes = lib.q40_attn_causal_window_workspace_bytes(S, H, Hkv, D, offset, max(w, 1), sinks)
+        w, sinks = whole if window is None else min(window, whole), min(sinks, whole)
+        nbytes = lib.q40_attn_causal_window_workspace_bytes(S, H, Hkv, D, offset, w, sinks)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None           # of this call alone, as in _attn_pages
         check(lib.q40_attn_causal_window(q.data_ptr(), lds[0], k.data_ptr(), lds[1], v.data_ptr(), lds[2], out.data_ptr(), lds[3], S, H, Hkv, D,
-                                         offset, max(w, 1), sinks, _ptr(ws), nbytes, err, st), "q40_attn_causal_window")
+                                         offset, w, sinks, _ptr(ws), nbytes, err, st), "q40_attn_causal_window")
         return out
     check(lib.q40_attn_causal(q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
                               out.data_ptr(), out.stride(0), S, H, Hkv, D, _stream(dev)), "q40_attn_causal")
@@ -805,7 +808,7 @@ def _need_pools(what: str, k, v, k_scale, v_scale, page_size: int) -> int:
         raise Q40Error(f"{what}: pools of float16, int8 or float8_e4m3fn expected, got {k.dtype} and {v.dtype}")
     if k.dim() != 3 or k.shape != v.shape or not (k.is_contiguous() and v.is_contiguous()):
         raise Q40Error(f"{what}: contiguous pools [kv heads, slots, 128] of one shape expected, got {tuple(k.shape)} and {tuple(v.shape)}")
-    if page_size < 1:
+    if not 1 <= page_size <= 1 << 29:
         raise Q40Error(f"{what}: page_size {page_size}")
     if kind == 0:
         if k_scale is not None or v_scale is not None:
@@ -835,14 +838,16 @@ def _attn_pages(what, dev, p, q, k, v, k_scale, v_scale, L, page_size, seq_lens,
         raise Q40Error(f"{what}: window {window} below 1 or sinks {sinks} below 0")
     B, H, D = q.shape
     p, idx_bytes, tbl_stride = _page_table(what, p, B)
-    if L > p.shape[1] * page_size:
-        raise Q40Error(f"{what}: {L} keys do not fit a table of {p.shape[1]} pages of {page_size}")
+    if not 0 <= L <= min(p.shape[1] * page_size, 1 << 29):
+        raise Q40Error(f"{what}: {L} keys (at most 2^29) and a table of {p.shape[1]} pages of {page_size}")
     if seq_lens is not None:
         if seq_lens.shape != (B,):
             raise Q40Error(f"{what}: {B} lengths expected, got {tuple(seq_lens.shape)}")
         seq_lens = seq_lens.to(torch.int32).contiguous()
     q = _rows(q)
     o = torch.empty((B, H, D), device=dev, dtype=torch.float16)
+    if B == 0:
+        return o
     w, sinks = (0, 0) if window is None else (min(window, 1 << 30), min(sinks, 1 << 30))
     nbytes = lib.q40_attn_pages_workspace_bytes(B, H, k.shape[0], L, w, sinks)
     # of this call alone: calls on other streams and captured graphs that overlap it have their own
@@ -909,6 +914,10 @@ def page_append(p, k, v, kpool, vpool, pos, *, page_size: int = 1, offsets=None,
         q, q_out = _rows(q), torch.empty(q.shape, device=dev, dtype=torch.float16)
         if B == 0:
             q_out.zero_()
+    if T == 0 or B == 0:
+        return q_out
+    if q is not None and q.shape[1] == 0:
+        q = None
     if cos is not None:
         cos, sin = (t.clone() if t.data_ptr() % 16 else t for t in (cos.contiguous(), sin.contiguous()))
     check(lib.q40_page_append(p.data_ptr(), idx_bytes, tbl_stride, p.shape[1], pos.data_ptr(), _ptr(offsets), _ptr(q),

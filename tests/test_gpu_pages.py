@@ -486,6 +486,99 @@ def test_append_and_attention_in_a_graph_on_another_stream(K):
     assert all(torch.equal(y.view(torch.uint8), e.view(torch.uint8)) for y, e in zip((kp, vp, ks, vs), eager_cache))
 
 
+def test_nothing_to_do(K):
+    """No sequences, no tokens, tables without a page, queries of no position."""
+    g = generator(18)
+    (kp, ks), (vp, vs) = pool_of(g, "int8", 2, 4, 16), pool_of(g, "int8", 2, 4, 16)
+    none = lambda *s, dtype=torch.float16: torch.zeros(s, dtype=dtype, device="cuda")
+    i32 = torch.int32
+    assert K.page_flash_attn_q8(none(0, 2, dtype=i32), none(0, 4, D), kp, vp, ks, vs, page_size=16).shape == (0, 4, D)
+    got = K.page_flash_attn_q8(none(2, 0, dtype=i32), normal(g, 2, 4, D), kp, vp, ks, vs, page_size=16)
+    assert got.shape == (2, 4, D) and not got.any()
+    before = [x.clone() for x in (kp, vp, ks, vs)]
+    cos, sin = tables(8)
+    extra = dict(page_size=16, k_scale=ks, v_scale=vs, cos=cos, sin=sin)
+    assert K.page_append(none(0, 2, dtype=i32), none(0, 2, D), none(0, 2, D), kp, vp, none(0, dtype=i32), q=none(0, 4, D), **extra).shape == (0, 4, D)
+    assert K.page_append(none(2, 2, dtype=i32), none(0, 2, D), none(0, 2, D), kp, vp, none(2, dtype=i32), offsets=none(3, dtype=i32), **extra) is None
+    rows = normal(g, 3, 2, D)
+    assert not K.page_append(none(0, 2, dtype=i32), rows, rows, kp, vp, none(0, dtype=i32), offsets=none(1, dtype=i32), q=normal(g, 3, 4, D), **extra).any()
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip((kp, vp, ks, vs), before))
+    assert K.causal_attn(none(0, 4, D), normal(g, 7, 2, D), normal(g, 7, 2, D), window=3, offset=7).shape == (0, 4, D)
+
+
+def test_split_calls_in_graphs_that_overlap(K):
+    """Two captured graphs of calls with scratch, replayed at once on two streams, and eager calls on a third: each has scratch of its own."""
+    g = generator(19)
+    n = 6000
+    q, k, v = normal(g, 60, 8, D), normal(g, n, 2, D), normal(g, n, 2, D)
+    lens = torch.tensor([5000, 2000], dtype=torch.int32, device="cuda")
+    run, *_ = decode(K, "e4m3", g, 2, 8, 2, 16, 5000, lens, None, 0)
+    prompt = lambda: K.causal_attn(q, k, v, window=5000, sinks=4, offset=n - 60)
+    want = [prompt(), run()]
+    streams, graphs = [torch.cuda.Stream() for _ in range(3)], []
+    for st in streams[:2]:
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=st):
+                out = [prompt(), run()]
+            graphs.append((st, graph, out))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for st, graph, _ in graphs:
+            with torch.cuda.stream(st):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = [prompt(), run()]
+    torch.cuda.synchronize()
+    for outs in [o for *_, o in graphs] + [eager]:
+        assert all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
+def test_calls_of_two_threads(K):
+    import threading
+    g = generator(20)
+    lens = torch.tensor([3000, 1500, 700], dtype=torch.int32, device="cuda")
+    run, *_ = decode(K, "int8", g, 3, 8, 2, 16, 3000, lens, None, 0)
+    q, k, v = normal(g, 300, 4, D), normal(g, 2000, 2, D), normal(g, 2000, 2, D)
+    prompt = lambda: K.causal_attn(q, k, v, window=1500, sinks=4, offset=1700)
+    want, bad = [run(), prompt()], []
+
+    def work(call, right):
+        for _ in range(50):
+            if not torch.equal(call(), right):
+                bad.append(call)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip((run, prompt) * 2, want * 2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
+
+
+def test_without_the_extension(K, monkeypatch):
+    """The general way of each call gives what the native one does."""
+    g = generator(21)
+    lens = torch.tensor([300, 17], dtype=torch.int32, device="cuda")
+    calls = [decode(K, "int8", g, 2, 4, 2, 16, 300, lens, 100, 3)[0], decode(K, "f16", g, 2, 4, 2, 16, 300, lens, 100, 3)[0]]
+    q, k, v = normal(g, 100, 4, D), normal(g, 100, 2, D), normal(g, 100, 2, D)
+    calls.append(lambda: K.causal_attn(q, k, v, window=30))
+    cos, sin = tables(64)
+    p, pos = table_of(g, 2, 2, 4), torch.tensor([3, 16], dtype=torch.int32, device="cuda")
+    start = [pool_of(g, "e4m3", 2, 4, 16) for _ in range(2)]
+
+    def appended():
+        (kp, ks), (vp, vs) = [(c.clone(), s.clone()) for c, s in start]
+        versions = [x._version for x in (kp, ks, vp, vs)]
+        out = K.page_append(p, k[:2], v[:2], kp, vp, pos, page_size=16, k_scale=ks, v_scale=vs, q=q[:2], cos=cos, sin=sin)
+        assert all(x._version > n for x, n in zip((kp, ks, vp, vs), versions))      # the writes are counted
+        return torch.cat([x.reshape(-1).float() for x in (out, kp, ks, vp, vs)])
+
+    calls.append(appended)
+    native = [c() for c in calls]
+    monkeypatch.setattr(K, "_host_calls", None)
+    assert all(torch.equal(c(), n) for c, n in zip(calls, native))
+
+
 def test_refusals(K):
     g = generator(17)
     (kp, ks), (vp, vs) = pool_of(g, "int8", 2, 4, 16), pool_of(g, "int8", 2, 4, 16)
@@ -506,7 +599,8 @@ def test_refusals(K):
            lambda: K.page_append(p, k, v, kp, vp, pos, k_scale=ks, v_scale=vs, q=q, **ok), lambda: K.page_append(p, k, v, kp, vp, pos, k_scale=ks, v_scale=vs, offsets=pos, **ok),
            lambda: K.page_append(p, k, v, kp, vp, pos, k_scale=ks, v_scale=vs, cos=tables(4)[0], **ok), lambda: K.page_append(p, k, v, kp.half(), vp.half(), pos, k_scale=ks, v_scale=vs, **ok),
            lambda: K.page_append(p.cpu(), k, v, kp, vp, pos, k_scale=ks, v_scale=vs, **ok),
-           lambda: K.causal_attn(q, q, q, window=0), lambda: K.causal_attn(q, q, q, window=3, sinks=-1), lambda: K.causal_attn(q, q, q, offset=1), lambda: K.causal_attn(q, q, q, offset=-1),
+           lambda: K.causal_attn(q, q, q, window=0), lambda: K.page_flash_attn_q8(p.expand(2, 2).repeat(1, 1 << 17), q, kp, vp, ks, vs, page_size=1 << 30),
+           lambda: K.causal_attn(q, q, q, window=3, sinks=-1), lambda: K.causal_attn(q, q, q, offset=1), lambda: K.causal_attn(q, q, q, offset=-1),
            lambda: K.causal_attn(q, q, q[:, :2], window=3), lambda: K.causal_attn(q, q[:, :3], q[:, :3], window=3), lambda: K.causal_attn(q, q, q, q[:1], window=3)]
     for call in bad:
         with pytest.raises(K.Q40Error):
