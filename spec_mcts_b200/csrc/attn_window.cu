@@ -67,14 +67,15 @@ attn_window_kernel(const Args a) {
     const auto all_see = [&](int lo, int hi) { return key0 + TILE_KEYS <= lo + 1 && (key0 > hi - a.window || key0 + TILE_KEYS <= a.sinks); };
     if (!all_see(p_first, p_last)) {
       uint4* const row = reinterpret_cast<uint4*>(smem + RB * TILE_ROW_BYTES + stage * 2 * TILE_BYTES + TILE_BYTES);
-      bool found = false;
+      __half2 most = u32_as_h2(0);             // magnitudes: what is not finite is above all that is, or stays
 #pragma unroll
       for (int j = 0; j < TILE_BYTES / 16 / NT; ++j) {
         const uint4 x = row[tid + j * NT];
         const uint32_t e[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) found |= (e[c] & 0x7c00u) == 0x7c00u || (e[c] & 0x7c000000u) == 0x7c000000u;
+        for (int c = 0; c < 4; ++c) most = __hmax2_nan(most, __habs2(u32_as_h2(e[c])));
       }
+      const bool found = not_finite(__low2half(most)) || not_finite(__high2half(most));
       if (__syncthreads_or(found)) {
         taken_out = true;
         __half* const x = reinterpret_cast<__half*>(row);
