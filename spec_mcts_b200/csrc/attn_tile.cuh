@@ -89,8 +89,9 @@ struct WarpRows {
 
   // KEYS keys of a tile: S = Q K^T, online softmax, O += P V.  With MASK, key i of the tile counts for row g below n0 and for row g + 8
   // below n1.  With WINDOW, moreover, it counts from key from0 or from1 on, or below `first`.  A row all of whose scores so far are -inf
-  // keeps its sum and outputs at zero.
-  template <bool MASK, int KEYS = TILE_KEYS, bool WINDOW = false>
+  // keeps its sum and outputs at zero.  Weights, which are rounded to fp16 for the product, sums and outputs come times 2^BITS: up to 2^14, that
+  // many more of the small ones are kept.
+  template <bool MASK, int KEYS = TILE_KEYS, bool WINDOW = false, int BITS = 0>
   __device__ __forceinline__ void step(uint32_t kt, uint32_t vt, float scale_log2, int n0, int n1, int lane, int from0 = 0, int from1 = 0,
                                        int first = 0) {
     const int t = lane & 3;
@@ -138,7 +139,7 @@ struct WarpRows {
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float p = ex2(s[nt][j] - m[j >> 1]);
+        const float p = ex2(s[nt][j] - (m[j >> 1] - BITS));
         s[nt][j] = p;
         ls[j >> 1] += p;
       }

@@ -14,6 +14,7 @@ namespace q40 {
 namespace window {
 
 constexpr int NWARPS = 4, RB = NWARPS * 16, NT = NWARPS * 32;
+constexpr int BITS = 14;                     // log2 of a row's largest weight
 
 __global__ void __launch_bounds__(NT)
 attn_window_kernel(const Args a) {
@@ -84,9 +85,9 @@ attn_window_kernel(const Args a) {
         __syncthreads();
       }
     }
-    if (all_see(min(warp_first, p_last), min(warp_last, p_last))) w.step<false>(kt, vt, a.scale_log2, 0, 0, lane);
+    if (all_see(min(warp_first, p_last), min(warp_last, p_last))) w.step<false, TILE_KEYS, false, BITS>(kt, vt, a.scale_log2, 0, 0, lane);
     else if (key0 <= warp_last && (key0 + TILE_KEYS > warp_first - a.window + 1 || key0 < a.sinks))
-      w.step<true, TILE_KEYS, true>(kt, vt, a.scale_log2, min(p0, p_last) + 1 - key0, min(p1, p_last) + 1 - key0, lane, p0 - a.window + 1 - key0,
+      w.step<true, TILE_KEYS, true, BITS>(kt, vt, a.scale_log2, min(p0, p_last) + 1 - key0, min(p1, p_last) + 1 - key0, lane, p0 - a.window + 1 - key0,
                                     p1 - a.window + 1 - key0, a.sinks - key0);
     __syncthreads();
   }

@@ -8,8 +8,11 @@
 //   warps 10, 11         look through the values that some query of a tile sees in part: see below
 // Tensor memory: S (and P) of the two tiles at columns 0 and 128, O at 256 and 384.
 //
-// A row's maximum stays while no score passes it by 8 (a weight is then at most 2^8, which fp16 holds), so that O is seldom rescaled; who
-// rescales finds no MMA of its O on the way, since S of a step is finished after O += P V of the step before.
+// m is 7 below a row's largest score, and stays until one passes it by 15, so that O is seldom rescaled; who rescales finds no MMA of its O on the
+// way, since S of a step is finished after O += P V of the step before.
+// A weight is rounded to fp16: off by 2^-11 of itself at most from 2^-21 of a row's largest on, and by 2^-32 of that below it.  (The sum has them in fp32: with m at the largest
+// score itself, 8192 keys at 2^-26 of it were lost to O, but not to the sum.)  Two parts a weight, as for one query over pages, would be another eight of a step's sixteen MMAs
+// and 2.5e-4 to 2.9e-4 of the result's norm off 64 bits would be 2.0e-4, which is the rounding of the result.
 //
 // A masked key has a weight of 0, and 0 times a value that is not finite is no number: in tiles with masked places such values are taken out of
 // shared memory before the MMA, and added at the end to the rows that see them (as in attn_window_kernel).
@@ -41,7 +44,8 @@ using ttc::mbar_wait;
 constexpr int BQ = 128, BK = 128, THREADS = 384;            // queries of a CTA's tile, keys of a tile
 constexpr uint32_t TILE = BK * ATTN_D * 2;               // 32 KB: two blocks of 64 dims, rows of 128 bytes
 constexpr uint32_t HALF = TILE / 2;
-constexpr float STAY = 8.f;
+// log2 of a row's largest weight: where the maximum is set, and most.  fp16 holds 2^15
+constexpr float WEIGHT_SET = 7.f, WEIGHT_TOP = 15.f;
 
 struct Maps { CUtensorMap q, k, v; };
 
@@ -184,9 +188,9 @@ struct Row {
 #pragma unroll
     for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[BK - 4 + e]);
     const float most = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * a.scale_log2;
-    const bool passes = most > m + STAY;
+    const bool passes = most > m + WEIGHT_TOP;
     if (__any_sync(0xffffffffu, passes)) {
-      const float now = passes ? most : m, corr = fmaxf(ex2(m - now), 1.17549435e-38f);      // (never 0: infinities stay)
+      const float now = passes ? most - WEIGHT_SET : m, corr = fmaxf(ex2(m - now), 1.17549435e-38f);      // (never 0: infinities stay)
       m = now;
       l *= corr;
       if (n > 0) {

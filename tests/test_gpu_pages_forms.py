@@ -1,0 +1,38 @@
+"""Calls of the paged cache and of windows that the other tests do not make, each against its definition in 64 bits."""
+import pytest
+import torch
+
+from test_gpu_pages import WEIGHT, D, K, generator, normal, prompt_reference  # noqa: F401  (K: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def general(q, k, v, window, sinks=0, offset=0, err=None, out=None):
+    """The C call: without `err`, and without a workspace."""
+    from spec_mcts_b200._lib import check, lib
+    s, h, _ = q.shape
+    o = torch.empty_like(q) if out is None else out
+    check(lib.q40_attn_causal_window(q.data_ptr(), h * D, k.data_ptr(), k.shape[1] * D, v.data_ptr(), v.shape[1] * D, o.data_ptr(), o.stride(0), s, h, k.shape[1], D, offset, window,
+                                     sinks, None, 0, None if err is None else err.data_ptr(), torch.cuda.current_stream().cuda_stream), "q40_attn_causal_window")
+    return o
+
+
+def check_weights(got, want, size, v):
+    """Weights are off by 2^-11 of each, or, where that is more, by half a step of the smallest fp16 (2^-25) when a row's largest is at least 2^7; the rest
+    as in a decode step, whose scores, powers and sums are off by `WEIGHT`."""
+    bound = 2 ** -11 * want.abs() + (WEIGHT + 2 ** -11) * size + v.shape[0] * 2 ** -32 * v.float().nan_to_num(0, 0, 0).abs().max() + 2 ** -25
+    assert ((got.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("way", ["tensor cores", "general"])
+@pytest.mark.parametrize("s,h,hkv,window,sinks,offset", [(300, 2, 1, 10000, 0, 8000), (1, 4, 2, 9000, 0, 8000), (300, 2, 2, 5000, 4, 8000), (17, 2, 2, 1000, 0, 100)])
+def test_prompt_of_one_key_above_many(K, way, s, h, hkv, window, sinks, offset):
+    """Weights 2^-26 of the first key's, whose value is 0: the result is what they sum up to."""
+    g = generator(s + h)
+    q, k, v = normal(g, s, h, D), torch.zeros(offset + s, hkv, D, dtype=torch.float16, device="cuda"), 1 + normal(g, offset + s, hkv, D) / 8
+    q[..., 0] = 8.0
+    k[0, :, 0] = 26 / (8 * 0.12751741)                # (1 / sqrt(128) log2 e)
+    v[0] = 0
+    run = K.causal_attn if way == "tensor cores" else lambda *a, **kw: general(*a, **kw)
+    got = run(q, k, v, window=window, sinks=sinks, offset=offset)
+    check_weights(got, *prompt_reference(q, k, v, window, sinks, offset), v)
