@@ -6,7 +6,8 @@
 //
 // A masked key has a weight of 0, and 0 times a value that is not finite is no number.  In a tile that some query sees in part, values
 // that are not finite are therefore taken out in shared memory, and added at the end to the queries that see their key: an infinity or NaN comes
-// out of a sum whatever its weight is.
+// out of a sum whatever its weight is.  In the other tiles they stay; a weight that fp16 has as 0, or a maximum that moves far, makes no number of an infinity
+// there as well, and a row that ends with one takes the sum of the values that it sees and that are not finite.
 #include "attn_tile.cuh"
 #include "attn_window.cuh"
 
@@ -93,24 +94,38 @@ attn_window_kernel(const Args a) {
   }
   cp_async_wait<0>();
   w.finish();
-  if (taken_out)                             // rare, and slow
+  bool lost[2] = {false, false};             // no number, and not by a score
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+#pragma unroll
+    for (int dt = 0; dt < 16; ++dt) lost[r] |= w.o[dt][2 * r] != w.o[dt][2 * r] || w.o[dt][2 * r + 1] != w.o[dt][2 * r + 1];
+    lost[r] &= w.l[r] == w.l[r];
+  }
+  if (taken_out || lost[0] || lost[1]) {     // rare, and slow
+    uint32_t found[2] = {0, 0};
     for (int i = 0; i < ntiles; ++i) {
       const int key0 = tile_of(i) * TILE_KEYS;
-      if (key0 + TILE_KEYS <= p_first + 1 && (key0 > p_last - a.window || key0 + TILE_KEYS <= a.sinks)) continue;
+      const bool all = key0 + TILE_KEYS <= p_first + 1 && (key0 > p_last - a.window || key0 + TILE_KEYS <= a.sinks);
+      if (all && !lost[0] && !lost[1]) continue;
       for (int j = key0; j < min(key0 + TILE_KEYS, k_end); ++j) {
         const __half* const x = a.v + (int64_t)j * a.ldv + hk * D + 2 * t;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const int p = r ? p1 : p0;
-          if (p > p_last || j > p || (p - j >= a.window && j >= a.sinks)) continue;
+          if (p > p_last || j > p || (p - j >= a.window && j >= a.sinks) || (all && !lost[r])) continue;
 #pragma unroll
           for (int dt = 0; dt < 16; ++dt)
 #pragma unroll
             for (int c = 0; c < 2; ++c)
-              if (not_finite(x[dt * 8 + c])) w.o[dt][2 * r + c] += __half2float(x[dt * 8 + c]);
+              if (not_finite(x[dt * 8 + c])) {
+                const uint32_t bit = 1u << (2 * dt + c);
+                w.o[dt][2 * r + c] = (lost[r] && !(found[r] & bit) ? 0.f : w.o[dt][2 * r + c]) + __half2float(x[dt * 8 + c]);
+                found[r] |= bit;
+              }
         }
       }
     }
+  }
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int p = r ? p1 : p0;

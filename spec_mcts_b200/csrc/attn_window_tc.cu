@@ -15,7 +15,8 @@
 // and 2.5e-4 to 2.9e-4 of the result's norm off 64 bits would be 2.0e-4, which is the rounding of the result.
 //
 // A masked key has a weight of 0, and 0 times a value that is not finite is no number: in tiles with masked places such values are taken out of
-// shared memory before the MMA, and added at the end to the rows that see them (as in attn_window_kernel).
+// shared memory before the MMA, and added at the end to the rows that see them (as in attn_window_kernel).  In tiles that all see they stay; a weight
+// that fp16 has as 0 makes no number of them there as well, and a row that ends with one takes the sum of what it sees that is not finite.
 //
 // Every wait is bounded: on expiry the error word is set, what is left is skipped, the CTA's own copies and MMAs are waited for (bounded too),
 // and tensor memory is freed.
@@ -247,18 +248,33 @@ struct Row {
       if (n == 0)                                  // none of the split's keys: nothing has been written there
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = 0.f;
-      if (taken_out && there)                      // rare, and slow
+      uint64_t all[16];                            // (a sum is no number where one of them is none, and where they are infinite both ways, which does no harm)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) all[e] = pack2(o[2 * e], o[2 * e + 1]);
+#pragma unroll
+      for (int e = 8; e > 0; e >>= 1)
+#pragma unroll
+        for (int d = 0; d < e; ++d) all[d] = add2(all[d], all[d + e]);
+      float x, y;
+      unpack2(all[0], x, y);
+      const bool lost = x + y != x + y && l == l;  // no number, and not by a score: see above
+      if ((taken_out || lost) && there) {          // rare, and slow
+        uint32_t found = 0;
         for (int j = 0; j < tiles.n; ++j) {
           const int tile = tiles.tile(j), key0 = tile * BK;
-          if (!sees[0].part(tile) && !sees[1].part(tile)) continue;
+          if (!lost && !sees[0].part(tile) && !sees[1].part(tile)) continue;
           for (int k = key0; k < min(key0 + BK, p + 1); ++k) {
             if (p - k >= a.window && k >= a.sinks) continue;
             const __half* const v = a.v + (int64_t)k * a.ldv + hk * ATTN_D + 32 * c;
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (not_finite(v[e])) o[e] += __half2float(v[e]);
+              if (not_finite(v[e])) {
+                o[e] = (lost && !(found & (1u << e)) ? 0.f : o[e]) + __half2float(v[e]);
+                found |= 1u << e;
+              }
           }
         }
+      }
       if (there && a.splits > 1) {
         float4* const part = reinterpret_cast<float4*>(a.po + part_at * ATTN_D + 32 * c);
 #pragma unroll

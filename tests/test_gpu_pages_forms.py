@@ -36,3 +36,30 @@ def test_prompt_of_one_key_above_many(K, way, s, h, hkv, window, sinks, offset):
     run = K.causal_attn if way == "tensor cores" else lambda *a, **kw: general(*a, **kw)
     got = run(q, k, v, window=window, sinks=sinks, offset=offset)
     check_weights(got, *prompt_reference(q, k, v, window, sinks, offset), v)
+
+
+@pytest.mark.parametrize("way", ["tensor cores", "general"])
+@pytest.mark.parametrize("s,h,hkv,offset,far", [(700, 4, 2, 0, 300), (700, 4, 2, 0, 3), (60, 2, 1, 64, 70), (100, 8, 2, 2000, 1900), (300, 4, 4, 400, 500), (1, 2, 1, 3000, 2000)])
+def test_prompt_infinite_values_of_keys_far_below(K, way, s, h, hkv, offset, far):
+    """An infinite value comes out to every query that sees its key, whatever its weight is and whether or not all of a tile's queries see it."""
+    g = generator(s + far)
+    n = offset + s
+    q, k, v = normal(g, s, h, D), normal(g, n, hkv, D), normal(g, n, hkv, D)
+    q[..., 0] = 8.0
+    k[5:7, :, 0], k[far, :, 0] = -400.0, 40.0         # scores far below the others, and one far above them
+    late = n - 30 if s > 30 else n - 1                # in a tile that some queries see in part
+    k[late, :, 0] = -400.0
+    v[5, 0, 3], v[5, 0, 70], v[5:7, 0, 9], v[6, 0, 9], v[5, 0, 11], v[late, 0, 11], v[5, 0, 127] = torch.inf, -torch.inf, torch.inf, -torch.inf, torch.inf, -torch.inf, torch.nan
+    run = K.causal_attn if way == "tensor cores" else lambda *a, **kw: general(*a, **kw)
+    got = run(q, k, v, window=n, offset=offset)
+    at = torch.arange(offset, n, device="cuda")[:, None]
+    five, six, end = at >= 5, at >= 6, at >= late
+    rep = got[:, :h // hkv]
+    assert ((rep[..., 3] == torch.inf) == five).all() and ((rep[..., 70] == -torch.inf) == five).all() and (rep[..., 127].isnan() == five).all()
+    assert ((rep[..., 9] == torch.inf) == (five & ~six)).all() and (rep[..., 9].isnan() == six).all()
+    assert ((rep[..., 11] == torch.inf) == (five & ~end)).all() and (rep[..., 11].isnan() == end).all()
+    clean = [x for x in range(D) if x not in (3, 9, 11, 70, 127)]
+    assert rep[..., clean].isfinite().all() and got[:, h // hkv:].isfinite().all()
+    fine = lambda x: torch.cat((x[:, :h // hkv, clean].flatten(1), x[:, h // hkv:].flatten(1)), 1)
+    want, size = prompt_reference(q, k, v.nan_to_num(0, 0, 0), n, 0, offset)
+    check_weights(fine(got), fine(want), fine(size), v)
