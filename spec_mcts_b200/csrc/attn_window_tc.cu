@@ -208,7 +208,7 @@ struct Row {
       }
     }
     const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), m2 = pack2(-m, -m);
-    uint64_t sum[2] = {pack2(l, 0.f), 0};
+    uint64_t sum[2] = {0, 0};                      // of this step: weight by weight onto l, the low bits of each would be lost to a long sum
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       uint32_t pk[32];
@@ -229,7 +229,7 @@ struct Row {
     }
     float x, y;
     unpack2(add2(sum[0], sum[1]), x, y);
-    l = x + y;
+    l += x + y;
     ++n;
   }
   // ... and its output, or a split's partial result.  taken_out: values that are not finite were taken out of tiles that `sees` say are seen in part

@@ -1,4 +1,6 @@
 """Calls of the paged cache and of windows that the other tests do not make, each against its definition in 64 bits."""
+import math
+
 import pytest
 import torch
 
@@ -63,3 +65,17 @@ def test_prompt_infinite_values_of_keys_far_below(K, way, s, h, hkv, offset, far
     fine = lambda x: torch.cat((x[:, :h // hkv, clean].flatten(1), x[:, h // hkv:].flatten(1)), 1)
     want, size = prompt_reference(q, k, v.nan_to_num(0, 0, 0), n, 0, offset)
     check_weights(fine(got), fine(want), fine(size), v)
+
+
+def test_prompt_sum_of_many_weights(K):
+    """The first key's value over the sum of 2^20 weights, each of which is 1.03 of a power of two: added one by one to a sum of 2^19 and more of that power, a weight would lose
+    its 0.03.  Eighty heads, so that CTAs do not share the keys."""
+    n, h = 1 << 20, 80
+    q, k, v = (torch.zeros(s, dtype=torch.float16, device="cuda") for s in ((1, h, D), (n, 1, D), (n, 1, D)))
+    q[..., 0], k[0, 0, 0], v[0] = 8.0, 9.9574 / (8 * 0.12751741), 1000.0
+    got = K.causal_attn(q, k, v, window=n, offset=n - 1)
+    assert K.tc_error_flag() == 0
+    first = math.exp(8 * k[0, 0, 0].item() / math.sqrt(D))
+    want = 1000 * first / (first + n - 1)
+    # a weight's score, power and rounding (the first's value is exact); a step adds 128 weights to the sum, half a unit in the last place off: 2^-24 x 2^20 / 128
+    assert (got.double() - want).abs().max() <= want * (2 ** -11 + WEIGHT + 2 ** -11 + 2 ** -11)
