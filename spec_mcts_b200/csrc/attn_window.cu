@@ -155,7 +155,7 @@ static Args args_of(int S, int H, int Hkv, int offset, int window, int sinks) {
 }
 // Whether the kernel on tcgen05 takes the call.  Us here / there, 32 heads: 64 queries of themselves 4.5 / 5.3, 100 6.5 / 5.5, 256 11.2 / 8.7; a query behind 300 keys of which it sees
 // 68 8.0 / 8.7, 64 such queries 11.0 / 8.7; a query behind 4000 with a window of 1024 30.9 / 10.7
-static bool wide(const Args& a) { return a.S > 64 || min(a.offset, a.window - 1) + a.S + a.sinks > 128; }
+static bool wide(const Args& a) { return a.S > 64 || (int64_t)min(a.offset, a.window - 1) + a.S + a.sinks > 128; }
 static bool fits(int S, int H, int Hkv, int D, int offset, int window, int sinks) {
   return S >= 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && offset >= 0 && window > 0 && sinks >= 0 && (int64_t)S + offset <= (1 << 30) && D == ATTN_D;
 }
