@@ -34,6 +34,7 @@ constexpr int FEW = 148;                   // units
 // 122 / 122 / 122 / 133 / 144.  A second chunk costs a launch, 2 to 3 us: 256 keys of 1 x 500 8.0, 512 6.7
 constexpr int CHUNK_MIN = 512, CHUNK_MAX = 8192;
 constexpr int CHUNK_WAVE = 2048;
+constexpr int64_t MOST_CHUNKS = 65535;     // of a unit, as the grid has it: behind 8192 x 65535 keys chunks are of 16384
 constexpr int64_t WAVE = 296, CTAS = 1200; // CTAs that a call is cut into, about: one wave of them, where that leaves chunks of up to CHUNK_WAVE
 
 struct Args {
@@ -96,7 +97,7 @@ __host__ __device__ __forceinline__ int chunk_of(int64_t n, int64_t units) {
   while (chunk < CHUNK_WAVE && chunk * wave < n) chunk *= 2;
   if (wave > 1 && chunk * wave >= n) return chunk;
   chunk = CHUNK_MIN;
-  while (chunk < CHUNK_MAX && chunk * all < n) chunk *= 2;
+  while ((chunk < CHUNK_MAX && chunk * all < n) || chunk * MOST_CHUNKS < n) chunk *= 2;
   return chunk;
 }
 
@@ -462,6 +463,7 @@ static Plan plan_of(int B, int H, int Hkv, int L, int window, int sinks) {
     if (keys > 0) n = std::max(n, (keys + chunk_of(keys, p.units) - 1) / chunk_of(keys, p.units));
   };
   at(most);
+  at(CHUNK_MAX * MOST_CHUNKS);
   for (int64_t chunk = CHUNK_MIN; chunk <= CHUNK_MAX; chunk *= 2) {
     at(chunk * (WAVE / p.units));
     at(chunk * std::max<int64_t>(1, CTAS / p.units));
@@ -518,7 +520,7 @@ extern "C" int q40_attn_pages(const void* page_tbl, int idx_bytes, int64_t tbl_s
     return Q40_E_ALIGN;
   const Plan p = plan_of(B, H, Hkv, Lmax, window, sinks);
   const int64_t parts = p.units * p.nchunks * p.heads;
-  if (parts > 0x7fffffffLL || p.nchunks > 65535) return Q40_E_SHAPE;
+  if (parts > 0x7fffffffLL || p.nchunks > MOST_CHUNKS) return Q40_E_SHAPE;
   if (p.nchunks > 1) {
     if (!workspace || workspace_bytes < (size_t)parts * (ATTN_D + 2) * sizeof(float)) return Q40_E_WORKSPACE;
     if (!q40_aligned(workspace, 16)) return Q40_E_ALIGN;

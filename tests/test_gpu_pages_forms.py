@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_pages import WEIGHT, D, K, generator, normal, prompt_reference  # noqa: F401  (K: the fixture)
+from test_gpu_pages import WEIGHT, D, K, check_decode, generator, normal, prompt_reference  # noqa: F401  (K: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +79,25 @@ def test_prompt_sum_of_many_weights(K):
     want = 1000 * first / (first + n - 1)
     # a weight's score, power and rounding (the first's value is exact); a step adds 128 weights to the sum, half a unit in the last place off: 2^-24 x 2^20 / 128
     assert (got.double() - want).abs().max() <= want * (2 ** -11 + WEIGHT + 2 ** -11 + 2 ** -11)
+
+
+def test_decode_of_2_to_29_keys(K):
+    """A table that lists one page over and over, and another one at the end of each sequence, with a key above all others: the last chunk of each unit."""
+    g = generator(29)
+    lens = [1 << 29, 65535 * 8192 + 1, 65535 * 8192]
+    p = torch.zeros(3, 1 << 25, dtype=torch.int32, device="cuda")
+    for i, n in enumerate(lens):
+        p[i, (n - 1) // 16] = 1
+    codes = torch.randint(-127, 128, (1, 32, D), generator=g, device="cuda").to(torch.int8)
+    k, v, scale = codes.clone(), codes.clone(), torch.full((1, 2), 2.0 ** -7, device="cuda")
+    k[..., 0] = -127
+    k[0, [16 + (n - 1) % 16 for n in lens], 0] = 127          # 2^129 times the weight of the others, of which there are 2^29
+    q = torch.zeros(3, 1, D, dtype=torch.float16, device="cuda")
+    q[..., 0] = 512.0
+    q[..., 1:] = normal(g, 3, 1, D - 1) / 64
+    got = K.page_flash_attn_q8(p, q, k, v, scale, scale, page_size=16, seq_lens=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    for i, n in enumerate(lens):
+        seen = torch.arange(16, 16 + (n - 1) % 16 + 1, device="cuda")           # of the last page; the others do not count
+        s = (k[0, seen].double() @ q[i, 0].double()) * 2.0 ** -7 / math.sqrt(D)
+        want = torch.softmax(s, 0) @ (v[0, seen].double() * 2.0 ** -7)
+        check_decode(got[i, 0], want, (v[0].double() * 2.0 ** -7).abs().amax().expand(D))
