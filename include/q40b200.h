@@ -326,7 +326,7 @@ int q40_attn_pages(const void* page_tbl, int idx_bytes, int64_t tbl_stride, cons
  * 8-bit pools: a page's scale is max(scale so far, largest magnitude of its new rows / 127 or 448), where a page whose first slot is written has
  * none so far; if it grows, the page's rows in front of the new ones are coded anew.  A value that is not finite makes the scale NaN until
  * the page is begun anew.  Tokens of one call that go to one slot, in 8 bits also sequences that append to one page, leave those slots (that
- * page and its scale) undefined.  16-byte aligned, strides multiples of 8.  No counterpart in the reference beyond the append of
+ * page and its scale) undefined.  Pages of up to 2^26 tokens in 8 bits.  16-byte aligned, strides multiples of 8.  No counterpart in the reference beyond the append of
  * hf_model_q40_kv_shared.py:365-371 to its own cache. */
 int q40_page_append(const void* page_tbl, int idx_bytes, int64_t tbl_stride, int tbl_width, const int32_t* pos, const int32_t* offsets,
                     const void* q, int64_t q_stride, void* q_out, const void* k, int64_t k_stride, const void* v, int64_t v_stride,

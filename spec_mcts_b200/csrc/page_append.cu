@@ -37,6 +37,7 @@ struct Args {
 constexpr int THREADS = 128;
 constexpr int EACH = 4;                   // heads of a lane group in large calls
 constexpr int64_t MANY = 32768;           // ... of more rows than these: fewer would not fill the SMs with a quarter of the lane groups
+constexpr int MOST_ROWS = 1 << 26;        // of a page in 8 bits: its earlier rows are counted through in pieces of 8 bytes, 16 a row, in 32 bits
 constexpr int UNITS = THREADS / 8;        // rows of 128 values of a block's pass, eight lanes each
 
 // The last i of [0, n) whose first(i) is not above x (0 where there is none)
@@ -342,7 +343,7 @@ extern "C" int q40_page_append(const void* page_tbl, int idx_bytes, int64_t tbl_
   if (B < 0 || T < 0 || (q && H <= 0) || Hkv <= 0 || page_size <= 0 || P <= 0 || tbl_width <= 0 || tbl_stride < tbl_width) return Q40_E_SHAPE;
   if (!offsets && T != B) return Q40_E_SHAPE;
   if (cos_tbl && n_pos <= 0) return Q40_E_SHAPE;
-  if (cache_type != CACHE_F16 && P % page_size != 0) return Q40_E_SHAPE;
+  if (cache_type != CACHE_F16 && (P % page_size != 0 || page_size > MOST_ROWS)) return Q40_E_SHAPE;
   const int64_t pages = (P + page_size - 1) / page_size;
   if (pages > 0x7fffffffLL) return Q40_E_SHAPE;
   if (k_stride < (int64_t)Hkv * D || v_stride < (int64_t)Hkv * D || (q && q_stride < (int64_t)H * D)) return Q40_E_SHAPE;

@@ -1,7 +1,7 @@
 """The paged cache's and window attention's entry points at the largest sizes that they take, before anything is enqueued."""
 
 from spec_mcts_b200._lib import lib
-from test_pages_cpu import SHAPE, WORKSPACE, attn
+from test_pages_cpu import SHAPE, WORKSPACE, append, attn
 
 
 def test_window_workspace_of_2_to_30_positions():
@@ -17,3 +17,12 @@ def test_attention_of_2_to_29_keys():
     for keys in (65535 * 8192, 65535 * 8192 + 1, (1 << 29) - 1, 1 << 29):
         assert attn(L=keys, tstride=1 << 25) == WORKSPACE and need(keys) == 65535 * row
     assert need(1 << 28) == 32768 * row and attn(L=(1 << 29) + 1, tstride=1 << 26) == SHAPE
+
+
+def test_append_refuses_8_bit_pages_above_2_to_26():
+    """One CTA codes a page's earlier rows anew, 2^27 of them in 2^31 pieces."""
+    for kind in (1, 2):
+        assert append(ps=1 << 27, P=1 << 27, kind=kind, B=0, T=0) == SHAPE
+        assert append(ps=(1 << 26) + 1, P=(1 << 26) + 1, kind=kind, B=0, T=0) == SHAPE
+        assert append(ps=1 << 26, P=1 << 26, kind=kind, B=0, T=0) == 0
+    assert append(ps=1 << 29, P=1 << 29, kind=0, B=0, T=0) == 0
