@@ -164,7 +164,7 @@ PageAppend page_append_fn = nullptr;
 CausalWindow causal_window_fn = nullptr;
 CausalWindowBytes causal_window_bytes = nullptr;
 
-constexpr int64_t HEAD = 128, MOST = 1 << 30;
+constexpr int64_t HEAD = 128, MOST = 1 << 30, MOST_PAGE = 1 << 29;
 
 // A whole number of up to MOST; None is `none`
 bool whole(PyObject* o, int64_t none, int64_t& x) {
@@ -235,7 +235,7 @@ PyObject* attn_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int64_t L, ps, window, sinks, ld;
   Table tbl;
   if (!fine || !whole(args[6], -1, L) || !whole(args[7], -1, ps) || !whole(args[9], 0, window) || !whole(args[10], -1, sinks) || L < 0 || ps < 1 ||
-      sinks < 0 || window < (args[9] == Py_None ? 0 : 1))
+      ps > MOST_PAGE || sinks < 0 || window < (args[9] == Py_None ? 0 : 1))
     Py_RETURN_NONE;
   const int dev = c10::cuda::current_device();
   if (!rows_of(q, dev, ld)) Py_RETURN_NONE;
@@ -272,7 +272,7 @@ PyObject* page_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
                    *q = tensor_or_none(args[10], fine), *cos = tensor_or_none(args[11], fine), *sin = tensor_or_none(args[12], fine);
   int64_t ps, ldk, ldv, ldq = 0;
   Table tbl;
-  if (!fine || !whole(args[6], -1, ps) || ps < 1) Py_RETURN_NONE;
+  if (!fine || !whole(args[6], -1, ps) || ps < 1 || ps > MOST_PAGE) Py_RETURN_NONE;
   const int dev = c10::cuda::current_device();
   const int kind = pools_of(kp, vp, ks, vs, dev, ps);
   if (kind < 0 || !rows_of(k, dev, ldk) || !rows_of(v, dev, ldv) || k->sizes() != v->sizes() || k->size(1) != kp->size(0) || !is(pos, dev, at::kInt) ||

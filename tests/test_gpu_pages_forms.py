@@ -101,3 +101,17 @@ def test_decode_of_2_to_29_keys(K):
         s = (k[0, seen].double() @ q[i, 0].double()) * 2.0 ** -7 / math.sqrt(D)
         want = torch.softmax(s, 0) @ (v[0, seen].double() * 2.0 ** -7)
         check_decode(got[i, 0], want, (v[0].double() * 2.0 ** -7).abs().amax().expand(D))
+
+
+def test_page_sizes_that_no_call_takes(K):
+    """Above 2^29: the native call refuses what the general way does."""
+    g = generator(4)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    p, pos, rows, q = torch.zeros(1, 1, **i32), torch.zeros(1, **i32), normal(g, 1, 2, D), normal(g, 1, 4, D)
+    pool = torch.zeros(2, 64, D, dtype=torch.float16, device="cuda")
+    for size in ((1 << 29) + 1, 1 << 30, 1 << 40):
+        with pytest.raises(K.Q40Error):
+            K.page_append(p, rows, rows, pool, pool.clone(), pos, page_size=size)
+        with pytest.raises(K.Q40Error):
+            K.page_flash_attn(p, q, pool, pool, 64, 1, 10, 4, D, page_size=size, window=4)
+    assert not pool.any()
