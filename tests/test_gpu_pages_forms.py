@@ -115,3 +115,21 @@ def test_page_sizes_that_no_call_takes(K):
         with pytest.raises(K.Q40Error):
             K.page_flash_attn(p, q, pool, pool, 64, 1, 10, 4, D, page_size=size, window=4)
     assert not pool.any()
+
+
+def test_prompt_behind_100_million_keys(K):
+    """A CTA goes through its tiles for over a second: whoever waits for the last of them, or for all, does not give up after the 0.6 s of another wait.  One tensor of 26 GB is keys
+    and values."""
+    n, s, h = 100_000_000, 256, 148
+    if torch.cuda.mem_get_info()[0] < 30e9:
+        pytest.skip("needs 30 GB")
+    kv = torch.zeros(n, 1, D, dtype=torch.float16, device="cuda")
+    q = torch.zeros(s, h, D, dtype=torch.float16, device="cuda")
+    q[..., 0] = 8.0
+    kv[n - 300, 0, 0] = kv[n - 10, 0, 0] = 100.0              # 2^102 times the weight of a key of zeros
+    kv[n - 10, 0, 1] = 50.0
+    got = K.causal_attn(q, kv, kv, window=n, offset=n - s)
+    assert K.tc_error_flag() == 0
+    want = torch.zeros_like(got)
+    want[..., 0], want[s - 10:, :, 1] = 100.0, 25.0
+    assert torch.equal(got, want)
