@@ -4,9 +4,10 @@ import math
 import pytest
 import torch
 
-from test_gpu_pages import WEIGHT, D, K, check_decode, generator, normal, prompt_reference  # noqa: F401  (K: the fixture)
+from test_gpu_pages import WEIGHT, D, K, append, check_decode, decode, generator, normal, prompt_reference  # noqa: F401  (K: the fixture)
 
 pytestmark = pytest.mark.gpu
+KINDS = ["f16", "int8", "e4m3"]
 
 
 def general(q, k, v, window, sinks=0, offset=0, err=None, out=None):
@@ -133,3 +134,74 @@ def test_prompt_behind_100_million_keys(K):
     want = torch.zeros_like(got)
     want[..., 0], want[s - 10:, :, 1] = 100.0, 25.0
     assert torch.equal(got, want)
+
+
+# more than 148 units (sequences times groups of up to eight heads of a kv head), of one chunk of keys and of several: 2, 3, 4, 5, 7, 8 heads, and 12 as two groups
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("b,h,hkv,ps,keys,window,sinks", [(50, 8, 4, 16, 300, None, 0), (60, 9, 3, 20, 290, 200, 5), (100, 32, 8, 16, 520, None, 0), (160, 5, 1, 64, 130, 60, 0), (80, 14, 2, 16, 257, 100, 4),
+                                                          (20, 64, 8, 64, 300, None, 0), (40, 24, 2, 16, 300, 256, 1), (80, 4, 2, 16, 1600, None, 0), (53, 12, 3, 16, 1500, 1400, 4),
+                                                          (20, 64, 8, 16, 2000, None, 0), (170, 6, 1, 16, 1100, None, 0), (19, 64, 8, 64, 2300, 2100, 100)])
+def test_decode_of_large_batches(K, kind, b, h, hkv, ps, keys, window, sinks):
+    if kind == "f16" and window is None:
+        window = keys
+    g = generator(b + h + keys)
+    lens = torch.randint(keys // 4, keys + 1, (b,), generator=g, device="cuda", dtype=torch.int32)
+    lens[:4] = torch.tensor([keys, 0, 1, keys - 1])
+    run, want, size, _ = decode(K, kind, g, b, h, hkv, ps, keys, lens, window, sinks)
+    got = run()
+    check_decode(got, want, size)
+    assert not got[1].any() and torch.equal(run(), got)
+
+
+# more than 32768 rows, where a lane group takes four heads: parts of fewer, and parts that go from keys to values (hkv 3, 5, 6, and 1 beside 5 heads)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rotate", [True, False])
+@pytest.mark.parametrize("lens,starts,h,hkv,ps", [([1000, 0, 1, 777, 1100], [0, 5, 63, 100, 17], 6, 6, 64), ([4000, 1500], [3, 0], 5, 3, 100), ([9000, 7500], [0, 250], 1, 1, 256),
+                                                  ([1201, 999, 1100], [15, 16, 17], 9, 5, 16)])
+def test_append_of_long_runs(K, kind, rotate, lens, starts, h, hkv, ps):
+    assert sum(lens) * ((h if rotate else 0) + 2 * hkv) > 32768
+    append(K, kind, generator(sum(lens)), lens, starts, h, hkv, ps, rotate=rotate, extra=3)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_append_of_one_token_to_many_sequences(K, kind):
+    append(K, kind, generator(3), [1] * 1500, [i % 391 for i in range(1500)], 14, 5, 64, decode_form=True)
+
+
+@pytest.mark.parametrize("s,h,hkv,window,sinks,offset", [(1, 4, 2, 16, 4, 4000), (17, 4, 4, 16, 4, 4000), (64, 8, 2, 40, 10, 4001), (64, 2, 1, 1, 60, 999), (33, 3, 3, 20, 64, 700)])
+def test_prompt_of_few_queries_far_from_the_first_keys(K, s, h, hkv, window, sinks, offset):
+    g = generator(s)
+    q, k, v = normal(g, s, h, D), normal(g, offset + s, hkv, D), normal(g, offset + s, hkv, D)
+    check_weights(K.causal_attn(q, k, v, window=window, sinks=sinks, offset=offset), *prompt_reference(q, k, v, window, sinks, offset), v)
+
+
+@pytest.mark.parametrize("s,h,hkv,window,sinks,offset", [(300, 4, 2, 100, 70, 500), (1, 2, 2, 3000, 0, 2900), (129, 8, 1, 33, 200, 0), (700, 2, 1, 10000, 0, 10)])
+def test_prompt_by_the_general_kernel(K, s, h, hkv, window, sinks, offset):
+    """No error word: the kernel for small calls, over several blocks of queries and many tiles."""
+    g = generator(s)
+    q, k, v = normal(g, s, h, D), normal(g, offset + s, hkv, D), normal(g, offset + s, hkv, D)
+    check_weights(general(q, k, v, window, sinks, offset), *prompt_reference(q, k, v, window, sinks, offset), v)
+
+
+@pytest.mark.parametrize("s,window,offset", [(100, 5000, 5000), (1, 4000, 4000), (257, 3000, 3000)])
+def test_prompt_without_a_workspace(K, s, window, offset):
+    """... CTAs do not share the keys."""
+    g = generator(s)
+    q, k, v = normal(g, s, 4, D), normal(g, offset + s, 2, D), normal(g, offset + s, 2, D)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    check_weights(general(q, k, v, window, 3, offset, err=err), *prompt_reference(q, k, v, window, 3, offset), v)
+    assert not err.any()
+
+
+@pytest.mark.parametrize("s", [60, 300])
+@pytest.mark.parametrize("first,heads", [(2, 4), (0, 4), (8, 5)])
+def test_prompt_into_rows_off_16_bytes(K, s, first, heads):
+    """Output addresses that are multiples of 4 bytes, or rows that are not multiples of 16."""
+    g = generator(s)
+    q, k, v = normal(g, s, 4, D), normal(g, s, 2, D), normal(g, s, 2, D)
+    ld = heads * D + (2 if heads == 5 else 0)
+    room = torch.full((first + s * ld,), 7.0, dtype=torch.float16, device="cuda")
+    out = room[first:].view(s, ld)[:, :4 * D].unflatten(1, (4, D))
+    assert K.causal_attn(q, k, v, out, window=100, sinks=3).data_ptr() == out.data_ptr()
+    check_weights(out, *prompt_reference(q, k, v, 100, 3, 0), v)
+    assert (room[:first] == 7).all() and (room[first:].view(s, ld)[:, 4 * D:] == 7).all()
