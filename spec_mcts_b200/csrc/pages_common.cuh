@@ -14,9 +14,7 @@ enum CacheType { CACHE_F16 = 0, CACHE_I8 = 1, CACHE_E4M3 = 2 };
 template <int T>
 constexpr int cache_bytes = T == CACHE_F16 ? 2 : 1;
 template <int T>
-constexpr float cache_top = T == CACHE_I8 ? 127.f : 448.f;        // the code that a block's largest value gets
-template <int T>
-constexpr float cache_top_inv = T == CACHE_I8 ? 1.f / 127.f : 1.f / 448.f;
+constexpr float cache_top_inv = T == CACHE_I8 ? 1.f / 127.f : 1.f / 448.f;        // one over the code that a page's largest value gets
 
 // Where the tokens of a sequence are: page ids of `width` entries a sequence
 struct PageTable {
