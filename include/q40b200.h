@@ -473,6 +473,7 @@ int q40_attn_causal(const void* q, int64_t ldq, const void* k, int64_t ldk, cons
 
 /* q40_attn_causal for a prompt's positions offset .. offset + S - 1, whose keys and values are rows 0 .. offset + S - 1 of k and v, with a
  * window: the query at position p attends the keys j <= p with p - j < window or j < sinks.  offset + S <= 2^30.
+ * A value that is not finite reaches the queries that see its key, whatever its weight, and no others.  Weights are rounded to fp16 for the product.
  * `err` is a device int that a kernel on tcgen05, for longer prompts, sets to 1 if one of its bounded waits expires (NULL: that kernel is not used).
  * With *_workspace_bytes bytes of workspace (16-byte aligned, no initialisation; calls that may overlap need one each) CTAs share the keys where
  * queries are few; without (NULL) they do not. */

@@ -883,7 +883,7 @@ def page_append(p, k, v, kpool, vpool, pos, *, page_size: int = 1, offsets=None,
     returned rotated (zeros for rows of no sequence); a rotated value is rounded once, where rope_ keeps the reference's roundings.
 
     Rows of no sequence and positions without a page are not written.  An 8-bit page's scale grows with what comes, and its earlier
-    rows are coded anew when it does.  Tokens of one call that share a slot, or in 8 bits sequences that append to one page, leave it undefined
+    rows are coded anew when it does (pages of up to 2^26 tokens).  Tokens of one call that share a slot, or in 8 bits sequences that append to one page, leave it undefined
     (q40_page_append in include/q40b200.h)."""
     if _host_calls is not None:
         done = _host_calls.page_append(p, k, v, kpool, vpool, pos, page_size, offsets, k_scale, v_scale, q, cos, sin)     # None: not a plain call

@@ -205,3 +205,32 @@ def test_prompt_into_rows_off_16_bytes(K, s, first, heads):
     assert K.causal_attn(q, k, v, out, window=100, sinks=3).data_ptr() == out.data_ptr()
     check_weights(out, *prompt_reference(q, k, v, 100, 3, 0), v)
     assert (room[:first] == 7).all() and (room[first:].view(s, ld)[:, 4 * D:] == 7).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_prompt_in_chunks_as_documented(K, kind):
+    """Two chunks: keys rotated by rope_ beside those that page_append puts in the cache, and, of fp16 pages, the cache's own."""
+    from test_gpu_pages import TYPES, rotated, tables
+    g = generator(40)
+    total, done, h, hkv, ps, window, sinks = 200, 130, 8, 2, 16, 60, 3
+    x, (cos, sin) = normal(g, total, h + 2 * hkv, D), tables(total)
+    table = torch.randperm(13, generator=g, device="cuda", dtype=torch.int32)[None]
+    kpool = torch.zeros(hkv, 13 * ps, D, device="cuda").to(TYPES[kind])
+    vpool = kpool.clone()
+    scales = {} if kind == "f16" else dict(k_scale=torch.zeros(hkv, 13, device="cuda"), v_scale=torch.zeros(hkv, 13, device="cuda"))
+    k_of_one, v_of_one = (torch.zeros(total, hkv, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    at = torch.arange(total, device="cuda")
+    slots = table[0].long()[at // ps] * ps + at % ps
+    for first, n in ((0, done), (done, total - done)):
+        q, k, v = (y[first:first + n] for y in (x[:, :h], x[:, h:h + hkv], x[:, h + hkv:]))
+        q = K.page_append(table, k, v, kpool, vpool, torch.tensor([first], dtype=torch.int32, device="cuda"), page_size=ps, offsets=torch.tensor([0, n], dtype=torch.int32, device="cuda"),
+                          q=q, cos=cos, sin=sin, **scales)
+        k_of_one[first:first + n].copy_(k), v_of_one[first:first + n].copy_(v)
+        K.rope_(k_of_one[first:first + n], torch.arange(first, first + n, device="cuda"), cos, sin)
+        # both products and their sum rounded by 2^-11 (2^13 times the 2^-24 of `products`), and 2^-25 where they are subnormal
+        want, products = rotated(k, at[first:first + n], cos, sin)
+        assert ((k_of_one[first:first + n].double() - want).abs() <= 8200 * products + 2 ** -11 * want.abs() + 3 * 2 ** -25).all()
+        pairs = [(k_of_one, v_of_one)] + ([(p[:, slots].transpose(0, 1).contiguous() for p in (kpool, vpool))] if kind == "f16" else [])
+        for ks, vs in pairs:
+            got = K.causal_attn(q, ks, vs, window=window, sinks=sinks, offset=first)
+            check_weights(got, *prompt_reference(q, ks, vs, window, sinks, first), vs)
