@@ -13,9 +13,9 @@
 // Lane (g, t) has the scores of keys g and g + 8.  A key's scale multiplies its score; a value's, vs, its weight, as 2^(s + log2 vs - m),
 // where m is the largest s + log2 vs: the weights of the values, and not those of the scores, have to fit in fp16.
 //
-// What bounds it: many keys, HBM (64 sequences of up to 2048 e4m3 keys of 32 heads 124 us, 6.5 TB/s; 100 windows of 4096 fp16 keys of 8 heads 243 us, 6.9 TB/s), with eight
-// heads a unit, or at the power limit, instructions (18 a key of one head, 39 of eight; 8 x 65536 int8 keys under 64 heads 158 us where HBM takes 129); few keys, a warp's chain
-// of 1 us per 32 of them (512 int8 keys of 32 heads 5.9 us, 2000 9.7).
+// What bounds it: many keys, HBM (64 sequences of up to 2048 e4m3 keys of 32 heads 124 us, 6.5 TB/s; 100 windows of 4096 fp16 keys of 8 heads 243 us, 6.9 TB/s), at the
+// power limit instructions (18 a key of one head, 39 of eight); few units of eight heads, neither (8 x 65536 int8 keys under 64 heads 158 us where HBM takes 129: at 8 x 16384 issue slots are 54 %
+// busy, and a warp, whose ring has one stage, does not copy while it computes); few keys, a warp's chain of 1 us per 32 of them (512 int8 keys of 32 heads 5.9 us, 2000 9.7).
 #include <algorithm>
 
 #include "attn_tile.cuh"
@@ -26,7 +26,7 @@ namespace pages {
 
 constexpr int MERGE_THREADS = 128;
 // Warps of a CTA: eight with one stage of their ring while the units are no more than the SMs, else four with two.  Us, eight / four: 1 x 500 int8 keys of 8 heads
-// 5.7 / 6.7, 8 x 500 6.0 / 6.7, 8 x 2000 11.1 / 13.0, 64 units of up to 65536 157 / 152; fp16 1 x 2000 of 32 heads 9.3 / 10.5.  Eight with two stages (one CTA an SM) 1 x
+// 5.7 / 6.7, 8 x 500 6.0 / 6.7, 8 x 2000 11.1 / 13.0, 64 units of up to 65536 157 / 152 (four would be better for these, but lengths are not known here, and a table's width is not to decide); fp16 1 x 2000 of 32 heads 9.3 / 10.5.  Eight with two stages (one CTA an SM) 1 x
 // 30000 30 where one has 26
 constexpr int FEW = 148;                   // units
 // Keys of a chunk: one wave of CTAs (two an SM), if that leaves chunks of up to 2048 keys, else about 1200 CTAs, whose chunks even out lengths.  Us: 1 x 30000 keys of

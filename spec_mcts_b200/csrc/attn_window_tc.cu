@@ -21,7 +21,7 @@
 // Every wait is bounded: on expiry the error word is set, what is left is skipped, the CTA's own copies and MMAs are waited for (bounded too),
 // and tensor memory is freed.
 //
-// What bounds it: 16384 positions, window 4096, 64 heads on 8 take 1.655 ms, 1.17 PFLOP/s (70 % of a cuBLAS product's burst rate; at the power limit 0.99 of its 1.40).  The MMAs alone,
+// What bounds it: 16384 positions, window 4096, 64 heads on 8 take 1.66 to 1.70 ms, by the card, 1.13 PFLOP/s and more (68 % of a cuBLAS product's burst rate; at the power limit 1.00 of its 1.40).  The MMAs alone,
 // with softmax left out, take 1.469: one of 128 x 128 x 16 takes 87 cycles where 64 would be peak, and the hand-overs of a step the rest: a softmax of 128 keys takes 1750
 // cycles (maximum 280, each half of the weights 670) while the other tile's MMAs take 1480.  Steps on the way, ms: P handed on whole 1.89, in halves 1.80; two stages
 // of keys and of values, five slots for both 1.72; fewer comparisons and commits in the issuing thread 1.69.  A pair of CTAs that shares keys and values (cta_group::2) 1.80.

@@ -10,7 +10,7 @@
 // not finite makes its page's scale NaN, which whoever reads the page sees, until the page is begun anew.
 //
 // What bounds it: one token, a chain of four loads (position, page, scale or tables, store; 2.1 us with a launch); prompts, HBM: 4001 tokens of 96 heads in fp16
-// 33.0 us, 6.0 TB/s, 8191 of 64 + 2 x 8 heads into int8 pages of 64 56.7 us, 5.7 TB/s (with one head a lane group 83, pages behind the queries 65).
+// 33.0 us, 6.0 TB/s, 8191 of 64 + 2 x 8 heads into int8 pages of 64 56.7 us, 5.7 TB/s (with one head a lane group 83, pages behind the queries 65; its four heads a lane group at eight CTAs an SM spill 44 bytes a thread).
 #include "pages_common.cuh"
 
 namespace q40 {
