@@ -308,6 +308,8 @@ int q40_attn_paged(const void* page_tbl, int idx_bytes, int64_t tbl_stride, cons
  * at most Lmax <= 2^29 count) and the order of tokens as in q40_attn_paged.  A sequence without keys gets zeros.  Keys that are not visible are not
  * read.  An element whose scale is NaN is NaN.  Results do not depend on Lmax.  Workspace: *_workspace_bytes bytes, 16-byte aligned, no
  * initialisation (0 bytes: may be NULL); calls that may overlap need one each.  No counterpart in the reference. */
+#define Q40_SOFTCAP_LEAST 0.01f
+#define Q40_SOFTCAP_MOST 1000.f
 #define Q40_CACHE_F16 0
 #define Q40_CACHE_I8 1
 #define Q40_CACHE_E4M3 2
@@ -316,6 +318,43 @@ int q40_attn_pages(const void* page_tbl, int idx_bytes, int64_t tbl_stride, cons
                    const void* kpool, const void* vpool, const float* k_scale, const float* v_scale, int cache_type, void* o, int64_t P,
                    int B, int Lmax, int H, int Hkv, int D, int page_size, int window, int sinks, void* workspace,
                    size_t workspace_bytes, void* stream);
+
+/* q40_attn_pages with changed scores, as in q40_attn_causal_scores: softcap (0: none) and slopes [H] (NULL: none); a key's distance is that
+ * to the sequence's last position.  Workspace of q40_attn_pages. */
+int q40_attn_pages_scores(const void* page_tbl, int idx_bytes, int64_t tbl_stride, const int32_t* seq_lens, const void* q, int64_t q_stride,
+                          const void* kpool, const void* vpool, const float* k_scale, const float* v_scale, int cache_type, void* o, int64_t P,
+                          int B, int Lmax, int H, int Hkv, int D, int page_size, int window, int sinks, float softcap, const float* slopes,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* The books of a paged cache, in device memory: a table of page ids [B, W] int32 (rows of ld entries), lengths lens [B], and refs [n_pages], how many sequences list
+ * each page (0 or below: it is free).  A sequence's pages are the first ceil(length / page_size) entries of its row.  Each call writes the books as they are afterwards
+ * to *_out, with 0 behind a row's pages; but for the exceptions named the outputs may be the inputs (the same addresses and strides), and must not overlap them
+ * otherwise.  Lengths outside of 0 .. W * page_size count as the nearest of these, ids outside of the pool as no page's.  W < 2^29, n_pages <= 2^28.
+ * Results do not depend on the order in which threads come.  Books that do not fit each other make them undefined, and nothing else.
+ *
+ * Sequence b becomes what sequence parents[b] was, whose pages it lists from then on, or one of length 0, if that is outside of 0 .. B - 1; refs count what is
+ * listed anew, and no longer.  Table and lengths must not be written in place (Q40_E_UNSUPPORTED).  No counterpart in the reference beyond the fork of
+ * hf_model_q40_kv_shared.py:282-297, which copies. */
+int q40_page_fork(const int32_t* table, int64_t ld, const int32_t* lens, const int32_t* refs, const int32_t* parents, int32_t* table_out, int64_t ld_out,
+                  int32_t* lens_out, int32_t* refs_out, int B, int W, int n_pages, int page_size, void* stream);
+
+/* Sequence b gets add[b] tokens more, up to 16384 sequences.  Below 0: so many of its last ones less (down to none); pages that hold none of the others are given
+ * back.  Above 0: pages for them, and a page of its own in the place of its last one, if that has room and other sequences list it (of sequences that all get tokens
+ * and share a page which no other lists, the last keeps it): a copy of its rows so far, and its scales, in all `heads` of the pools [heads, P, 128] (P >= n_pages *
+ * page_size, cache_type and scales as in q40_attn_pages; `heads` may be those of several layers).  Pages that are free before the call are handed out in ascending
+ * order, to the sequences in theirs (a copy first).  A sequence whose pages do not fit in W, or whose last page is none of the pool's, stays as it is; so does the first that wants more pages than are left,
+ * and every one behind it that wants any.  Workspace: 16-byte aligned, no initialisation; calls that may overlap need one each. */
+size_t q40_page_extend_workspace_bytes(int B, int n_pages);
+int q40_page_extend(const int32_t* table, int64_t ld, const int32_t* lens, const int32_t* refs, const int32_t* add, int32_t* table_out, int64_t ld_out,
+                    int32_t* lens_out, int32_t* refs_out, int B, int W, int n_pages, int page_size, void* kpool, void* vpool, float* k_scale,
+                    float* v_scale, int cache_type, int64_t P, int heads, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Moves pages in use so that they are the first of their pools: with n of them in use, those from n on go, in order, to the free ones below.  where [n_pages] tells
+ * each page's new id (-1: it was free). */
+size_t q40_page_compact_workspace_bytes(int n_pages);
+int q40_page_compact(const int32_t* table, int64_t ld, const int32_t* lens, const int32_t* refs, int32_t* table_out, int64_t ld_out, int32_t* refs_out,
+                     int32_t* where, int B, int W, int n_pages, int page_size, void* kpool, void* vpool, float* k_scale, float* v_scale, int cache_type,
+                     int64_t P, int heads, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Appends new tokens' keys and values (rows of k_stride / v_stride elements, Hkv heads side by side) to pages as q40_attn_pages
  * reads them.  offsets NULL: T == B, row b is sequence b's one new token, at position pos[b].  Else rows offsets[b] .. offsets[b+1] - 1
@@ -481,6 +520,18 @@ size_t q40_attn_causal_window_workspace_bytes(int S, int H, int Hkv, int D, int 
 int q40_attn_causal_window(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* o, int64_t ldo,
                            int S, int H, int Hkv, int D, int offset, int window, int sinks, void* workspace, size_t workspace_bytes, int* err,
                            void* stream);
+
+/* q40_attn_causal_window with changed scores and further masks.  The score of key j for the query at position p is c tanh(x / c) - slopes[h] |p - j|, with x =
+ * q . k / sqrt(128): softcap = c (Q40_SOFTCAP_LEAST to _MOST; 0: x as it is), slopes [H] fp32 in device memory (NULL: none).
+ * documents, n_documents + 1 rising rows in device memory, with offset == 0 (NULL: all positions are one document): rows documents[i] .. documents[i + 1] - 1 see each
+ * other alone, and first keys (`sinks`) are those of the document.  Rows in front of the first and behind the last become zeros, or, with keep_rest, are left as
+ * they are.  The first prefixes[i] positions of document i (device memory; NULL: `prefix` of each) see each other in both directions: a query sees the keys j
+ * that are not behind it or are in the prefix, with p - j < window or among the first `sinks`.
+ * Entries that do not rise, or are out of range, make results undefined, and nothing else.  err and a driver that makes tensor maps are needed (Q40_E_UNSUPPORTED). */
+size_t q40_attn_causal_scores_workspace_bytes(int S, int H, int Hkv, int D, int offset, int window, int sinks);
+int q40_attn_causal_scores(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* o, int64_t ldo, int S, int H, int Hkv,
+                           int D, int offset, int window, int sinks, float softcap, const float* slopes, const int32_t* documents, int n_documents,
+                           const int32_t* prefixes, int prefix, int keep_rest, void* workspace, size_t workspace_bytes, int* err, void* stream);
 
 /* The layers of a prompt pass, enqueued by one call: per layer q40_rmsnorm (adding the previous layer's output), q40_gemm_tiled_tc_multi
  * for wq, wk and wv (keys and values into the prompt cache), q40_rope_qk, q40_attn_causal, wo, q40_rmsnorm, q40_gemm_tiled_tc_ws with the SiLU

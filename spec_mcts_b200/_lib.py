@@ -50,6 +50,9 @@ SIGNATURES = {
     "q40_attn_causal_window": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64] + [c_int] * 7 +
                                [c_void_p, c_size_t, c_void_p, c_void_p]),
     "q40_attn_causal_window_workspace_bytes": (c_size_t, [c_int] * 7),
+    "q40_attn_causal_scores": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64] + [c_int] * 7 +
+                               [c_float, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "q40_attn_causal_scores_workspace_bytes": (c_size_t, [c_int] * 7),
     "q40_attn_causal": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int,
                                 c_int, c_int, c_int, c_void_p]),
     "q40_tp_layout": (c_int, [c_int, c_int, c_int, c_void_p]),
@@ -103,6 +106,15 @@ SIGNATURES = {
     "q40_attn_pages_workspace_bytes": (c_size_t, [c_int] * 6),
     "q40_attn_pages": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64] + [c_void_p] * 4 + [c_int, c_void_p, c_int64] +
                        [c_int] * 8 + [c_void_p, c_size_t, c_void_p]),
+    "q40_attn_pages_scores": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64] + [c_void_p] * 4 + [c_int, c_void_p, c_int64] +
+                              [c_int] * 8 + [c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "q40_page_fork": (c_int, [c_void_p, c_int64] + [c_void_p] * 4 + [c_int64, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p]),
+    "q40_page_extend_workspace_bytes": (c_size_t, [c_int] * 2),
+    "q40_page_extend": (c_int, [c_void_p, c_int64] + [c_void_p] * 4 + [c_int64, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 4 +
+                        [c_int, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
+    "q40_page_compact_workspace_bytes": (c_size_t, [c_int]),
+    "q40_page_compact": (c_int, [c_void_p, c_int64] + [c_void_p] * 3 + [c_int64, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 4 +
+                         [c_int, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
     "q40_page_append": (c_int, [c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
                                 c_int64, c_void_p, c_void_p, c_int] + [c_void_p] * 4 + [c_int, c_int64] + [c_int] * 6 + [c_void_p]),
     "q40_attn_shared_prefix_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),

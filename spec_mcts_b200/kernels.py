@@ -44,7 +44,7 @@ GROUP_SIZE = 64
 __all__ = [
     "quantize_q40", "dequantize_q40", "triton_deq_int40", "triton_q_int40", "triton_q_int40_sliced",
     "quantize_q40_rows", "matmul", "matmul_q40", "linear_q40", "flash_attn", "page_flash_attn",
-    "page_flash_attn_q8", "page_append", "causal_attn", "triton_attn", "chunk_attn", "shared_prefix_attn", "matmul_split_k", "rmsnorm", "rope_", "silu_mul",
+    "page_flash_attn_q8", "page_append", "page_fork", "page_extend", "page_compact", "causal_attn", "triton_attn", "chunk_attn", "shared_prefix_attn", "matmul_split_k", "rmsnorm", "rope_", "silu_mul",
     "gemv_fused", "gemv_stream", "stream_status", "embed_rows", "tc_error_flag", "relayout_tiled", "relayout_cache_config",
     "Q40Error",
 ]
@@ -576,13 +576,21 @@ def gemv_fused(mode: int, a: torch.Tensor, weights, *, norm_w=None, ss_in=None, 
 
 
 def causal_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional[torch.Tensor] = None, *,
-                window: Optional[int] = None, sinks: int = 0, offset: int = 0) -> torch.Tensor:
+                window: Optional[int] = None, sinks: int = 0, offset: int = 0, softcap: Optional[float] = None, slopes: Optional[torch.Tensor] = None,
+                documents: Optional[torch.Tensor] = None, prefix=0) -> torch.Tensor:
     """Causal attention of a prompt: q [S, H, 128], k / v [S, Hkv, 128] (position-major, last two dims
     contiguous) -> [S, H, 128]; position i attends positions 0..i (q40_attn_causal in include/q40b200.h).
 
     With `window` a position attends its last `window` positions, itself among them, and the first `sinks`.  With `offset` the queries
     are positions offset .. offset + S - 1 of a longer prompt, whose first offset + S keys and values k and v hold
-    (q40_attn_causal_window)."""
+    (q40_attn_causal_window).
+
+    q40_attn_causal_scores: with `softcap` c (0.01 to 1000) scores x become c tanh(x / c); with `slopes` [H] they then fall by slopes[h] for each position between query
+    and key.  With `documents`, int32 [n + 1], rows documents[i] .. documents[i + 1] - 1 are a prompt each, which sees itself alone (and its own first `sinks`);
+    rows of none become zeros, or stay as they are in `out`.  The first `prefix` positions (of each document; an int32 tensor [n]: of document i
+    its own number) see each other in both directions."""
+    if softcap is not None or slopes is not None or documents is not None or (prefix is not None and (isinstance(prefix, torch.Tensor) or prefix != 0)):
+        return _causal_scores(q, k, v, out, window, sinks, offset, softcap, slopes, documents, prefix)
     if out is None and (window is not None or sinks != 0 or offset != 0) and _host_calls is not None:
         o = _host_calls.causal_window(q, k, v, window, sinks, offset, _workspaces)      # None: not a plain call
         if o is not None:
@@ -620,6 +628,63 @@ def causal_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional
         return out
     check(lib.q40_attn_causal(q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
                               out.data_ptr(), out.stride(0), S, H, Hkv, D, _stream(dev)), "q40_attn_causal")
+    return out
+
+
+SOFTCAP = (0.01, 1000.0)             # Q40_SOFTCAP_LEAST, Q40_SOFTCAP_MOST
+
+
+def _scores_of(what: str, heads: int, softcap, slopes):
+    """Cap (0: none) and slopes (fp32, or None) as the library takes them."""
+    if softcap is not None and not SOFTCAP[0] <= softcap <= SOFTCAP[1]:
+        raise Q40Error(f"{what}: softcap {softcap} outside of {SOFTCAP[0]} to {SOFTCAP[1]:g}")
+    if slopes is not None:
+        if slopes.shape != (heads,) or not slopes.is_floating_point():
+            raise Q40Error(f"{what}: {heads} slopes expected, got {tuple(slopes.shape)} of {slopes.dtype}")
+        slopes = slopes.to(torch.float32).contiguous()
+    return 0.0 if softcap is None else float(softcap), slopes
+
+
+def _causal_scores(q, k, v, out, window, sinks, offset, softcap, slopes, documents, prefix):
+    own = prefix if isinstance(prefix, torch.Tensor) else None       # of each document
+    dev = _need_cuda(q, k, v, out, slopes, documents, own)
+    for t in (q, k, v):
+        if t.dtype != torch.float16 or t.dim() != 3 or t.shape[2] != 128 or t.stride(2) != 1 or (t.stride(1) != 128 and t.shape[1] > 1):
+            raise Q40Error("causal_attn: fp16 tensors [S, heads, 128] with contiguous heads expected")
+    S, H, D = q.shape
+    Hkv = k.shape[1]
+    if offset < 0 or sinks < 0 or (window is not None and window < 1):
+        raise Q40Error(f"causal_attn: window {window} below 1, sinks {sinks} or offset {offset} below 0")
+    if min(k.shape[0], v.shape[0]) < offset + S or v.shape[1] != Hkv:
+        raise Q40Error(f"causal_attn: keys {tuple(k.shape)} and values {tuple(v.shape)} do not hold {offset + S} positions of [kv heads, {D}]")
+    if out is not None and (out.shape != q.shape or out.dtype != torch.float16 or out.stride(2) != 1 or (out.stride(1) != D and H > 1)):
+        raise Q40Error("causal_attn: fp16 out like q with contiguous heads expected")
+    cap, slopes = _scores_of("causal_attn", H, softcap, slopes)
+    n = 0
+    if documents is not None:
+        n = documents.shape[0] - 1 if documents.dim() == 1 else -1
+        if n < 0 or documents.dtype != torch.int32 or offset != 0:
+            raise Q40Error(f"causal_attn: documents as int32 [n + 1] and offset 0 expected, got {tuple(documents.shape)} of {documents.dtype} and {offset}")
+        documents = documents.contiguous()
+    if own is not None:
+        if documents is None or own.shape != (n,) or own.dtype != torch.int32:
+            raise Q40Error(f"causal_attn: a prefix for each document as int32 [{n}] expected, got {tuple(own.shape)} of {own.dtype}")
+        own, prefix = own.contiguous(), 0
+    elif (prefix := prefix or 0) < 0:
+        raise Q40Error(f"causal_attn: prefix {prefix} below 0")
+    keep = out is not None
+    if out is None:
+        out = torch.empty((S, H, D), dtype=torch.float16, device=dev)
+    if S == 0:
+        return out
+    st, whole = _stream(dev), offset + S
+    err = _tc_error_page(dev, st).data_ptr() + 4092
+    lds = [t.stride(0) if t.shape[0] > 1 else t.shape[1] * D for t in (q, k, v, out)]
+    w, sinks = whole if window is None else min(window, whole), min(sinks, whole)
+    nbytes = lib.q40_attn_causal_scores_workspace_bytes(S, H, Hkv, D, offset, w, sinks)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None           # of this call alone, as in _attn_pages
+    check(lib.q40_attn_causal_scores(q.data_ptr(), lds[0], k.data_ptr(), lds[1], v.data_ptr(), lds[2], out.data_ptr(), lds[3], S, H, Hkv, D, offset, w, sinks, cap,
+                                     _ptr(slopes), _ptr(documents), n, _ptr(own), min(prefix, whole), keep, _ptr(ws), nbytes, err, st), "q40_attn_causal_scores")
     return out
 
 
@@ -757,21 +822,23 @@ def _table(p: torch.Tensor):
     return p.to(torch.int32), 4
 
 
-def page_flash_attn(p, q, k, v, P, B, L, H, D, *, page_size: int = 1, seq_lens=None, window: Optional[int] = None, sinks: int = 0):
+def page_flash_attn(p, q, k, v, P, B, L, H, D, *, page_size: int = 1, seq_lens=None, window: Optional[int] = None, sinks: int = 0,
+                    softcap: Optional[float] = None, slopes: Optional[torch.Tensor] = None):
     """Paged decode attention; same call as the reference's page_flash_attn
     (triton_kernels.py:764-789): p [B,L] int16 token-slot table, k/v pools [H,P,D].
     Extensions: page_size > 1 (p then lists page ids), int32 tables, per-branch seq_lens; with `window`, a query, which is its branch's
-    last position, attends that many last keys and the first `sinks` alone."""
-    windowed = window is not None or sinks != 0
-    if windowed and D == 128 and _host_calls is not None and q.shape == (B, H, D) and k.dtype == torch.float16 and k.shape[1:] == (P, D):
+    last position, attends that many last keys and the first `sinks` alone.  With `softcap` c (0.01 to 1000) scores x become c tanh(x / c); with `slopes` [H] they
+    then fall by slopes[h] for each position between key and query (q40_attn_pages_scores in include/q40b200.h)."""
+    windowed = window is not None or sinks != 0 or softcap is not None or slopes is not None
+    if windowed and softcap is None and slopes is None and D == 128 and _host_calls is not None and q.shape == (B, H, D) and k.dtype == torch.float16 and k.shape[1:] == (P, D):
         o = _host_calls.attn_pages(p, q, k, v, None, None, L, page_size, seq_lens, window, sinks)      # None: not a plain call
         if o is not None:
             return o
-    dev = _need_cuda(p, q, k, v, seq_lens)
+    dev = _need_cuda(p, q, k, v, seq_lens, slopes)
     if windowed:
         if k.dtype != torch.float16 or v.dtype != torch.float16 or q.shape != (B, H, D) or k.shape[1:] != (P, D) or v.shape != k.shape:
             raise Q40Error(f"page_flash_attn: fp16 pools [kv heads, {P}, {D}] and queries [{B}, {H}, {D}] expected")
-        return _attn_pages("page_flash_attn", dev, p, q, k.contiguous(), v.contiguous(), None, None, L, page_size, seq_lens, window, sinks)
+        return _attn_pages("page_flash_attn", dev, p, q, k.contiguous(), v.contiguous(), None, None, L, page_size, seq_lens, window, sinks, softcap, slopes)
     p, idx_bytes = _table(p)
     if p.stride(-1) != 1:
         p = p.contiguous()
@@ -830,13 +897,15 @@ def _page_table(what: str, p: torch.Tensor, rows: int):
     return p, idx_bytes, p.stride(0) if rows > 1 else p.shape[1]
 
 
-def _attn_pages(what, dev, p, q, k, v, k_scale, v_scale, L, page_size, seq_lens, window, sinks):
+def _attn_pages(what, dev, p, q, k, v, k_scale, v_scale, L, page_size, seq_lens, window, sinks, softcap=None, slopes=None):
     kind = _need_pools(what, k, v, k_scale, v_scale, page_size)
     if q.dim() != 3 or q.dtype != torch.float16 or q.shape[2] != k.shape[2]:
         raise Q40Error(f"{what}: fp16 queries [sequences, heads, {k.shape[2]}] expected, got {tuple(q.shape)} of {q.dtype}")
     if (window is not None and window < 1) or sinks < 0:
         raise Q40Error(f"{what}: window {window} below 1 or sinks {sinks} below 0")
     B, H, D = q.shape
+    changed = softcap is not None or slopes is not None
+    cap, slopes = _scores_of(what, H, softcap, slopes)
     p, idx_bytes, tbl_stride = _page_table(what, p, B)
     if not 0 <= L <= min(p.shape[1] * page_size, 1 << 29):
         raise Q40Error(f"{what}: {L} keys (at most 2^29) and a table of {p.shape[1]} pages of {page_size}")
@@ -852,25 +921,30 @@ def _attn_pages(what, dev, p, q, k, v, k_scale, v_scale, L, page_size, seq_lens,
     nbytes = lib.q40_attn_pages_workspace_bytes(B, H, k.shape[0], L, w, sinks)
     # of this call alone: calls on other streams and captured graphs that overlap it have their own
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    check(lib.q40_attn_pages(p.data_ptr(), idx_bytes, tbl_stride, _ptr(seq_lens), q.data_ptr(), _row_stride(q), k.data_ptr(), v.data_ptr(),
-                             _ptr(k_scale), _ptr(v_scale), kind, o.data_ptr(), k.shape[1], B, L, H, k.shape[0], D, page_size, w, sinks,
-                             _ptr(ws), nbytes, _stream(dev)), "q40_attn_pages")
+    args = (p.data_ptr(), idx_bytes, tbl_stride, _ptr(seq_lens), q.data_ptr(), _row_stride(q), k.data_ptr(), v.data_ptr(), _ptr(k_scale), _ptr(v_scale), kind,
+            o.data_ptr(), k.shape[1], B, L, H, k.shape[0], D, page_size, w, sinks)
+    if changed:
+        check(lib.q40_attn_pages_scores(*args, cap, _ptr(slopes), _ptr(ws), nbytes, _stream(dev)), "q40_attn_pages_scores")
+    else:
+        check(lib.q40_attn_pages(*args, _ptr(ws), nbytes, _stream(dev)), "q40_attn_pages")
     return o
 
 
-def page_flash_attn_q8(p, q, k, v, k_scale, v_scale, *, page_size: int, seq_lens=None, window: Optional[int] = None, sinks: int = 0):
+def page_flash_attn_q8(p, q, k, v, k_scale, v_scale, *, page_size: int, seq_lens=None, window: Optional[int] = None, sinks: int = 0,
+                       softcap: Optional[float] = None, slopes: Optional[torch.Tensor] = None):
     """page_flash_attn over a cache held in 8 bits: pools k / v [Hkv, P, 128] of int8 or float8_e4m3fn codes with one fp32 scale for each
     page and kv head, k_scale / v_scale [Hkv, P / page_size] (element = code * scale), as page_append writes them.  q [B, H, 128] is
     one query for each sequence, its last position; p [B, pages] lists page ids, seq_lens [B] the lengths (None: the table's whole width).
-    With `window` a query attends that many last keys and the first `sinks` alone (q40_attn_pages in include/q40b200.h)."""
-    if _host_calls is not None and k.dtype != torch.float16:
+    With `window` a query attends that many last keys and the first `sinks` alone (q40_attn_pages in include/q40b200.h).  `softcap` and `slopes` as in
+    page_flash_attn."""
+    if _host_calls is not None and softcap is None and slopes is None and k.dtype != torch.float16:
         o = _host_calls.attn_pages(p, q, k, v, k_scale, v_scale, p.shape[-1] * page_size, page_size, seq_lens, window, sinks)      # None: not a plain call
         if o is not None:
             return o
-    dev = _need_cuda(p, q, k, v, k_scale, v_scale, seq_lens)
+    dev = _need_cuda(p, q, k, v, k_scale, v_scale, seq_lens, slopes)
     if k.dtype == torch.float16:
         raise Q40Error("page_flash_attn_q8: 8-bit pools expected; page_flash_attn reads fp16 ones")
-    return _attn_pages("page_flash_attn_q8", dev, p, q, k, v, k_scale, v_scale, p.shape[-1] * page_size, page_size, seq_lens, window, sinks)
+    return _attn_pages("page_flash_attn_q8", dev, p, q, k, v, k_scale, v_scale, p.shape[-1] * page_size, page_size, seq_lens, window, sinks, softcap, slopes)
 
 
 def page_append(p, k, v, kpool, vpool, pos, *, page_size: int = 1, offsets=None, k_scale=None, v_scale=None, q=None, cos=None, sin=None):
@@ -927,6 +1001,123 @@ def page_append(p, k, v, kpool, vpool, pos, *, page_size: int = 1, offsets=None,
     # writes that torch did not make itself: counted, as by quantize_q40_rows
     torch.autograd.graph.increment_version([t for t in (kpool, vpool, k_scale, v_scale) if t is not None and not t.is_inference()])
     return q_out
+
+
+def _span(t: torch.Tensor):
+    """Addresses that a tensor lies in."""
+    return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())) if t.numel() else 0)
+
+
+def _books(what: str, p, lens, refs, page_size: int, out, fresh):
+    """The books of a paged cache as the library reads them, and what it writes them to: `out`, or new tensors like `fresh`."""
+    if p.dim() != 2 or p.dtype != torch.int32 or lens.shape != p.shape[:1] or lens.dtype != torch.int32 or refs.dim() != 1 or refs.dtype != torch.int32:
+        raise Q40Error(f"{what}: int32 table [sequences, pages], lengths [sequences] and references [pages of the pool] expected, got {tuple(p.shape)} of {p.dtype}, "
+                       f"{tuple(lens.shape)} of {lens.dtype} and {tuple(refs.shape)} of {refs.dtype}")
+    if not 1 <= page_size <= 1 << 29 or p.shape[1] >= 1 << 29 or refs.shape[0] > 1 << 28:
+        raise Q40Error(f"{what}: page_size {page_size}, {p.shape[1]} pages a sequence, {refs.shape[0]} in all")
+    made = p, lens, refs
+    replaces = [next((m for m in made if m is t), None) for t in fresh[:2]] + [fresh[2] if len(set(map(id, fresh))) == 3 else None]
+    if p.stride(1) != 1 and p.shape[1] > 1 or (p.shape[0] > 1 and p.stride(0) < p.shape[1]):
+        p = p.contiguous()
+    lens, refs = lens.contiguous(), refs.contiguous()
+    if out is None:
+        return p, lens, refs, [torch.empty(t.shape, dtype=torch.int32, device=t.device) for t in fresh]
+    if len(out) != len(fresh):
+        raise Q40Error(f"{what}: out has {len(out)} tensors, {len(fresh)} expected")
+    for t, like in zip(out, fresh):
+        if t.shape != like.shape or t.dtype != torch.int32 or not t.is_contiguous() and (t.dim() == 1 or t.stride(1) != 1 or t.stride(0) < t.shape[1]):
+            raise Q40Error(f"{what}: out like the books expected, got {tuple(t.shape)} of {t.dtype} with strides {t.stride()}")
+    for i, t in enumerate(out):
+        for other in [*made, *out[:i]]:
+            (a, b), (c, d) = _span(t), _span(other)
+            same = other is replaces[i] and a == c and t.stride() == other.stride()
+            if max(a, c) < min(b, d) and not same:
+                raise Q40Error(f"{what}: out overlaps the books, or itself, other than by being what it replaces")
+    return p, lens, refs, list(out)
+
+
+def _table_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _counted(*ts) -> None:
+    """Writes that torch did not make itself, as by quantize_q40_rows."""
+    torch.autograd.graph.increment_version([t for t in ts if t is not None and not t.is_inference()])
+
+
+def _books_pools(what: str, kpool, vpool, k_scale, v_scale, refs, page_size: int):
+    """Pools [.., kv heads, P, 128], of several layers too, as [heads, P, 128], and their Q40_CACHE_*."""
+    if kpool.dim() < 3 or kpool.shape != vpool.shape or not (kpool.is_contiguous() and vpool.is_contiguous()):
+        raise Q40Error(f"{what}: contiguous pools [.., kv heads, slots, 128] of one shape expected, got {tuple(kpool.shape)} and {tuple(vpool.shape)}")
+    for s in (k_scale, v_scale):
+        if s is not None and (s.shape[:-1] != kpool.shape[:-2] or not s.is_contiguous()):
+            raise Q40Error(f"{what}: contiguous scales like the pools expected, got {tuple(s.shape)}")
+    flat = lambda t: None if t is None else t.reshape(math.prod(kpool.shape[:-2]), *t.shape[len(kpool.shape) - 2:])
+    k, v, ks, vs = flat(kpool), flat(vpool), flat(k_scale), flat(v_scale)
+    kind = _need_pools(what, k, v, ks, vs, page_size)
+    if k.shape[2] != 128 or refs.shape[0] * page_size > k.shape[1]:
+        raise Q40Error(f"{what}: {refs.shape[0]} pages of {page_size} tokens of 128 and pools {tuple(kpool.shape)}")
+    return k, v, ks, vs, kind
+
+
+def page_fork(p, lens, refs, parents, *, page_size: int, out=None):
+    """Sequences of a paged cache become continuations of others, whose pages they share: sequence b is from then on what sequence parents[b] was, and holds nothing if that is
+    -1.  The cache's books are the table p [B, pages] of page ids and lengths lens [B], as page_append and page_flash_attn read them, and refs [pages of the pool], how many
+    sequences list each page (0: it is free); all int32.  Returns them as they are afterwards (zeros behind a sequence's pages), in new tensors or in
+    out = (p, lens, refs), which may be the books themselves.  page_extend gives sequences that share a page their own before they write to it
+    (q40_page_fork in include/q40b200.h)."""
+    dev = _need_cuda(p, lens, refs, parents, *(out or ()))
+    p, lens, refs, new = _books("page_fork", p, lens, refs, page_size, out, (p, lens, refs))
+    B, W = p.shape
+    if parents.shape != (B,) or parents.is_floating_point():
+        raise Q40Error(f"page_fork: {B} parents expected, got {tuple(parents.shape)} of {parents.dtype}")
+    parents = parents.to(torch.int32).contiguous()
+    if out is not None:                           # sequences read each other's rows
+        p = p.clone() if p.data_ptr() == new[0].data_ptr() else p
+        lens = lens.clone() if lens.data_ptr() == new[1].data_ptr() else lens
+    check(lib.q40_page_fork(p.data_ptr(), _table_stride(p), lens.data_ptr(), refs.data_ptr(), parents.data_ptr(), new[0].data_ptr(), _table_stride(new[0]),
+                            new[1].data_ptr(), new[2].data_ptr(), B, W, refs.shape[0], page_size, _stream(dev)), "page_fork")
+    if out is not None:
+        _counted(*new)
+    return tuple(new)
+
+
+def page_extend(p, lens, refs, kpool, vpool, add, *, page_size: int, k_scale=None, v_scale=None, out=None):
+    """Pages for the next add[b] tokens of each sequence, whose length grows by them (page_append then writes them, from position lens[b] as it was on); where add[b] is below
+    0, its last tokens are taken back, and their pages given back.  A last page that has room, and that other sequences list, becomes a page of its own, with a copy of
+    its rows in the pools [.., Hkv, P, 128] (of several layers at once, in front of the heads; scales [.., Hkv, P / page_size] of 8-bit ones alike), in place.  Free pages are
+    handed out in ascending order; a sequence that its row of the table or the free pages have no room for keeps its length, and so does every one behind the latter that needs a
+    page.  Books and `out` as in page_fork; up to 16384 sequences (q40_page_extend in include/q40b200.h)."""
+    dev = _need_cuda(p, lens, refs, kpool, vpool, add, k_scale, v_scale, *(out or ()))
+    k, v, ks, vs, kind = _books_pools("page_extend", kpool, vpool, k_scale, v_scale, refs, page_size)
+    p, lens, refs, new = _books("page_extend", p, lens, refs, page_size, out, (p, lens, refs))
+    B, W = p.shape
+    if add.shape != (B,) or add.is_floating_point() or B > 16384:
+        raise Q40Error(f"page_extend: numbers of tokens for {B} sequences (at most 16384) expected, got {tuple(add.shape)} of {add.dtype}")
+    add = add.to(torch.int32).contiguous()
+    nbytes = lib.q40_page_extend_workspace_bytes(B, refs.shape[0])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)        # of this call alone, as in _attn_pages
+    check(lib.q40_page_extend(p.data_ptr(), _table_stride(p), lens.data_ptr(), refs.data_ptr(), add.data_ptr(), new[0].data_ptr(), _table_stride(new[0]), new[1].data_ptr(),
+                              new[2].data_ptr(), B, W, refs.shape[0], page_size, k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), kind, k.shape[1], k.shape[0], ws.data_ptr(),
+                              nbytes, _stream(dev)), "page_extend")
+    _counted(kpool, vpool, k_scale, v_scale, *(out or ()))
+    return tuple(new)
+
+
+def page_compact(p, lens, refs, kpool, vpool, *, page_size: int, k_scale=None, v_scale=None, out=None):
+    """Pages in use become the first ones of their pools (in place; pools and scales as in page_extend): with n of them, those from n on move, in order, to the free ones
+    below.  Returns the table and the references as they are afterwards, and where [pages of the pool], the new id of each page (-1: it was free), in new tensors or in
+    out = (p, refs, where), of which the first two may be the books themselves (q40_page_compact in include/q40b200.h)."""
+    dev = _need_cuda(p, lens, refs, kpool, vpool, k_scale, v_scale, *(out or ()))
+    k, v, ks, vs, kind = _books_pools("page_compact", kpool, vpool, k_scale, v_scale, refs, page_size)
+    p, lens, refs, new = _books("page_compact", p, lens, refs, page_size, out, (p, refs, refs))
+    nbytes = lib.q40_page_compact_workspace_bytes(refs.shape[0])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    check(lib.q40_page_compact(p.data_ptr(), _table_stride(p), lens.data_ptr(), refs.data_ptr(), new[0].data_ptr(), _table_stride(new[0]), new[1].data_ptr(),
+                               new[2].data_ptr(), p.shape[0], p.shape[1], refs.shape[0], page_size, k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), kind, k.shape[1],
+                               k.shape[0], ws.data_ptr(), nbytes, _stream(dev)), "page_compact")
+    _counted(kpool, vpool, k_scale, v_scale, *(out or ()))
+    return tuple(new)
 
 
 def shared_prefix_attn(q, prefix_k, prefix_v, prefix_len, p, seq_lens, kpool, vpool, *,
