@@ -11,9 +11,12 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <ATen/ops/clone.h>
 #include <ATen/ops/empty.h>
 
 #include <algorithm>
+#include <initializer_list>
+#include <utility>
 
 namespace {
 
@@ -158,6 +161,23 @@ using PageAppend = int (*)(const void*, int, int64_t, int, const int32_t*, const
 using CausalWindow = int (*)(const void*, int64_t, const void*, int64_t, const void*, int64_t, void*, int64_t, int, int, int, int, int, int, int, void*,
                              size_t, int*, void*);
 using CausalWindowBytes = size_t (*)(int, int, int, int, int, int, int);
+using AttnPagesScores = int (*)(const void*, int, int64_t, const int32_t*, const void*, int64_t, const void*, const void*, const float*, const float*, int, void*,
+                                int64_t, int, int, int, int, int, int, int, int, float, const float*, void*, size_t, void*);
+using CausalScores = int (*)(const void*, int64_t, const void*, int64_t, const void*, int64_t, void*, int64_t, int, int, int, int, int, int, int, float, const float*,
+                             const int32_t*, int, const int32_t*, int, int, void*, size_t, int*, void*);
+using PageFork = int (*)(const int32_t*, int64_t, const int32_t*, const int32_t*, const int32_t*, int32_t*, int64_t, int32_t*, int32_t*, int, int, int, int, void*);
+using PageExtend = int (*)(const int32_t*, int64_t, const int32_t*, const int32_t*, const int32_t*, int32_t*, int64_t, int32_t*, int32_t*, int, int, int, int, void*, void*, float*,
+                           float*, int, int64_t, int, void*, size_t, void*);
+using PageCompact = int (*)(const int32_t*, int64_t, const int32_t*, const int32_t*, int32_t*, int64_t, int32_t*, int32_t*, int, int, int, int, void*, void*, float*, float*, int,
+                            int64_t, int, void*, size_t, void*);
+AttnPagesScores attn_pages_scores_fn = nullptr;
+CausalScores causal_scores_fn = nullptr;
+CausalWindowBytes causal_scores_bytes = nullptr;
+PageFork page_fork_fn = nullptr;
+PageExtend page_extend_fn = nullptr;
+PageCompact page_compact_fn = nullptr;
+size_t (*page_extend_bytes)(int, int) = nullptr;
+size_t (*page_compact_bytes)(int) = nullptr;
 AttnPages attn_pages_fn = nullptr;
 AttnPagesBytes attn_pages_bytes = nullptr;
 PageAppend page_append_fn = nullptr;
@@ -225,10 +245,22 @@ at::Tensor heads(int64_t rows, int64_t n, int dev) {
 // Tensors that are used while other Python threads run
 at::Tensor held(const at::Tensor* t) { return t ? *t : at::Tensor(); }
 
-// attn_pages(p, q, k, v, k_scale, v_scale, L, page_size, seq_lens, window, sinks) -> o or None
+// A cap (0: None) and slopes of H heads (nullptr: None)
+bool scores_of(PyObject* cap, PyObject* slopes, int dev, int64_t H, float& c, const at::Tensor*& t) {
+  c = 0.f;
+  if (cap != Py_None) {
+    if (PyFloat_CheckExact(cap)) c = (float)PyFloat_AS_DOUBLE(cap);
+    if (!(c > 0.f)) return false;
+  }
+  bool fine = true;
+  t = tensor_or_none(slopes, fine);
+  return fine && (!t || vector_of(t, dev, at::kFloat, H));
+}
+
+// attn_pages(p, q, k, v, k_scale, v_scale, L, page_size, seq_lens, window, sinks, softcap, slopes) -> o or None
 PyObject* attn_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 11 || !attn_pages_fn) Py_RETURN_NONE;
+  if (n != 13 || !attn_pages_fn) Py_RETURN_NONE;
   bool fine = true;
   const at::Tensor *p = tensor(args[0]), *q = tensor(args[1]), *k = tensor(args[2]), *v = tensor(args[3]), *ks = tensor_or_none(args[4], fine),
                    *vs = tensor_or_none(args[5], fine), *lens = tensor_or_none(args[8], fine);
@@ -243,9 +275,14 @@ PyObject* attn_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int kind = pools_of(k, v, ks, vs, dev, ps);
   if (kind < 0 || !table_of(p, dev, B, tbl) || L > tbl.width * ps || (lens && !vector_of(lens, dev, at::kInt, B))) Py_RETURN_NONE;
   if (args[9] == Py_None) sinks = 0;
+  float cap;
+  const at::Tensor* slopes;
+  if (!scores_of(args[11], args[12], dev, H, cap, slopes)) Py_RETURN_NONE;
+  const bool changed = slopes || cap != 0.f;
+  if (changed && !attn_pages_scores_fn) Py_RETURN_NONE;
   const int Hkv = (int)k->size(0);
   const auto stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
-  const at::Tensor own[] = {held(p), held(q), held(k), held(v), held(ks), held(vs), held(lens)};
+  const at::Tensor own[] = {held(p), held(q), held(k), held(v), held(ks), held(vs), held(lens), held(slopes)};
   at::Tensor o, ws;
   int rc;
   {
@@ -253,9 +290,14 @@ PyObject* attn_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const size_t bytes = attn_pages_bytes((int)B, (int)H, Hkv, (int)L, (int)window, (int)sinks);
     o = heads(B, H, dev);
     ws = scratch(bytes, dev);
-    rc = attn_pages_fn(tbl.ids, tbl.bytes, tbl.ld, (const int32_t*)ptr(lens), own[1].data_ptr(), ld, own[2].data_ptr(), own[3].data_ptr(), (const float*)ptr(ks),
-                       (const float*)ptr(vs), kind, o.data_ptr(), own[2].size(1), (int)B, (int)L, (int)H, Hkv, (int)HEAD, (int)ps, (int)window, (int)sinks,
-                       bytes ? ws.data_ptr() : nullptr, bytes, stream);
+    const auto at = [&](int i) { return own[i].defined() ? own[i].data_ptr() : nullptr; };
+    if (changed)
+      rc = attn_pages_scores_fn(tbl.ids, tbl.bytes, tbl.ld, (const int32_t*)at(6), at(1), ld, at(2), at(3), (const float*)at(4), (const float*)at(5), kind, o.data_ptr(),
+                                own[2].size(1), (int)B, (int)L, (int)H, Hkv, (int)HEAD, (int)ps, (int)window, (int)sinks, cap, (const float*)at(7),
+                                bytes ? ws.data_ptr() : nullptr, bytes, stream);
+    else
+      rc = attn_pages_fn(tbl.ids, tbl.bytes, tbl.ld, (const int32_t*)at(6), at(1), ld, at(2), at(3), (const float*)at(4), (const float*)at(5), kind, o.data_ptr(),
+                         own[2].size(1), (int)B, (int)L, (int)H, Hkv, (int)HEAD, (int)ps, (int)window, (int)sinks, bytes ? ws.data_ptr() : nullptr, bytes, stream);
   }
   if (rc != 0) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(o));
@@ -350,6 +392,236 @@ PyObject* causal_window(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// causal_scores(q, k, v, window, sinks, offset, softcap, slopes, documents, prefix, kernels._workspaces) -> o or None
+PyObject* causal_scores(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 11 || !causal_scores_fn) Py_RETURN_NONE;
+  bool fine = true;
+  const at::Tensor *q = tensor(args[0]), *k = tensor(args[1]), *v = tensor(args[2]), *docs = tensor_or_none(args[8], fine), *slopes;
+  int64_t window, sinks, offset, prefix = 0, ldq, ldk, ldv;
+  float cap;
+  const int dev = c10::cuda::current_device();
+  if (!fine || !whole(args[3], MOST, window) || !whole(args[4], -1, sinks) || !whole(args[5], -1, offset) || window < 1 || sinks < 0 || offset < 0 ||
+      !rows_of(q, dev, ldq) || !rows_of(k, dev, ldk) || !rows_of(v, dev, ldv) || !scores_of(args[6], args[7], dev, q->size(1), cap, slopes))
+    Py_RETURN_NONE;
+  const int64_t S = q->size(0), all = offset + S;
+  if (k->size(1) != v->size(1) || k->size(0) < all || v->size(0) < all || all > MOST) Py_RETURN_NONE;
+  if (docs && (offset || docs->dim() != 1 || docs->size(0) < 1 || docs->size(0) > MOST || !vector_of(docs, dev, at::kInt, docs->size(0)))) Py_RETURN_NONE;
+  const at::Tensor* prefixes = tensor(args[9]);
+  if (prefixes ? !docs || !vector_of(prefixes, dev, at::kInt, docs->size(0) - 1) : !whole(args[9], 0, prefix) || prefix < 0) Py_RETURN_NONE;
+  const auto stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+  PyObject* st = PyLong_FromVoidPtr(stream);
+  if (!st) return nullptr;
+  const at::Tensor page = workspace(args[10], dev, st);
+  Py_DECREF(st);
+  if (!page.defined()) Py_RETURN_NONE;
+  const int H = (int)q->size(1), Hkv = (int)k->size(1), w = (int)std::min(window, all), s = (int)std::min(sinks, all), n_docs = docs ? (int)docs->size(0) - 1 : 0;
+  const at::Tensor own[] = {held(q), held(k), held(v), held(slopes), held(docs), held(prefixes)};
+  at::Tensor o, ws;
+  int rc;
+  {
+    WithoutInterpreter without;
+    const size_t bytes = causal_scores_bytes((int)S, H, Hkv, (int)HEAD, (int)offset, w, s);
+    o = heads(S, H, dev);
+    ws = scratch(bytes, dev);
+    // (a prefix for each of no documents has no address, and none is looked up)
+    const auto at = [&](int i) { return own[i].defined() ? own[i].data_ptr() : nullptr; };
+    rc = causal_scores_fn(at(0), ldq, at(1), ldk, at(2), ldv, o.data_ptr(), H * HEAD, (int)S, H, Hkv, (int)HEAD, (int)offset, w, s, cap, (const float*)at(3),
+                          (const int32_t*)at(4), n_docs, (const int32_t*)at(5), (int)std::min(prefix, all), 0, bytes ? ws.data_ptr() : nullptr, bytes,
+                          (int*)((char*)page.data_ptr() + 4092), stream);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(o));
+  END_HANDLE_TH_ERRORS
+}
+
+// The books of a paged cache, where they lie as the library reads them
+struct Books {
+  at::Tensor table, lens, refs;
+  int64_t B, W, n, ld;
+};
+bool books_of(PyObject* const* args, int dev, Books& b) {
+  const at::Tensor *p = tensor(args[0]), *lens = tensor(args[1]), *refs = tensor(args[2]);
+  if (!is(p, dev, at::kInt) || p->dim() != 2 || p->size(0) < 1 || p->size(0) > INT32_MAX || p->size(1) < 1 || p->size(1) >= MOST_PAGE || (p->stride(1) != 1 && p->size(1) > 1) ||
+      !vector_of(lens, dev, at::kInt, p->size(0)) || !is(refs, dev, at::kInt) || refs->dim() != 1 || refs->size(0) < 1 || refs->size(0) > 1 << 28 || !refs->is_contiguous())
+    return false;
+  b = {*p, *lens, *refs, p->size(0), p->size(1), refs->size(0), p->size(0) > 1 ? p->stride(0) : p->size(1)};
+  return b.ld >= b.W;
+}
+// Books that are written in place must not overlap
+bool apart(const Books& b) {
+  const auto span = [](const at::Tensor& t, int64_t n) { return std::pair<const char*, const char*>((const char*)t.data_ptr(), (const char*)t.data_ptr() + 4 * n); };
+  const std::pair<const char*, const char*> x[] = {span(b.table, (b.B - 1) * b.ld + b.W), span(b.lens, b.B), span(b.refs, b.n)};
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < i; ++j)
+      if (x[i].first < x[j].second && x[j].first < x[i].second) return false;
+  return true;
+}
+// Pools [heads, P, 128], or of layers in front, and scales of those
+struct BooksPools {
+  at::Tensor k, v, ks, vs;
+  int kind;
+  int64_t heads, P;
+};
+bool books_pools_of(PyObject* const* args, int dev, const Books& b, int64_t ps, BooksPools& p) {
+  bool fine = true;
+  const at::Tensor *k = tensor(args[0]), *v = tensor(args[1]), *ks = tensor_or_none(args[2], fine), *vs = tensor_or_none(args[3], fine);
+  if (!fine || !k || !v || !on(*k, dev) || !on(*v, dev) || k->dim() < 3 || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() || !k->is_contiguous() ||
+      !v->is_contiguous() || k->size(-1) != HEAD || k->numel() == 0)
+    return false;
+  p.P = k->size(-2);
+  p.heads = k->numel() / (p.P * HEAD);
+  const auto type = k->scalar_type();
+  p.kind = type == at::kHalf ? 0 : type == at::kChar ? 1 : type == at::kFloat8_e4m3fn ? 2 : -1;
+  if (p.kind < 0 || p.P > INT32_MAX || p.heads > INT32_MAX || b.n * ps > p.P || (p.kind == 0 ? ks || vs : !ks || !vs || p.P % ps != 0)) return false;
+  for (const at::Tensor* s : {ks, vs})
+    if (s && (!is(s, dev, at::kFloat) || !s->is_contiguous() || s->dim() != k->dim() - 1 || s->size(-1) != p.P / ps || s->sizes().slice(0, s->dim() - 1) != k->sizes().slice(0, k->dim() - 2)))
+      return false;
+  p.k = *k, p.v = *v, p.ks = held(ks), p.vs = held(vs);
+  return true;
+}
+at::Tensor ints(at::IntArrayRef size, int dev) { return at::empty(size, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)dev)); }
+void written(const at::Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+// `out`: 0 None, 1 a tuple that begins with these objects, -1 something else
+int in_place(PyObject* out, std::initializer_list<PyObject*> books) {
+  if (out == Py_None) return 0;
+  if (!PyTuple_Check(out) || PyTuple_GET_SIZE(out) != 3) return -1;
+  Py_ssize_t i = 0;
+  for (PyObject* b : books)
+    if (PyTuple_GET_ITEM(out, i++) != b) return -1;
+  return 1;
+}
+PyObject* three(at::Tensor a, at::Tensor b, at::Tensor c) {
+  PyObject* r = PyTuple_New(3);
+  if (!r) return nullptr;
+  Py_ssize_t i = 0;
+  for (at::Tensor* t : {&a, &b, &c}) {
+    PyObject* x = THPVariable_Wrap(std::move(*t));
+    if (!x) {
+      Py_DECREF(r);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(r, i++, x);
+  }
+  return r;
+}
+int* int_ptr(const at::Tensor& t) { return (int*)t.data_ptr(); }
+float* float_ptr(const at::Tensor& t) { return t.defined() ? (float*)t.data_ptr() : nullptr; }
+
+// page_fork(p, lens, refs, parents, page_size, out) -> (p, lens, refs) or None
+PyObject* page_fork(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !page_fork_fn) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device(), place = in_place(args[5], {args[0], args[1], args[2]});
+  Books b;
+  int64_t ps;
+  const at::Tensor* parents = tensor(args[3]);
+  if (place < 0 || !books_of(args, dev, b) || !vector_of(parents, dev, at::kInt, b.B) || !whole(args[4], -1, ps) || ps < 1 || ps > MOST_PAGE) Py_RETURN_NONE;
+  if (place && !apart(b)) Py_RETURN_NONE;
+  const auto stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+  const at::Tensor from = *parents;
+  at::Tensor table, lens, refs, old_table, old_lens;
+  int rc;
+  {
+    WithoutInterpreter without;
+    table = place ? b.table : ints({b.B, b.W}, dev);
+    lens = place ? b.lens : ints({b.B}, dev);
+    refs = place ? b.refs : ints({b.n}, dev);
+    old_table = place ? b.table.clone() : b.table;       // sequences read each other's rows
+    old_lens = place ? b.lens.clone() : b.lens;
+    rc = page_fork_fn(int_ptr(old_table), b.B > 1 ? old_table.stride(0) : b.W, int_ptr(old_lens), int_ptr(b.refs), int_ptr(from), int_ptr(table), b.B > 1 ? table.stride(0) : b.W,
+                      int_ptr(lens), int_ptr(refs), (int)b.B, (int)b.W, (int)b.n, (int)ps, stream);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  if (place)
+    for (const at::Tensor* t : {&table, &lens, &refs}) written(*t);
+  return three(table, lens, refs);
+  END_HANDLE_TH_ERRORS
+}
+
+// page_extend(p, lens, refs, kpool, vpool, k_scale, v_scale, add, page_size, out) -> (p, lens, refs) or None
+PyObject* page_extend(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10 || !page_extend_fn) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device(), place = in_place(args[9], {args[0], args[1], args[2]});
+  Books b;
+  BooksPools p;
+  int64_t ps;
+  const at::Tensor* add = tensor(args[7]);
+  if (place < 0 || !books_of(args, dev, b) || b.B > 16384 || !vector_of(add, dev, at::kInt, b.B) || !whole(args[8], -1, ps) || ps < 1 || ps > MOST_PAGE ||
+      !books_pools_of(args + 3, dev, b, ps, p))
+    Py_RETURN_NONE;
+  if (place && !apart(b)) Py_RETURN_NONE;
+  const auto stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+  const at::Tensor more = *add;
+  at::Tensor table, lens, refs, ws;
+  int rc;
+  {
+    WithoutInterpreter without;
+    table = place ? b.table : ints({b.B, b.W}, dev);
+    lens = place ? b.lens : ints({b.B}, dev);
+    refs = place ? b.refs : ints({b.n}, dev);
+    const size_t bytes = page_extend_bytes((int)b.B, (int)b.n);
+    ws = scratch(bytes, dev);
+    rc = page_extend_fn(int_ptr(b.table), b.ld, int_ptr(b.lens), int_ptr(b.refs), int_ptr(more), int_ptr(table), place ? b.ld : b.W, int_ptr(lens), int_ptr(refs), (int)b.B,
+                        (int)b.W, (int)b.n, (int)ps, p.k.data_ptr(), p.v.data_ptr(), float_ptr(p.ks), float_ptr(p.vs), p.kind, p.P, (int)p.heads, ws.data_ptr(), bytes, stream);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  for (const at::Tensor* t : {&p.k, &p.v, &p.ks, &p.vs}) written(*t);
+  if (place)
+    for (const at::Tensor* t : {&table, &lens, &refs}) written(*t);
+  return three(table, lens, refs);
+  END_HANDLE_TH_ERRORS
+}
+
+// page_compact(p, lens, refs, kpool, vpool, k_scale, v_scale, page_size, out) -> (p, refs, where) or None
+PyObject* page_compact(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || !page_compact_fn) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  if (args[8] != Py_None) Py_RETURN_NONE;
+  Books b;
+  BooksPools p;
+  int64_t ps;
+  if (!books_of(args, dev, b) || !whole(args[7], -1, ps) || ps < 1 || ps > MOST_PAGE || !books_pools_of(args + 3, dev, b, ps, p)) Py_RETURN_NONE;
+  const auto stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+  at::Tensor table, refs, where, ws;
+  int rc;
+  {
+    WithoutInterpreter without;
+    table = ints({b.B, b.W}, dev);
+    refs = ints({b.n}, dev);
+    where = ints({b.n}, dev);
+    const size_t bytes = page_compact_bytes((int)b.n);
+    ws = scratch(bytes, dev);
+    rc = page_compact_fn(int_ptr(b.table), b.ld, int_ptr(b.lens), int_ptr(b.refs), int_ptr(table), b.W, int_ptr(refs), int_ptr(where), (int)b.B, (int)b.W, (int)b.n, (int)ps,
+                         p.k.data_ptr(), p.v.data_ptr(), float_ptr(p.ks), float_ptr(p.vs), p.kind, p.P, (int)p.heads, ws.data_ptr(), bytes, stream);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  for (const at::Tensor* t : {&p.k, &p.v, &p.ks, &p.vs}) written(*t);
+  return three(table, refs, where);
+  END_HANDLE_TH_ERRORS
+}
+
+// init_books(addresses of q40_attn_pages_scores, q40_attn_causal_scores, _workspace_bytes, q40_page_fork, q40_page_extend, _workspace_bytes, q40_page_compact,
+// _workspace_bytes)
+PyObject* init_books(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n == 8) {
+    attn_pages_scores_fn = (AttnPagesScores)PyLong_AsVoidPtr(args[0]);
+    causal_scores_fn = (CausalScores)PyLong_AsVoidPtr(args[1]);
+    causal_scores_bytes = (CausalWindowBytes)PyLong_AsVoidPtr(args[2]);
+    page_fork_fn = (PageFork)PyLong_AsVoidPtr(args[3]);
+    page_extend_fn = (PageExtend)PyLong_AsVoidPtr(args[4]);
+    page_extend_bytes = (size_t (*)(int, int))PyLong_AsVoidPtr(args[5]);
+    page_compact_fn = (PageCompact)PyLong_AsVoidPtr(args[6]);
+    page_compact_bytes = (size_t (*)(int))PyLong_AsVoidPtr(args[7]);
+  }
+  if (PyErr_Occurred()) return nullptr;
+  Py_RETURN_NONE;
+}
+
 // init_pages(addresses of q40_attn_pages, _workspace_bytes, q40_page_append, q40_attn_causal_window, _workspace_bytes)
 PyObject* init_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n == 5) {
@@ -378,6 +650,11 @@ PyMethodDef methods[] = {{"matmul", (PyCFunction)(void*)matmul, METH_FASTCALL, n
                          {"attn_pages", (PyCFunction)(void*)attn_pages, METH_FASTCALL, nullptr},
                          {"page_append", (PyCFunction)(void*)page_append, METH_FASTCALL, nullptr},
                          {"causal_window", (PyCFunction)(void*)causal_window, METH_FASTCALL, nullptr},
+                         {"causal_scores", (PyCFunction)(void*)causal_scores, METH_FASTCALL, nullptr},
+                         {"page_fork", (PyCFunction)(void*)page_fork, METH_FASTCALL, nullptr},
+                         {"page_extend", (PyCFunction)(void*)page_extend, METH_FASTCALL, nullptr},
+                         {"page_compact", (PyCFunction)(void*)page_compact, METH_FASTCALL, nullptr},
+                         {"init_books", (PyCFunction)(void*)init_books, METH_FASTCALL, nullptr},
                          {"init_pages", (PyCFunction)(void*)init_pages, METH_FASTCALL, nullptr},
                          {"init", (PyCFunction)(void*)init, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

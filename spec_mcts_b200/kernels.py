@@ -33,6 +33,8 @@ def _load_host_calls():
     m.init(*[address(f) for f in (lib.q40_matmul_tiled, lib.q40_gemm_nk)])
     m.init_pages(*[address(f) for f in (lib.q40_attn_pages, lib.q40_attn_pages_workspace_bytes, lib.q40_page_append, lib.q40_attn_causal_window,
                                         lib.q40_attn_causal_window_workspace_bytes)])
+    m.init_books(*[address(f) for f in (lib.q40_attn_pages_scores, lib.q40_attn_causal_scores, lib.q40_attn_causal_scores_workspace_bytes, lib.q40_page_fork,
+                                        lib.q40_page_extend, lib.q40_page_extend_workspace_bytes, lib.q40_page_compact, lib.q40_page_compact_workspace_bytes)])
     return m
 
 
@@ -634,6 +636,11 @@ def causal_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional
 SOFTCAP = (0.01, 1000.0)             # Q40_SOFTCAP_LEAST, Q40_SOFTCAP_MOST
 
 
+def _plain_cap(softcap):
+    """A cap as the native calls take it: a float, or something else for them to hand back."""
+    return float(softcap) if type(softcap) is int else softcap
+
+
 def _scores_of(what: str, heads: int, softcap, slopes):
     """Cap (0: none) and slopes (fp32, or None) as the library takes them."""
     if softcap is not None and not SOFTCAP[0] <= softcap <= SOFTCAP[1]:
@@ -647,6 +654,10 @@ def _scores_of(what: str, heads: int, softcap, slopes):
 
 def _causal_scores(q, k, v, out, window, sinks, offset, softcap, slopes, documents, prefix):
     own = prefix if isinstance(prefix, torch.Tensor) else None       # of each document
+    if out is None and _host_calls is not None:
+        o = _host_calls.causal_scores(q, k, v, window, sinks, offset, _plain_cap(softcap), slopes, documents, prefix, _workspaces)      # None: not a plain call
+        if o is not None:
+            return o
     dev = _need_cuda(q, k, v, out, slopes, documents, own)
     for t in (q, k, v):
         if t.dtype != torch.float16 or t.dim() != 3 or t.shape[2] != 128 or t.stride(2) != 1 or (t.stride(1) != 128 and t.shape[1] > 1):
@@ -830,8 +841,8 @@ def page_flash_attn(p, q, k, v, P, B, L, H, D, *, page_size: int = 1, seq_lens=N
     last position, attends that many last keys and the first `sinks` alone.  With `softcap` c (0.01 to 1000) scores x become c tanh(x / c); with `slopes` [H] they
     then fall by slopes[h] for each position between key and query (q40_attn_pages_scores in include/q40b200.h)."""
     windowed = window is not None or sinks != 0 or softcap is not None or slopes is not None
-    if windowed and softcap is None and slopes is None and D == 128 and _host_calls is not None and q.shape == (B, H, D) and k.dtype == torch.float16 and k.shape[1:] == (P, D):
-        o = _host_calls.attn_pages(p, q, k, v, None, None, L, page_size, seq_lens, window, sinks)      # None: not a plain call
+    if windowed and D == 128 and _host_calls is not None and q.shape == (B, H, D) and k.dtype == torch.float16 and k.shape[1:] == (P, D):
+        o = _host_calls.attn_pages(p, q, k, v, None, None, L, page_size, seq_lens, window, sinks, _plain_cap(softcap), slopes)      # None: not a plain call
         if o is not None:
             return o
     dev = _need_cuda(p, q, k, v, seq_lens, slopes)
@@ -937,8 +948,8 @@ def page_flash_attn_q8(p, q, k, v, k_scale, v_scale, *, page_size: int, seq_lens
     one query for each sequence, its last position; p [B, pages] lists page ids, seq_lens [B] the lengths (None: the table's whole width).
     With `window` a query attends that many last keys and the first `sinks` alone (q40_attn_pages in include/q40b200.h).  `softcap` and `slopes` as in
     page_flash_attn."""
-    if _host_calls is not None and softcap is None and slopes is None and k.dtype != torch.float16:
-        o = _host_calls.attn_pages(p, q, k, v, k_scale, v_scale, p.shape[-1] * page_size, page_size, seq_lens, window, sinks)      # None: not a plain call
+    if _host_calls is not None and k.dtype != torch.float16:
+        o = _host_calls.attn_pages(p, q, k, v, k_scale, v_scale, p.shape[-1] * page_size, page_size, seq_lens, window, sinks, _plain_cap(softcap), slopes)      # None: not a plain call
         if o is not None:
             return o
     dev = _need_cuda(p, q, k, v, k_scale, v_scale, seq_lens, slopes)
@@ -1066,6 +1077,10 @@ def page_fork(p, lens, refs, parents, *, page_size: int, out=None):
     sequences list each page (0: it is free); all int32.  Returns them as they are afterwards (zeros behind a sequence's pages), in new tensors or in
     out = (p, lens, refs), which may be the books themselves.  page_extend gives sequences that share a page their own before they write to it
     (q40_page_fork in include/q40b200.h)."""
+    if _host_calls is not None:
+        new = _host_calls.page_fork(p, lens, refs, parents, page_size, out)      # None: not a plain call
+        if new is not None:
+            return new
     dev = _need_cuda(p, lens, refs, parents, *(out or ()))
     p, lens, refs, new = _books("page_fork", p, lens, refs, page_size, out, (p, lens, refs))
     B, W = p.shape
@@ -1088,6 +1103,10 @@ def page_extend(p, lens, refs, kpool, vpool, add, *, page_size: int, k_scale=Non
     its rows in the pools [.., Hkv, P, 128] (of several layers at once, in front of the heads; scales [.., Hkv, P / page_size] of 8-bit ones alike), in place.  Free pages are
     handed out in ascending order; a sequence that its row of the table or the free pages have no room for keeps its length, and so does every one behind the latter that needs a
     page.  Books and `out` as in page_fork; up to 16384 sequences (q40_page_extend in include/q40b200.h)."""
+    if _host_calls is not None:
+        new = _host_calls.page_extend(p, lens, refs, kpool, vpool, k_scale, v_scale, add, page_size, out)      # None: not a plain call
+        if new is not None:
+            return new
     dev = _need_cuda(p, lens, refs, kpool, vpool, add, k_scale, v_scale, *(out or ()))
     k, v, ks, vs, kind = _books_pools("page_extend", kpool, vpool, k_scale, v_scale, refs, page_size)
     p, lens, refs, new = _books("page_extend", p, lens, refs, page_size, out, (p, lens, refs))
@@ -1108,6 +1127,10 @@ def page_compact(p, lens, refs, kpool, vpool, *, page_size: int, k_scale=None, v
     """Pages in use become the first ones of their pools (in place; pools and scales as in page_extend): with n of them, those from n on move, in order, to the free ones
     below.  Returns the table and the references as they are afterwards, and where [pages of the pool], the new id of each page (-1: it was free), in new tensors or in
     out = (p, refs, where), of which the first two may be the books themselves (q40_page_compact in include/q40b200.h)."""
+    if _host_calls is not None:
+        new = _host_calls.page_compact(p, lens, refs, kpool, vpool, k_scale, v_scale, page_size, out)      # None: not a plain call
+        if new is not None:
+            return new
     dev = _need_cuda(p, lens, refs, kpool, vpool, k_scale, v_scale, *(out or ()))
     k, v, ks, vs, kind = _books_pools("page_compact", kpool, vpool, k_scale, v_scale, refs, page_size)
     p, lens, refs, new = _books("page_compact", p, lens, refs, page_size, out, (p, refs, refs))
