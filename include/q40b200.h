@@ -328,30 +328,31 @@ int q40_attn_pages_scores(const void* page_tbl, int idx_bytes, int64_t tbl_strid
 
 /* The books of a paged cache, in device memory: a table of page ids [B, W] int32 (rows of ld entries), lengths lens [B], and refs [n_pages], how many sequences list
  * each page (0 or below: it is free).  A sequence's pages are the first ceil(length / page_size) entries of its row.  Each call writes the books as they are afterwards
- * to *_out, with 0 behind a row's pages; but for the exceptions named the outputs may be the inputs (the same addresses and strides), and must not overlap them
- * otherwise.  Lengths outside of 0 .. W * page_size count as the nearest of these, ids outside of the pool as no page's.  W < 2^29, n_pages <= 2^28.
+ * to *_out, with 0 behind a row's pages; the outputs may be the inputs (the same addresses and strides), and must not overlap them otherwise.  Lengths outside of 0 .. W * page_size count as the nearest of these, ids outside of the pool as no page's.  W < 2^29, n_pages <= 2^28.
  * Results do not depend on the order in which threads come.  Books that do not fit each other make them undefined, and nothing else.
  *
  * Sequence b becomes what sequence parents[b] was, whose pages it lists from then on, or one of length 0, if that is outside of 0 .. B - 1; refs count what is
- * listed anew, and no longer.  Table and lengths must not be written in place (Q40_E_UNSUPPORTED).  No counterpart in the reference beyond the fork of
- * hf_model_q40_kv_shared.py:282-297, which copies. */
+ * listed anew, and no longer.  Workspace (4-byte aligned, no initialisation; calls that may overlap need one each) for calls in place alone, which copy table and
+ * lengths to it where they are large (0 bytes: may be NULL).  No counterpart in the reference beyond the fork of hf_model_q40_kv_shared.py:282-297, which copies. */
+size_t q40_page_fork_workspace_bytes(int B, int W, int n_pages);
 int q40_page_fork(const int32_t* table, int64_t ld, const int32_t* lens, const int32_t* refs, const int32_t* parents, int32_t* table_out, int64_t ld_out,
-                  int32_t* lens_out, int32_t* refs_out, int B, int W, int n_pages, int page_size, void* stream);
+                  int32_t* lens_out, int32_t* refs_out, int B, int W, int n_pages, int page_size, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Sequence b gets add[b] tokens more, up to 16384 sequences.  Below 0: so many of its last ones less (down to none); pages that hold none of the others are given
  * back.  Above 0: pages for them, and a page of its own in the place of its last one, if that has room and other sequences list it (of sequences that all get tokens
  * and share a page which no other lists, the last keeps it): a copy of its rows so far, and its scales, in all `heads` of the pools [heads, P, 128] (P >= n_pages *
  * page_size, cache_type and scales as in q40_attn_pages; `heads` may be those of several layers).  Pages that are free before the call are handed out in ascending
  * order, to the sequences in theirs (a copy first).  A sequence whose pages do not fit in W, or whose last page is none of the pool's, stays as it is; so does the first that wants more pages than are left,
- * and every one behind it that wants any.  Workspace: 16-byte aligned, no initialisation; calls that may overlap need one each. */
-size_t q40_page_extend_workspace_bytes(int B, int n_pages);
+ * and every one behind it that wants any.  Workspace: *_workspace_bytes bytes (in_place: one of the outputs is an input; 0 bytes: may be NULL), 16-byte aligned, no
+ * initialisation; calls that may overlap need one each. */
+size_t q40_page_extend_workspace_bytes(int B, int n_pages, int in_place);
 int q40_page_extend(const int32_t* table, int64_t ld, const int32_t* lens, const int32_t* refs, const int32_t* add, int32_t* table_out, int64_t ld_out,
                     int32_t* lens_out, int32_t* refs_out, int B, int W, int n_pages, int page_size, void* kpool, void* vpool, float* k_scale,
                     float* v_scale, int cache_type, int64_t P, int heads, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Moves pages in use so that they are the first of their pools: with n of them in use, those from n on go, in order, to the free ones below.  where [n_pages] tells
- * each page's new id (-1: it was free). */
-size_t q40_page_compact_workspace_bytes(int n_pages);
+ * each page's new id (-1: it was free).  Workspace as in q40_page_extend. */
+size_t q40_page_compact_workspace_bytes(int n_pages, int in_place);
 int q40_page_compact(const int32_t* table, int64_t ld, const int32_t* lens, const int32_t* refs, int32_t* table_out, int64_t ld_out, int32_t* refs_out,
                      int32_t* where, int B, int W, int n_pages, int page_size, void* kpool, void* vpool, float* k_scale, float* v_scale, int cache_type,
                      int64_t P, int heads, void* workspace, size_t workspace_bytes, void* stream);

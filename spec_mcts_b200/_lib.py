@@ -108,11 +108,12 @@ SIGNATURES = {
                        [c_int] * 8 + [c_void_p, c_size_t, c_void_p]),
     "q40_attn_pages_scores": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64] + [c_void_p] * 4 + [c_int, c_void_p, c_int64] +
                               [c_int] * 8 + [c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
-    "q40_page_fork": (c_int, [c_void_p, c_int64] + [c_void_p] * 4 + [c_int64, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p]),
-    "q40_page_extend_workspace_bytes": (c_size_t, [c_int] * 2),
+    "q40_page_fork_workspace_bytes": (c_size_t, [c_int] * 3),
+    "q40_page_fork": (c_int, [c_void_p, c_int64] + [c_void_p] * 4 + [c_int64, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p, c_size_t, c_void_p]),
+    "q40_page_extend_workspace_bytes": (c_size_t, [c_int] * 3),
     "q40_page_extend": (c_int, [c_void_p, c_int64] + [c_void_p] * 4 + [c_int64, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 4 +
                         [c_int, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
-    "q40_page_compact_workspace_bytes": (c_size_t, [c_int]),
+    "q40_page_compact_workspace_bytes": (c_size_t, [c_int] * 2),
     "q40_page_compact": (c_int, [c_void_p, c_int64] + [c_void_p] * 3 + [c_int64, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 4 +
                          [c_int, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
     "q40_page_append": (c_int, [c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,

@@ -11,12 +11,10 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <ATen/ops/clone.h>
 #include <ATen/ops/empty.h>
 
 #include <algorithm>
 #include <initializer_list>
-#include <utility>
 
 namespace {
 
@@ -165,7 +163,8 @@ using AttnPagesScores = int (*)(const void*, int, int64_t, const int32_t*, const
                                 int64_t, int, int, int, int, int, int, int, int, float, const float*, void*, size_t, void*);
 using CausalScores = int (*)(const void*, int64_t, const void*, int64_t, const void*, int64_t, void*, int64_t, int, int, int, int, int, int, int, float, const float*,
                              const int32_t*, int, const int32_t*, int, int, void*, size_t, int*, void*);
-using PageFork = int (*)(const int32_t*, int64_t, const int32_t*, const int32_t*, const int32_t*, int32_t*, int64_t, int32_t*, int32_t*, int, int, int, int, void*);
+using PageFork = int (*)(const int32_t*, int64_t, const int32_t*, const int32_t*, const int32_t*, int32_t*, int64_t, int32_t*, int32_t*, int, int, int, int, void*,
+                         size_t, void*);
 using PageExtend = int (*)(const int32_t*, int64_t, const int32_t*, const int32_t*, const int32_t*, int32_t*, int64_t, int32_t*, int32_t*, int, int, int, int, void*, void*, float*,
                            float*, int, int64_t, int, void*, size_t, void*);
 using PageCompact = int (*)(const int32_t*, int64_t, const int32_t*, const int32_t*, int32_t*, int64_t, int32_t*, int32_t*, int, int, int, int, void*, void*, float*, float*, int,
@@ -176,8 +175,9 @@ CausalWindowBytes causal_scores_bytes = nullptr;
 PageFork page_fork_fn = nullptr;
 PageExtend page_extend_fn = nullptr;
 PageCompact page_compact_fn = nullptr;
-size_t (*page_extend_bytes)(int, int) = nullptr;
-size_t (*page_compact_bytes)(int) = nullptr;
+size_t (*page_fork_bytes)(int, int, int) = nullptr;
+size_t (*page_extend_bytes)(int, int, int) = nullptr;
+size_t (*page_compact_bytes)(int, int) = nullptr;
 AttnPages attn_pages_fn = nullptr;
 AttnPagesBytes attn_pages_bytes = nullptr;
 PageAppend page_append_fn = nullptr;
@@ -448,13 +448,14 @@ bool books_of(PyObject* const* args, int dev, Books& b) {
   b = {*p, *lens, *refs, p->size(0), p->size(1), refs->size(0), p->size(0) > 1 ? p->stride(0) : p->size(1)};
   return b.ld >= b.W;
 }
-// Books that are written in place must not overlap
-bool apart(const Books& b) {
-  const auto span = [](const at::Tensor& t, int64_t n) { return std::pair<const char*, const char*>((const char*)t.data_ptr(), (const char*)t.data_ptr() + 4 * n); };
-  const std::pair<const char*, const char*> x[] = {span(b.table, (b.B - 1) * b.ld + b.W), span(b.lens, b.B), span(b.refs, b.n)};
-  for (int i = 0; i < 3; ++i)
+// Books that are written in place must not overlap, nor `more` them
+bool apart(const Books& b, const at::Tensor* more = nullptr) {
+  struct Span { const char *from, *to; };
+  const auto span = [](const at::Tensor& t, int64_t n) { return Span{(const char*)t.data_ptr(), (const char*)t.data_ptr() + 4 * n}; };
+  const Span x[] = {span(b.table, (b.B - 1) * b.ld + b.W), span(b.lens, b.B), span(b.refs, b.n), more ? span(*more, more->numel()) : Span{}};
+  for (int i = 0; i < 4; ++i)
     for (int j = 0; j < i; ++j)
-      if (x[i].first < x[j].second && x[j].first < x[i].second) return false;
+      if (x[i].from < x[j].to && x[j].from < x[i].to) return false;
   return true;
 }
 // Pools [heads, P, 128], or of layers in front, and scales of those
@@ -522,17 +523,17 @@ PyObject* page_fork(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (place && !apart(b)) Py_RETURN_NONE;
   const auto stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
   const at::Tensor from = *parents;
-  at::Tensor table, lens, refs, old_table, old_lens;
+  at::Tensor table, lens, refs, ws;
   int rc;
   {
     WithoutInterpreter without;
     table = place ? b.table : ints({b.B, b.W}, dev);
     lens = place ? b.lens : ints({b.B}, dev);
     refs = place ? b.refs : ints({b.n}, dev);
-    old_table = place ? b.table.clone() : b.table;       // sequences read each other's rows
-    old_lens = place ? b.lens.clone() : b.lens;
-    rc = page_fork_fn(int_ptr(old_table), b.B > 1 ? old_table.stride(0) : b.W, int_ptr(old_lens), int_ptr(b.refs), int_ptr(from), int_ptr(table), b.B > 1 ? table.stride(0) : b.W,
-                      int_ptr(lens), int_ptr(refs), (int)b.B, (int)b.W, (int)b.n, (int)ps, stream);
+    const size_t bytes = place ? page_fork_bytes((int)b.B, (int)b.W, (int)b.n) : 0;
+    ws = scratch(bytes, dev);
+    rc = page_fork_fn(int_ptr(b.table), b.ld, int_ptr(b.lens), int_ptr(b.refs), int_ptr(from), int_ptr(table), place ? b.ld : b.W, int_ptr(lens), int_ptr(refs), (int)b.B,
+                      (int)b.W, (int)b.n, (int)ps, bytes ? ws.data_ptr() : nullptr, bytes, stream);
   }
   if (rc != 0) Py_RETURN_NONE;
   if (place)
@@ -563,10 +564,10 @@ PyObject* page_extend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     table = place ? b.table : ints({b.B, b.W}, dev);
     lens = place ? b.lens : ints({b.B}, dev);
     refs = place ? b.refs : ints({b.n}, dev);
-    const size_t bytes = page_extend_bytes((int)b.B, (int)b.n);
+    const size_t bytes = page_extend_bytes((int)b.B, (int)b.n, place);
     ws = scratch(bytes, dev);
     rc = page_extend_fn(int_ptr(b.table), b.ld, int_ptr(b.lens), int_ptr(b.refs), int_ptr(more), int_ptr(table), place ? b.ld : b.W, int_ptr(lens), int_ptr(refs), (int)b.B,
-                        (int)b.W, (int)b.n, (int)ps, p.k.data_ptr(), p.v.data_ptr(), float_ptr(p.ks), float_ptr(p.vs), p.kind, p.P, (int)p.heads, ws.data_ptr(), bytes, stream);
+                        (int)b.W, (int)b.n, (int)ps, p.k.data_ptr(), p.v.data_ptr(), float_ptr(p.ks), float_ptr(p.vs), p.kind, p.P, (int)p.heads, bytes ? ws.data_ptr() : nullptr, bytes, stream);
   }
   if (rc != 0) Py_RETURN_NONE;
   for (const at::Tensor* t : {&p.k, &p.v, &p.ks, &p.vs}) written(*t);
@@ -580,43 +581,47 @@ PyObject* page_extend(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* page_compact(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 9 || !page_compact_fn) Py_RETURN_NONE;
-  const int dev = c10::cuda::current_device();
-  if (args[8] != Py_None) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device(), place = in_place(args[8], {args[0], args[2]});
   Books b;
   BooksPools p;
   int64_t ps;
-  if (!books_of(args, dev, b) || !whole(args[7], -1, ps) || ps < 1 || ps > MOST_PAGE || !books_pools_of(args + 3, dev, b, ps, p)) Py_RETURN_NONE;
+  if (place < 0 || !books_of(args, dev, b) || !whole(args[7], -1, ps) || ps < 1 || ps > MOST_PAGE || !books_pools_of(args + 3, dev, b, ps, p)) Py_RETURN_NONE;
   const auto stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
-  at::Tensor table, refs, where, ws;
+  const at::Tensor* given = place ? tensor(PyTuple_GET_ITEM(args[8], 2)) : nullptr;
+  if (place && (!vector_of(given, dev, at::kInt, b.n) || !apart(b, given))) Py_RETURN_NONE;
+  at::Tensor table, refs, where = held(given), ws;
   int rc;
   {
     WithoutInterpreter without;
-    table = ints({b.B, b.W}, dev);
-    refs = ints({b.n}, dev);
-    where = ints({b.n}, dev);
-    const size_t bytes = page_compact_bytes((int)b.n);
+    table = place ? b.table : ints({b.B, b.W}, dev);
+    refs = place ? b.refs : ints({b.n}, dev);
+    if (!place) where = ints({b.n}, dev);
+    const size_t bytes = page_compact_bytes((int)b.n, place);
     ws = scratch(bytes, dev);
-    rc = page_compact_fn(int_ptr(b.table), b.ld, int_ptr(b.lens), int_ptr(b.refs), int_ptr(table), b.W, int_ptr(refs), int_ptr(where), (int)b.B, (int)b.W, (int)b.n, (int)ps,
-                         p.k.data_ptr(), p.v.data_ptr(), float_ptr(p.ks), float_ptr(p.vs), p.kind, p.P, (int)p.heads, ws.data_ptr(), bytes, stream);
+    rc = page_compact_fn(int_ptr(b.table), b.ld, int_ptr(b.lens), int_ptr(b.refs), int_ptr(table), place ? b.ld : b.W, int_ptr(refs), int_ptr(where), (int)b.B, (int)b.W, (int)b.n, (int)ps,
+                         p.k.data_ptr(), p.v.data_ptr(), float_ptr(p.ks), float_ptr(p.vs), p.kind, p.P, (int)p.heads, bytes ? ws.data_ptr() : nullptr, bytes, stream);
   }
   if (rc != 0) Py_RETURN_NONE;
   for (const at::Tensor* t : {&p.k, &p.v, &p.ks, &p.vs}) written(*t);
+  if (place)
+    for (const at::Tensor* t : {&table, &refs, &where}) written(*t);
   return three(table, refs, where);
   END_HANDLE_TH_ERRORS
 }
 
-// init_books(addresses of q40_attn_pages_scores, q40_attn_causal_scores, _workspace_bytes, q40_page_fork, q40_page_extend, _workspace_bytes, q40_page_compact,
-// _workspace_bytes)
+// init_books(addresses of q40_attn_pages_scores, q40_attn_causal_scores, _workspace_bytes, q40_page_fork, _workspace_bytes, q40_page_extend, _workspace_bytes,
+// q40_page_compact, _workspace_bytes)
 PyObject* init_books(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n == 8) {
+  if (n == 9) {
     attn_pages_scores_fn = (AttnPagesScores)PyLong_AsVoidPtr(args[0]);
     causal_scores_fn = (CausalScores)PyLong_AsVoidPtr(args[1]);
     causal_scores_bytes = (CausalWindowBytes)PyLong_AsVoidPtr(args[2]);
     page_fork_fn = (PageFork)PyLong_AsVoidPtr(args[3]);
-    page_extend_fn = (PageExtend)PyLong_AsVoidPtr(args[4]);
-    page_extend_bytes = (size_t (*)(int, int))PyLong_AsVoidPtr(args[5]);
-    page_compact_fn = (PageCompact)PyLong_AsVoidPtr(args[6]);
-    page_compact_bytes = (size_t (*)(int))PyLong_AsVoidPtr(args[7]);
+    page_fork_bytes = (size_t (*)(int, int, int))PyLong_AsVoidPtr(args[4]);
+    page_extend_fn = (PageExtend)PyLong_AsVoidPtr(args[5]);
+    page_extend_bytes = (size_t (*)(int, int, int))PyLong_AsVoidPtr(args[6]);
+    page_compact_fn = (PageCompact)PyLong_AsVoidPtr(args[7]);
+    page_compact_bytes = (size_t (*)(int, int))PyLong_AsVoidPtr(args[8]);
   }
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;

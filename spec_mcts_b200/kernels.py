@@ -33,7 +33,7 @@ def _load_host_calls():
     m.init(*[address(f) for f in (lib.q40_matmul_tiled, lib.q40_gemm_nk)])
     m.init_pages(*[address(f) for f in (lib.q40_attn_pages, lib.q40_attn_pages_workspace_bytes, lib.q40_page_append, lib.q40_attn_causal_window,
                                         lib.q40_attn_causal_window_workspace_bytes)])
-    m.init_books(*[address(f) for f in (lib.q40_attn_pages_scores, lib.q40_attn_causal_scores, lib.q40_attn_causal_scores_workspace_bytes, lib.q40_page_fork,
+    m.init_books(*[address(f) for f in (lib.q40_attn_pages_scores, lib.q40_attn_causal_scores, lib.q40_attn_causal_scores_workspace_bytes, lib.q40_page_fork, lib.q40_page_fork_workspace_bytes,
                                         lib.q40_page_extend, lib.q40_page_extend_workspace_bytes, lib.q40_page_compact, lib.q40_page_compact_workspace_bytes)])
     return m
 
@@ -1087,11 +1087,10 @@ def page_fork(p, lens, refs, parents, *, page_size: int, out=None):
     if parents.shape != (B,) or parents.is_floating_point():
         raise Q40Error(f"page_fork: {B} parents expected, got {tuple(parents.shape)} of {parents.dtype}")
     parents = parents.to(torch.int32).contiguous()
-    if out is not None:                           # sequences read each other's rows
-        p = p.clone() if p.data_ptr() == new[0].data_ptr() else p
-        lens = lens.clone() if lens.data_ptr() == new[1].data_ptr() else lens
+    nbytes = lib.q40_page_fork_workspace_bytes(B, W, refs.shape[0]) if out is not None else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None           # of this call alone, as in _attn_pages
     check(lib.q40_page_fork(p.data_ptr(), _table_stride(p), lens.data_ptr(), refs.data_ptr(), parents.data_ptr(), new[0].data_ptr(), _table_stride(new[0]),
-                            new[1].data_ptr(), new[2].data_ptr(), B, W, refs.shape[0], page_size, _stream(dev)), "page_fork")
+                            new[1].data_ptr(), new[2].data_ptr(), B, W, refs.shape[0], page_size, _ptr(ws), nbytes, _stream(dev)), "page_fork")
     if out is not None:
         _counted(*new)
     return tuple(new)
@@ -1114,10 +1113,10 @@ def page_extend(p, lens, refs, kpool, vpool, add, *, page_size: int, k_scale=Non
     if add.shape != (B,) or add.is_floating_point() or B > 16384:
         raise Q40Error(f"page_extend: numbers of tokens for {B} sequences (at most 16384) expected, got {tuple(add.shape)} of {add.dtype}")
     add = add.to(torch.int32).contiguous()
-    nbytes = lib.q40_page_extend_workspace_bytes(B, refs.shape[0])
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)        # of this call alone, as in _attn_pages
+    nbytes = lib.q40_page_extend_workspace_bytes(B, refs.shape[0], out is not None)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None           # of this call alone, as in _attn_pages
     check(lib.q40_page_extend(p.data_ptr(), _table_stride(p), lens.data_ptr(), refs.data_ptr(), add.data_ptr(), new[0].data_ptr(), _table_stride(new[0]), new[1].data_ptr(),
-                              new[2].data_ptr(), B, W, refs.shape[0], page_size, k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), kind, k.shape[1], k.shape[0], ws.data_ptr(),
+                              new[2].data_ptr(), B, W, refs.shape[0], page_size, k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), kind, k.shape[1], k.shape[0], _ptr(ws),
                               nbytes, _stream(dev)), "page_extend")
     _counted(kpool, vpool, k_scale, v_scale, *(out or ()))
     return tuple(new)
@@ -1134,11 +1133,11 @@ def page_compact(p, lens, refs, kpool, vpool, *, page_size: int, k_scale=None, v
     dev = _need_cuda(p, lens, refs, kpool, vpool, k_scale, v_scale, *(out or ()))
     k, v, ks, vs, kind = _books_pools("page_compact", kpool, vpool, k_scale, v_scale, refs, page_size)
     p, lens, refs, new = _books("page_compact", p, lens, refs, page_size, out, (p, refs, refs))
-    nbytes = lib.q40_page_compact_workspace_bytes(refs.shape[0])
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    nbytes = lib.q40_page_compact_workspace_bytes(refs.shape[0], out is not None)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     check(lib.q40_page_compact(p.data_ptr(), _table_stride(p), lens.data_ptr(), refs.data_ptr(), new[0].data_ptr(), _table_stride(new[0]), new[1].data_ptr(),
                                new[2].data_ptr(), p.shape[0], p.shape[1], refs.shape[0], page_size, k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), kind, k.shape[1],
-                               k.shape[0], ws.data_ptr(), nbytes, _stream(dev)), "page_compact")
+                               k.shape[0], _ptr(ws), nbytes, _stream(dev)), "page_compact")
     _counted(kpool, vpool, k_scale, v_scale, *(out or ()))
     return tuple(new)
 

@@ -139,6 +139,42 @@ def test_compact(K, b, most, ps, width, n_pages, in_place):
             assert args[0].tolist() == table and args[2].tolist() == refs
 
 
+@pytest.mark.parametrize("in_place", [(), (0,), (1,), (2,), (0, 1, 2)])
+def test_much_that_moves_and_books_partly_in_place(K, in_place):
+    """Pools of many layers, whose pages more than a cluster moves; some of the books in place."""
+    b, ps, width, n_pages, heads = 60, 16, 20, 500, 40
+    table, lens, refs = state(8, b, 200, ps, width, n_pages, 100)
+    add = [1 + i % 2 for i in range(b)]
+    g = generator(3)
+    (kp, ks), (vp, vs) = pool_of(g, "e4m3", heads, n_pages, ps), pool_of(g, "e4m3", heads, n_pages, ps)
+    fresh = lambda: [int32(table), int32(lens), int32(refs)]
+
+    def out_of(args, which):
+        return tuple(args[i] if n in in_place else torch.full_like(args[i], 9) for n, i in enumerate(which))
+
+    rows, new_lens, new_refs = hand.fork(table, lens, refs, [i // 3 for i in range(b)], ps)
+    args = fresh()
+    got = K.page_fork(*args, int32([i // 3 for i in range(b)]), page_size=ps, out=out_of(args, (0, 1, 2)))
+    assert torch.equal(got[0], filled(rows, width)) and got[1].tolist() == new_lens and got[2].tolist() == new_refs
+    rows, new_lens, new_refs, moves = hand.extend(table, lens, refs, add, ps, width)
+    assert len(moves) > 10
+    pools, args = (kp.clone(), vp.clone(), ks.clone(), vs.clone()), fresh()
+    got = K.page_extend(*args, *pools[:2], int32(add), page_size=ps, k_scale=pools[2], v_scale=pools[3], out=out_of(args, (0, 1, 2)))
+    assert torch.equal(got[0], filled(rows, width)) and got[1].tolist() == new_lens and got[2].tolist() == new_refs
+    for pool, scale, old, old_scale in zip(pools[:2], pools[2:], (kp, vp), (ks, vs)):
+        x, s = moved(old, old_scale, moves, ps)
+        assert torch.equal(pool.view(x.dtype), x) and torch.equal(scale, s)
+    rows, new_refs, where, moves = hand.compact(table, lens, refs, ps)
+    assert len(moves) > 10
+    pools, args = (kp.clone(), vp.clone(), ks.clone(), vs.clone()), fresh()
+    out = out_of(args, (0, 2)) + (torch.empty_like(args[2]),)
+    got = K.page_compact(*args, *pools[:2], page_size=ps, k_scale=pools[2], v_scale=pools[3], out=out)
+    assert torch.equal(got[0], filled(rows, width)) and got[1].tolist() == new_refs and got[2].tolist() == where and all(a is b for a, b in zip(got, out))
+    for pool, scale, old, old_scale in zip(pools[:2], pools[2:], (kp, vp), (ks, vs)):
+        x, s = moved(old, old_scale, moves, ps)
+        assert torch.equal(pool.view(x.dtype), x) and torch.equal(scale, s)
+
+
 def test_sequences_that_want_more_than_there_is(K):
     """More than 2^31 pages in all: the first that does not get its own, and those behind it that want any, stay as they are."""
     b, ps, width = 40, 1, 1 << 20

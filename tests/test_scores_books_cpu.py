@@ -46,8 +46,8 @@ def test_token_refuses(status, bad):
 B2, C2 = A + 1024, A + 2048
 
 
-def fork(t=A, ld=8, lens=A, refs=A, parents=A, to=B2, ldo=8, lo=B2, ro=B2, B=2, W=8, n=16, ps=16):
-    return lib.q40_page_fork(t, ld, lens, refs, parents, to, ldo, lo, ro, B, W, n, ps, None)
+def fork(t=A, ld=8, lens=A, refs=A, parents=A, to=B2, ldo=8, lo=B2, ro=B2, B=2, W=8, n=16, ps=16, ws=None, nb=0):
+    return lib.q40_page_fork(t, ld, lens, refs, parents, to, ldo, lo, ro, B, W, n, ps, ws, nb, None)
 
 
 def extend(t=A, ld=8, lens=A, refs=A, add=A, to=B2, ldo=8, lo=B2, ro=B2, B=2, W=8, n=16, ps=16, k=A, v=A, ks=A, vs=A, kind=1, P=256, heads=2, ws=C2, nb=1 << 20):
@@ -62,10 +62,10 @@ BOOKS = [(NULL, dict(t=None)), (NULL, dict(to=None)), (NULL, dict(lens=None)), (
          (SHAPE, dict(W=1 << 29, ld=1 << 29, ldo=1 << 29)), (SHAPE, dict(n=-1)), (SHAPE, dict(n=(1 << 28) + 1)), (SHAPE, dict(ps=0)), (SHAPE, dict(ps=(1 << 29) + 1)), (ALIGN, dict(t=A + 2)), (ALIGN, dict(lens=A + 1)),
          (ALIGN, dict(refs=A + 2)), (ALIGN, dict(to=B2 + 2)), (ALIGN, dict(ro=B2 + 1))]
 POOLS = [(NULL, dict(k=None)), (NULL, dict(vs=None)), (SHAPE, dict(P=255)), (SHAPE, dict(P=240)), (SHAPE, dict(heads=-1)), (UNSUPPORTED, dict(kind=3)), (UNSUPPORTED, dict(kind=-1)), (ALIGN, dict(v=A + 8)),
-         (ALIGN, dict(ks=A + 2)), (NULL, dict(ws=None)), (ALIGN, dict(ws=C2 + 4)), (WORKSPACE, dict(nb=15)), (SHAPE, dict(to=A, ldo=9))]
+         (ALIGN, dict(ks=A + 2)), (WORKSPACE, dict(to=A, ws=None)), (ALIGN, dict(ws=C2 + 4)), (WORKSPACE, dict(to=A, nb=15)), (WORKSPACE, dict(n=16385, ps=1, P=16385, nb=15)), (SHAPE, dict(to=A, ldo=9))]
 
 
-@pytest.mark.parametrize("status,bad", BOOKS + [(NULL, dict(parents=None)), (NULL, dict(lo=None)), (ALIGN, dict(parents=A + 2)), (ALIGN, dict(lo=A + 2)), (UNSUPPORTED, dict(to=A)), (UNSUPPORTED, dict(lo=A)),
+@pytest.mark.parametrize("status,bad", BOOKS + [(NULL, dict(parents=None)), (NULL, dict(lo=None)), (ALIGN, dict(parents=A + 2)), (ALIGN, dict(lo=A + 2)), (ALIGN, dict(ws=A + 2)), (SHAPE, dict(to=A, ldo=9)), (WORKSPACE, dict(to=A, B=600)), (WORKSPACE, dict(lo=A, B=600, ws=C2, nb=600 * 36 - 1)),
                                                 (0, dict(B=0, n=0))])
 def test_fork_refuses(status, bad):
     assert fork(**bad) == status
@@ -82,8 +82,11 @@ def test_compact_refuses(status, bad):
 
 
 def test_books_workspace():
-    assert lib.q40_page_extend_workspace_bytes(10, 100) == (70 + 200 + 4) * 4 and lib.q40_page_extend_workspace_bytes(-1, 5) == 0
-    assert lib.q40_page_compact_workspace_bytes(101) == (3 * 51 + 4) * 4 and lib.q40_page_compact_workspace_bytes(-1) == 0
+    assert lib.q40_page_fork_workspace_bytes(600, 8, 16) == 600 * 9 * 4 and lib.q40_page_fork_workspace_bytes(500, 8, 16) == 0
+    assert lib.q40_page_extend_workspace_bytes(10, 100, 1) == (70 + 200 + 4) * 4 and lib.q40_page_extend_workspace_bytes(-1, 5, 1) == 0
+    assert lib.q40_page_extend_workspace_bytes(10, 100, 0) == lib.q40_page_extend_workspace_bytes(1024, 16384, 0) == 0 < lib.q40_page_extend_workspace_bytes(1025, 1, 0)
+    assert lib.q40_page_compact_workspace_bytes(101, 1) == (3 * 51 + 4) * 4 and lib.q40_page_compact_workspace_bytes(-1, 1) == 0
+    assert lib.q40_page_compact_workspace_bytes(16384, 0) == 0 < lib.q40_page_compact_workspace_bytes(16385, 0)
 
 
 def test_hand_kept_books_stay_consistent():
