@@ -481,7 +481,20 @@ bool books_pools_of(PyObject* const* args, int dev, const Books& b, int64_t ps, 
   p.k = *k, p.v = *v, p.ks = held(ks), p.vs = held(vs);
   return true;
 }
-at::Tensor ints(at::IntArrayRef size, int dev) { return at::empty(size, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)dev)); }
+// New books: a table and two rows of numbers in one piece of memory, each from 16 bytes on (three pieces take 2 us more)
+void new_books(int64_t B, int64_t W, int64_t n1, int64_t n2, int dev, at::Tensor& table, at::Tensor& one, at::Tensor& two) {
+  const int64_t at1 = (B * W + 3) / 4 * 4, at2 = at1 + (n1 + 3) / 4 * 4;
+  const at::Tensor all = at::empty({at2 + n2}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)dev));
+  const auto part = [&](int64_t from, at::IntArrayRef size) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(from);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+    return t;
+  };
+  table = part(0, {B, W});
+  one = part(at1, {n1});
+  two = part(at2, {n2});
+}
 void written(const at::Tensor& t) {
   if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
@@ -527,9 +540,8 @@ PyObject* page_fork(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int rc;
   {
     WithoutInterpreter without;
-    table = place ? b.table : ints({b.B, b.W}, dev);
-    lens = place ? b.lens : ints({b.B}, dev);
-    refs = place ? b.refs : ints({b.n}, dev);
+    if (place) table = b.table, lens = b.lens, refs = b.refs;
+    else new_books(b.B, b.W, b.B, b.n, dev, table, lens, refs);
     const size_t bytes = place ? page_fork_bytes((int)b.B, (int)b.W, (int)b.n) : 0;
     ws = scratch(bytes, dev);
     rc = page_fork_fn(int_ptr(b.table), b.ld, int_ptr(b.lens), int_ptr(b.refs), int_ptr(from), int_ptr(table), place ? b.ld : b.W, int_ptr(lens), int_ptr(refs), (int)b.B,
@@ -561,9 +573,8 @@ PyObject* page_extend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int rc;
   {
     WithoutInterpreter without;
-    table = place ? b.table : ints({b.B, b.W}, dev);
-    lens = place ? b.lens : ints({b.B}, dev);
-    refs = place ? b.refs : ints({b.n}, dev);
+    if (place) table = b.table, lens = b.lens, refs = b.refs;
+    else new_books(b.B, b.W, b.B, b.n, dev, table, lens, refs);
     const size_t bytes = page_extend_bytes((int)b.B, (int)b.n, place);
     ws = scratch(bytes, dev);
     rc = page_extend_fn(int_ptr(b.table), b.ld, int_ptr(b.lens), int_ptr(b.refs), int_ptr(more), int_ptr(table), place ? b.ld : b.W, int_ptr(lens), int_ptr(refs), (int)b.B,
@@ -593,9 +604,8 @@ PyObject* page_compact(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int rc;
   {
     WithoutInterpreter without;
-    table = place ? b.table : ints({b.B, b.W}, dev);
-    refs = place ? b.refs : ints({b.n}, dev);
-    if (!place) where = ints({b.n}, dev);
+    if (place) table = b.table, refs = b.refs;
+    else new_books(b.B, b.W, b.n, b.n, dev, table, refs, where);
     const size_t bytes = page_compact_bytes((int)b.n, place);
     ws = scratch(bytes, dev);
     rc = page_compact_fn(int_ptr(b.table), b.ld, int_ptr(b.lens), int_ptr(b.refs), int_ptr(table), place ? b.ld : b.W, int_ptr(refs), int_ptr(where), (int)b.B, (int)b.W, (int)b.n, (int)ps,
