@@ -132,6 +132,7 @@ extern "C" int q40_attn_causal_scores(const void* q, int64_t ldq, const void* k,
     const double unit = 1. / (sqrt((double)D) * softcap);          // of a raw score, in caps
     a.cap_limit = (float)(TANH_TO / unit); a.cap_exp = (float)(2. * unit * 1.4426950408889634); a.cap_out = (float)(1. / unit);
     tanh_poly_of(unit, a.cap_k);
+    for (float& k : a.cap_k) k = (float)((double)k * a.scale_log2);
   }
   a.splits = 1;
   const int splits = splits_of(S, H, Hkv, offset, window, sinks);

@@ -246,8 +246,10 @@ struct Row {
 #pragma unroll
     for (int c = 0; c < 4; ++c) ld32(s_at + 32 * c, s + 32 * c);
     wait_ld();
-    if constexpr (F::CAP) cap(a, s);
-    if constexpr (F::BIAS) bias(a, s, p, key0);
+    Cap k;
+    if constexpr (F::CAP) k = cap(a, s);
+    float rise = 0.f, begin = 0.f;                 // scores with a bias are log2, less `begin + c rise` in places 16 c .. 16 c + 15
+    if constexpr (F::BIAS) bias(a, s, p, key0, k, rise, begin);
     if (masked) {
       const int last = (F::SPANS ? span.last : p) - key0, first = (F::SPANS ? span.start : 0) + a.sinks - key0;
       const int from = (F::SPANS ? max(p - a.window, span.start - 1) : p - a.window) - key0;      // seen: places <= last that are > from or < first
@@ -261,14 +263,27 @@ struct Row {
           if (!(seen & (1u << e))) s[c + e] = -CUDART_INF_F;
       }
     }
-    float mx[4] = {s[0], s[1], s[2], s[3]};
+    float most;
+    if constexpr (F::BIAS) {
+      most = -CUDART_INF_F;
 #pragma unroll
-    for (int c = 4; c < BK - 4; c += 8)
+      for (int c = 0; c < BK; c += 16) {
+        float mx[2] = {max3(s[c], s[c + 1], s[c + 2]), max3(s[c + 8], s[c + 9], s[c + 10])};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
+        for (int e = 3; e < 7; e += 2) mx[0] = max3(mx[0], s[c + e], s[c + e + 1]), mx[1] = max3(mx[1], s[c + 8 + e], s[c + 9 + e]);
+        most = fmaxf(most, fmaf((float)(c / 16), rise, begin) + max3(fmaxf(mx[0], mx[1]), s[c + 7], s[c + 15]));
+      }
+    } else {
+      float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[BK - 4 + e]);
-    const float scale = F::BIAS ? 1.f : a.scale_log2, most = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * scale;
+      for (int c = 4; c < BK - 4; c += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[BK - 4 + e]);
+      most = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
+      most *= F::CAP ? k.of(most * most) : a.scale_log2;
+    }
     const bool passes = most > m + WEIGHT_TOP;
     if (__any_sync(0xffffffffu, passes)) {
       const float now = passes ? most - WEIGHT_SET : m, corr = fmaxf(ex2(m - now), 1.17549435e-38f);      // (never 0: infinities stay)
@@ -287,7 +302,7 @@ struct Row {
         wait_st();
       }
     }
-    const uint64_t scale2 = pack2(scale, scale), m2 = pack2(-m, -m);
+    const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), m2 = pack2(-m, -m);
     uint64_t sum[2] = {0, 0};                      // of this step: weight by weight onto l, the low bits of each would be lost to a long sum
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -295,7 +310,13 @@ struct Row {
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
         float x, y;
-        unpack2(fma2(pack2(s[64 * c + 2 * e], s[64 * c + 2 * e + 1]), scale2, m2), x, y);
+        const uint64_t s2 = pack2(s[64 * c + 2 * e], s[64 * c + 2 * e + 1]);
+        if constexpr (F::BIAS) {
+          const float less = fmaf((float)(4 * c + e / 8), rise, begin) - m;
+          unpack2(add2(s2, pack2(less, less)), x, y);
+        } else {
+          unpack2(fma2(s2, F::CAP ? k.of(mul2(s2, s2)) : scale2, m2), x, y);
+        }
         x = ex2(x);
         y = ex2(y);
         sum[e & 1] = add2(sum[e & 1], pack2(x, y));
@@ -312,45 +333,55 @@ struct Row {
     l += x + y;
     ++n;
   }
-  // c tanh(s / c) of raw scores, in raw units: s times a polynomial in s^2 while all of a warp's are in its range
-  static __device__ __forceinline__ void cap(const Call& a, float (&s)[BK]) {
+  // A raw score s becomes s of(s^2) in log2: a polynomial while all of a warp's are in its range, else that much of what they have become by 2^x.  (The coefficient of the
+  // highest power is above 0 there too, so that a masked -inf stays one)
+  struct Cap {
+    float x[5];
+    __device__ __forceinline__ float of(float u) const { return fmaf(fmaf(fmaf(fmaf(x[4], u, x[3]), u, x[2]), u, x[1]), u, x[0]); }
+    __device__ __forceinline__ uint64_t of(uint64_t u) const {
+      uint64_t y = pack2(x[4], x[4]);
+#pragma unroll
+      for (int i = 3; i >= 0; --i) y = fma2(y, u, pack2(x[i], x[i]));
+      return y;
+    }
+  };
+  static __device__ __forceinline__ Cap cap(const Call& a, float (&s)[BK]) {
     float big[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < BK; c += 8)
 #pragma unroll
       for (int e = 0; e < 4; ++e) big[e] = max3(big[e], fabsf(s[c + e]), fabsf(s[c + 4 + e]));
+    Cap k;
     if (__any_sync(0xffffffffu, max3(fmaxf(big[0], big[1]), big[2], big[3]) > a.cap_limit)) {
 #pragma unroll
       for (int e = 0; e < BK; ++e) s[e] = tanh_by_exp(s[e] * a.cap_exp) * a.cap_out;
+      k = {{a.scale_log2, 0.f, 0.f, 0.f, 1e-44f}};
     } else {
-      uint64_t k[5];
 #pragma unroll
-      for (int i = 0; i < 5; ++i) k[i] = pack2(a.cap_k[i], a.cap_k[i]);
-#pragma unroll
-      for (int e = 0; e < BK; e += 2) {
-        const uint64_t x = pack2(s[e], s[e + 1]), u = mul2(x, x);
-        unpack2(mul2(x, fma2(fma2(fma2(fma2(k[4], u, k[3]), u, k[2]), u, k[1]), u, k[0])), s[e], s[e + 1]);
-      }
+      for (int i = 0; i < 5; ++i) k.x[i] = a.cap_k[i];
     }
+    return k;
   }
-  // Scores in log2 less what the distances cost
-  __device__ __forceinline__ void bias(const Call& a, float (&s)[BK], int p, int key0) const {
+  // Scores become log2 of what they are with their bias, less what 16 of them share: an instruction for two of them, where whole biases would be two
+  __device__ __forceinline__ void bias(const Call& a, float (&s)[BK], int p, int key0, const Cap& k, float& rise, float& begin) const {
     const float at = (float)(key0 - p);
-    if (__any_sync(0xffffffffu, key0 + BK - 1 > p && span.last > p)) {         // keys ahead of some row
+    const bool ahead = __any_sync(0xffffffffu, key0 + BK - 1 > p && span.last > p);          // keys ahead of some row
+    uint64_t each[8];
 #pragma unroll
-      for (int e = 0; e < BK; ++e) s[e] = fmaf(s[e], a.scale_log2, -slope * fabsf(at + (float)e));
+    for (int i = 0; i < 8; ++i) each[i] = ahead ? 0 : pack2(slope * (float)(2 * i), slope * (float)(2 * i + 1));
+    const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2);
+#pragma unroll
+    for (int e = 0; e < BK; e += 2) {
+      const uint64_t s2 = pack2(s[e], s[e + 1]);
+      unpack2(fma2(s2, F::CAP ? k.of(mul2(s2, s2)) : scale2, each[e / 2 % 8]), s[e], s[e + 1]);
+    }
+    if (ahead) {
+#pragma unroll
+      for (int e = 0; e < BK; ++e) s[e] = fmaf(-slope, fabsf(at + (float)e), s[e]);
+      rise = begin = 0.f;
     } else {
-      const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2);
-      uint64_t k[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) k[i] = pack2(slope * (float)(2 * i), slope * (float)(2 * i + 1));
-#pragma unroll
-      for (int c = 0; c < BK; c += 8) {
-        const float b = slope * (at + (float)c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          unpack2(fma2(pack2(s[c + 2 * i], s[c + 2 * i + 1]), scale2, add2(pack2(b, b), k[i])), s[c + 2 * i], s[c + 2 * i + 1]);
-      }
+      rise = 16.f * slope;
+      begin = slope * at;
     }
   }
   // ... and its output, or a split's partial result.  taken_out: values that are not finite were taken out of tiles that `sees` say are seen in part
