@@ -34,34 +34,51 @@ struct Scores {
   struct Places { SpanTiles tiles; SpanSees sees[2]; };
   static __device__ __forceinline__ bool keeps(const ScoreArgs& a) { return a.keep; }
 
-  static __device__ __forceinline__ Span span_of(const ScoreArgs& a, int row) {
-    if (!a.documents) {
-      const int p = a.offset + row;
-      return {0, max(p, a.prefix - 1)};
-    }
-    if (a.documents[0] > row) return {row, -2};
+  // The span of a row, documents(k) being where document k begins
+  template <class D>
+  static __device__ __forceinline__ Span span_in(const ScoreArgs& a, int row, D documents) {
+    if (documents(0) > row) return {row, -2};
     int k = 0, above = a.n_documents + 1;                // the last that begins at the row or in front of it
     while (above - k > 1) {
       const int mid = (k + above) >> 1;
-      if (a.documents[mid] <= row) k = mid;
+      if (documents(mid) <= row) k = mid;
       else above = mid;
     }
     if (k == a.n_documents) return {row, row - 1};
-    const int start = max(a.documents[k], 0), end = min(a.documents[k + 1], a.S);
+    const int start = max(documents(k), 0), end = min(documents(k + 1), a.S);
     const int prefix = min(a.prefixes ? a.prefixes[k] : a.prefix, end - start);
     return {start, max(row, start + prefix - 1)};
   }
+  static __device__ __forceinline__ Span span_of(const ScoreArgs& a, int row) {
+    const int p = a.offset + row;
+    return {0, max(p, a.prefix - 1)};
+  }
   // Every thread of the CTA calls it; a thread that has a row gets its span
-  static __device__ __forceinline__ Places places(const ScoreArgs& a, int row0, int split, Span& mine) {
+  template <class B>
+  static __device__ __forceinline__ Places places(const ScoreArgs& a, int row0, int split, Span& mine, B begin) {
     const int n = min(2 * BQ, a.S - row0), p0 = a.offset + row0;
     const int ends[4] = {0, min(BQ, n) - 1, BQ, n - 1};
     Span at[4];
+    const auto places_of = [&]() -> Places {
+      return {SpanTiles(a, row0, 2 * BQ, split, at[0], at[3], BIAS),
+              {SpanSees(p0, at[0], p0 + ends[1], at[1], a.window, a.sinks), SpanSees(p0 + BQ, at[2], p0 + n - 1, at[3], a.window, a.sinks)}};
+    };
     if (a.documents) {
+      // Where documents begin is read once by all threads, up to FEW of them; looked up in global memory, a handful took a microsecond
+      constexpr int FEW = 256;
       __shared__ Span edges[4];
+      __shared__ int begins[FEW];
       asm volatile("griddepcontrol.wait;" ::: "memory");
       const int r = threadIdx.x;
+      begin();                                           // (the queries are on their way meanwhile)
+      const bool few = a.n_documents < FEW;
+      if (few) {
+        if (r <= a.n_documents) begins[r] = a.documents[r];
+        __syncthreads();
+      }
       if (r < 2 * BQ) {
-        mine = span_of(a, row0 + min(r, n - 1));
+        const int row = row0 + min(r, n - 1);
+        mine = few ? span_in(a, row, [&](int k) { return begins[k]; }) : span_in(a, row, [&](int k) { return a.documents[k]; });
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (r == ends[e]) edges[e] = mine;
@@ -69,13 +86,15 @@ struct Scores {
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < 4; ++e) at[e] = edges[e];
+      return places_of();
     } else {
       mine = span_of(a, row0 + min((int)threadIdx.x, n - 1));
 #pragma unroll
       for (int e = 0; e < 4; ++e) at[e] = span_of(a, row0 + min(ends[e], n - 1));
+      const Places there = places_of();
+      begin();
+      return there;
     }
-    return {SpanTiles(a, row0, 2 * BQ, split, at[0], at[3]),
-            {SpanSees(p0, at[0], p0 + ends[1], at[1], a.window, a.sinks), SpanSees(p0 + BQ, at[2], p0 + n - 1, at[3], a.window, a.sinks)}};
   }
 };
 
