@@ -246,10 +246,12 @@ attn_pages_kernel(const Call<SCORES> a) {
   }
   float slope[HL];                               // of the lane's heads, log2
   int newest = 0;                                // the query's position: that of the last key
+  float skip = 0.f;
   if constexpr (SCORES) {
 #pragma unroll
     for (int j = 0; j < HL; ++j) slope[j] = a.slopes ? a.slopes[h0 + min(HL == 2 ? 2 * t + j : t >> GL, heads - 1)] * 1.44269504f : 0.f;
     newest = vis.n - 1 + vis.skip;
+    skip = (float)vis.skip;
   }
   float m[HL], l[HL], acc[8][4];
 #pragma unroll
@@ -302,16 +304,22 @@ attn_pages_kernel(const Call<SCORES> a) {
       for (int r = 0; r < 2 * MT; ++r) {
         const float scale = T == CACHE_F16 ? a.scale_log2 : a.scale_log2 * lds32(vt + KEYS * RB + (8 * r + g) * 4);
 #pragma unroll
-        for (int j = 0; j < HL; ++j) s[HL * r + j] = i0 + 8 * r + g < end ? x[r >> 1][2 * (r & 1) + j] * scale : 0.f;
+        for (int j = 0; j < HL; ++j) s[HL * r + j] = x[r >> 1][2 * (r & 1) + j] * scale;
       }
       if (a.cap_out != 0.f) cap(a, s);
+      if (a.slopes) {
+        const float far = (float)(newest - vis.skip - i0 - g);       // of key g; another is 8 r nearer, a first key `skip` further away
 #pragma unroll
-      for (int r = 0; r < 2 * MT; ++r) {
-        const int i = i0 + 8 * r + g;
-        const float far = (float)(newest - (i < vis.first ? i : i + vis.skip));
+        for (int r = 0; r < 2 * MT; ++r) {
+          const float d = far - (float)(8 * r) + (i0 + 8 * r + g < vis.first ? skip : 0.f);
 #pragma unroll
-        for (int j = 0; j < HL; ++j) x[r >> 1][2 * (r & 1) + j] = a.slopes ? fmaf(-slope[j], far, s[HL * r + j]) : s[HL * r + j];
+          for (int j = 0; j < HL; ++j) s[HL * r + j] = fmaf(-slope[j], d, s[HL * r + j]);
+        }
       }
+#pragma unroll
+      for (int r = 0; r < 2 * MT; ++r)
+#pragma unroll
+        for (int j = 0; j < HL; ++j) x[r >> 1][2 * (r & 1) + j] = s[HL * r + j];
     }
 #pragma unroll
     for (int r = 0; r < 2 * MT; ++r) {
