@@ -191,19 +191,27 @@ struct Run {
     hi = (int)min(first + each, (int64_t)pages);
   }
 };
-// The pages of a run, 32 at a time, four of these requested together: f(first page, this lane's references; 0 behind the end)
-template <class F>
-__device__ __forceinline__ void through(const int32_t* refs, const Run& run, F f) {
-  const int lane = threadIdx.x & 31;
-  for (int p0 = run.lo; p0 < run.hi; p0 += 128) {
-    int r[4];
+// The pages of a run, 32 at a time, four of these requested together, the first before what they are for: f(first page, this lane's references; 0 behind the end)
+struct Ahead {
+  int r[4];
+  __device__ __forceinline__ Ahead(const int32_t* refs, const Run& run, int p0) {
+    const int p = p0 + (int)(threadIdx.x & 31);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = p0 + 32 * i + lane < run.hi ? refs[p0 + 32 * i + lane] : 0;
+    for (int i = 0; i < 4; ++i) r[i] = p + 32 * i < run.hi ? refs[p + 32 * i] : 0;
+  }
+};
+template <class F>
+__device__ __forceinline__ void through(const int32_t* refs, const Run& run, Ahead ahead, F f) {
+  for (int p0 = run.lo; p0 < run.hi; p0 += 128) {
+    if (p0 > run.lo) ahead = Ahead(refs, run, p0);
+    const int(&r)[4] = ahead.r;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (p0 + 32 * i < run.hi) f(p0 + 32 * i, r[i]);
   }
 }
+template <class F>
+__device__ __forceinline__ void through(const int32_t* refs, const Run& run, F f) { through(refs, run, Ahead(refs, run, run.lo), f); }
 // Sum of x over the warps in front of this one, and over all of the CTA (each lane of a warp has its x).  All threads call it
 __device__ __forceinline__ int before_in_cta(int x, int* sums, int& all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -395,20 +403,23 @@ extend_few_kernel(const Extension a, const Pools pools) {
   int* const rows = dst + FEW_ROWS;
   int* const handed = rows + FEW_ROWS;           // [pages] free ones, in order
   int* const refs = handed + (a.pages + 3) / 4 * 4;          // [pages], of the CTA that counts
-  __shared__ int sums[WARPS];
+  __shared__ int sums[WARPS], masks[FEW_PAGES / 32];               // (masks: a bit for each free page)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x, ctas = gridDim.x;
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   const Run run(a.pages, warp, WARPS);
-  int free = 0;
-  through(a.refs, run, [&](int p0, int r) {
-    free += __popc(__ballot_sync(0xffffffffu, p0 + lane < run.hi && r <= 0));
-    if (!IN_PLACE && cta == 0 && p0 + lane < run.hi) refs[p0 + lane] = r;
-  });
+  const Ahead ahead(a.refs, run, run.lo);
   const bool there = tid < a.B;
   Growth g;
   if (there) g = Growth(a, tid);
+  int free = 0;
+  through(a.refs, run, ahead, [&](int p0, int r) {
+    const uint32_t mask = __ballot_sync(0xffffffffu, p0 + lane < run.hi && r <= 0);
+    free += __popc(mask);
+    if (lane == 0) masks[p0 / 32] = (int)mask;
+    if (!IN_PLACE && cta == 0 && p0 + lane < run.hi) refs[p0 + lane] = r;
+  });
   const bool shares = there && g.tail >= 0 && g.shared > 1;
   tails[tid] = shares ? g.tail : -1;
   int all_free;
@@ -429,24 +440,22 @@ extend_few_kernel(const Extension a, const Pools pools) {
     copies = !(writers == g.shared && last == tid);
   }
   const int need = g.grows ? min(g.n1 - g.n0 + (copies ? 1 : 0), a.pages + 1) : 0;       // (their sum is below 2^25)
-  int upto = need, wanted, front, n_moves;
+  int upto = need, wanted, n_moves;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += y;
   }
-  front = before_in_cta(__shfl_sync(0xffffffffu, upto, 31), sums, wanted);
-  upto += front;
+  upto += before_in_cta(__shfl_sync(0xffffffffu, upto, 31), sums, wanted);
   const bool granted = g.grows && (need == 0 || upto <= all_free);
   const bool moves = granted && copies;
   const uint32_t moving = __ballot_sync(0xffffffffu, moves);
-  front = before_in_cta(__popc(moving), sums, n_moves) + __popc(moving & ((1u << lane) - 1u));
-  through(a.refs, run, [&](int p0, int r) {
-    const bool is_free = p0 + lane < run.hi && r <= 0;
-    const uint32_t mask = __ballot_sync(0xffffffffu, is_free);
-    if (is_free) handed[rank + __popc(mask & ((1u << lane) - 1u))] = p0 + lane;
+  const int front = before_in_cta(__popc(moving), sums, n_moves) + __popc(moving & ((1u << lane) - 1u));       // (each CTA has the same order)
+  for (int p0 = run.lo; p0 < run.hi; p0 += 32) {
+    const uint32_t mask = (uint32_t)masks[p0 / 32];
+    if ((mask >> lane) & 1u) handed[rank + __popc(mask & ((1u << lane) - 1u))] = p0 + lane;
     rank += __popc(mask);
-  });
+  }
   int len = g.n;
   if (there) {
     const bool gives = a.add[tid] <= 0;
