@@ -5,11 +5,18 @@
 // j - s < sinks).  Its score of key j is c tanh(x / c) - slope |p - j|, x = q . k / sqrt(128).
 //
 // The kernel is that of attn_tc.cuh.  What is added, a step of 128 keys a row:
-//   cap      tanh(x) = x P(x^2), P of degree 4, while no |x / c| of the warp's rows is above 0.625: seven packed instructions for two scores and 32 of three inputs
-//            for the largest magnitude; else 1 - 2 / (1 + e^2x), two more of the sixteen-a-cycle functions a score, of which 2^x takes as long as the MMAs do
-//   bias     two packed instructions for two scores; distances are whole numbers, and each bias is rounded once or twice, by 2^-24 of itself
+//   cap      tanh(x) = x P(x^2), P of degree 4, while no |x / c| of the warp's rows is above 0.625, in the product that makes the exponent: five packed instructions
+//            more for two scores, and 64 of three inputs for the largest magnitude; else 1 - 2 / (1 + e^2x), two more of the sixteen-a-cycle functions a score, of
+//            which 2^x takes as long as the MMAs do.  (P of degree 7 in between, up to 1.25: 3920 -> 3444 us where all scores lie there, 16384 positions as below, but 320 ->
+//            364 where they lie on both sides, 4001 positions: not taken)
+//   bias     two packed instructions for two scores.  Sixteen keys share what their distances have in common; each bias is rounded twice, by 2^-24 of what is
+//            left to the nearest of them.  Near keys come first: their scores are the largest, and O, once scaled for each step of a steep slope, is not any more (2079 -> 1762 us)
 //   masks    what a row sees is an interval and the first keys of its document: words of bits, in tiles that some row does not see whole
-// Documents are looked up by each row (a search in the offsets) and once more for the tile of keys to start and end with.
+// Documents are looked up by each row; what a tile's first and last row see tells which tiles of keys it goes through.
+//
+// Us by the card: 16384 positions, window 4096, 64 heads on 8: 1650 with plain scores, 1760 with slopes, 2040 with a cap, 2440 with both; 4001 positions of 32 heads in nine
+// documents 71 (73 with slopes), where the bytes take 20 and the MMAs 25: 512 CTAs of some ten steps each, 3 us of start and 4 of end around 2 a step, with nothing
+// beside them on their SM.  One tile of queries a CTA and two CTAs an SM: 68 (75 with slopes), 2120 for the cap, 2290 for both: not taken, since others lose 5 %.
 #include "attn_tc.cuh"
 
 namespace q40 {

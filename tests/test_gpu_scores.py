@@ -90,7 +90,7 @@ def test_scores(K, s, h, hkv, window, sinks, offset, softcap, alibi):
 
 
 @pytest.mark.parametrize("softcap", [0.01, 0.5, 5.0, 1000.0])
-@pytest.mark.parametrize("size", [0.01, 1.0, 30.0])
+@pytest.mark.parametrize("size", [0.01, 1.0, 30.0, 200.0])
 def test_caps_of_every_size(K, softcap, size):
     """Scores far below and far above the cap, and both in one tile."""
     g = generator(3)
