@@ -53,7 +53,7 @@ struct Scores {
     }
     if (k == a.n_documents) return {row, row - 1};
     const int start = max(documents(k), 0), end = min(documents(k + 1), a.S);
-    const int prefix = min(a.prefixes ? a.prefixes[k] : a.prefix, end - start);
+    const int prefix = min(max(a.prefixes ? a.prefixes[k] : a.prefix, 0), end - start);
     return {start, max(row, start + prefix - 1)};
   }
   static __device__ __forceinline__ Span span_of(const ScoreArgs& a, int row) {

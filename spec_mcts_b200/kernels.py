@@ -478,7 +478,7 @@ def _tc_error_page(dev, st) -> torch.Tensor:
 
 
 def tc_error_flag(dev=None) -> int:
-    """1 if a tensor-core matmul launched through matmul_q40, linear_q40 or a prompt pass, or causal_attn with a window, on the current stream of `dev` gave up
+    """1 if a tensor-core matmul launched through matmul_q40, linear_q40 or a prompt pass, or causal_attn with a window, changed scores, documents or a prefix, on the current stream of `dev` gave up
     on one of its bounded waits since the workspace was created (synchronises the device).  Not reported: matmuls
     captured on a stream on which no call that needs a workspace was made outside of a capture before."""
     dev = _indexed(dev)
@@ -1047,6 +1047,11 @@ def _books(what: str, p, lens, refs, page_size: int, out, fresh):
     return p, lens, refs, list(out)
 
 
+def _numbers(t: torch.Tensor, least: int, most: int) -> torch.Tensor:
+    """Whole numbers as int32; of wider types, those out of range as the nearest."""
+    return (t.clamp(least, most) if t.dtype == torch.int64 else t).to(torch.int32).contiguous()
+
+
 def _table_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
@@ -1086,7 +1091,7 @@ def page_fork(p, lens, refs, parents, *, page_size: int, out=None):
     B, W = p.shape
     if parents.shape != (B,) or parents.is_floating_point():
         raise Q40Error(f"page_fork: {B} parents expected, got {tuple(parents.shape)} of {parents.dtype}")
-    parents = parents.to(torch.int32).contiguous()
+    parents = _numbers(parents, -1, B)
     nbytes = lib.q40_page_fork_workspace_bytes(B, W, refs.shape[0]) if out is not None else 0
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None           # of this call alone, as in _attn_pages
     check(lib.q40_page_fork(p.data_ptr(), _table_stride(p), lens.data_ptr(), refs.data_ptr(), parents.data_ptr(), new[0].data_ptr(), _table_stride(new[0]),
@@ -1112,7 +1117,7 @@ def page_extend(p, lens, refs, kpool, vpool, add, *, page_size: int, k_scale=Non
     B, W = p.shape
     if add.shape != (B,) or add.is_floating_point() or B > 16384:
         raise Q40Error(f"page_extend: numbers of tokens for {B} sequences (at most 16384) expected, got {tuple(add.shape)} of {add.dtype}")
-    add = add.to(torch.int32).contiguous()
+    add = _numbers(add, -(1 << 31), (1 << 31) - 1)
     nbytes = lib.q40_page_extend_workspace_bytes(B, refs.shape[0], out is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None           # of this call alone, as in _attn_pages
     check(lib.q40_page_extend(p.data_ptr(), _table_stride(p), lens.data_ptr(), refs.data_ptr(), add.data_ptr(), new[0].data_ptr(), _table_stride(new[0]), new[1].data_ptr(),

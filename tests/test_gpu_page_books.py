@@ -225,6 +225,22 @@ def test_books_that_do_not_fit_fault_nothing(K):
     test_extend(K, 16, 100, 5, 40, 300, False)
 
 
+def test_numbers_of_other_types(K):
+    """Wide ones out of range are so, and not what their low bits say."""
+    table, lens, refs = state(2, 9, 40, 4, 12, 90)
+    pool = lambda: normal(generator(1), 1, 360, D)
+    wide = lambda *x: torch.tensor(x, dtype=torch.int64, device="cuda")
+    books = int32(table), int32(lens), int32(refs)
+    far = K.page_fork(*books, wide(1 << 32, -(1 << 40), (1 << 33) + 1, 3, 4, 5, 6, 7, 8), page_size=4)
+    near = K.page_fork(*books, int32([-1, -1, -1, 3, 4, 5, 6, 7, 8]), page_size=4)
+    assert all(torch.equal(a, b) for a, b in zip(far, near))
+    far = K.page_extend(*books, pool(), pool(), wide(1 << 32, -(1 << 40), (1 << 33) + 1, 1, 1, 1, 0, 0, 0), page_size=4)
+    near = K.page_extend(*books, pool(), pool(), int32([1 << 30, -(1 << 30), 1 << 30, 1, 1, 1, 0, 0, 0]), page_size=4)
+    assert all(torch.equal(a, b) for a, b in zip(far, near))
+    short = K.page_extend(*books, pool(), pool(), int32([1, -1, 0, 1, 1, 1, 0, 0, 0]).short(), page_size=4)
+    assert all(torch.equal(a, b) for a, b in zip(short, K.page_extend(*books, pool(), pool(), int32([1, -1, 0, 1, 1, 1, 0, 0, 0]), page_size=4)))
+
+
 def test_strided_books(K):
     table, lens, refs = state(5, 20, 60, 4, 16, 200)
     wide = torch.full((20, 50), 9, dtype=torch.int32, device="cuda")

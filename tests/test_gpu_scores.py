@@ -116,7 +116,7 @@ def test_documents(K, documents, window, sinks):
 
 
 @pytest.mark.parametrize("softcap,alibi,window", [(None, False, None), (50.0, False, 70), (None, True, None), (5.0, True, 200)])
-@pytest.mark.parametrize("documents,prefixes", [([0, 40, 300], [10, 100]), ([0, 128, 384, 400, 1000], [128, 200, 0, 600]), ([5, 700, 990], [0, 1000]), ([0, 1, 2, 999], [1, -5, 1 << 30]),
+@pytest.mark.parametrize("documents,prefixes", [([0, 40, 300], [10, 100]), ([0, 128, 384, 400, 1000], [128, 200, 0, 600]), ([5, 700, 990], [0, 1000]), ([0, 1, 2, 999], [1, -5, 1 << 30]), ([0, 400, 999], [-(1 << 31), (1 << 31) - 1]),
                                                 ([0, 500, 1000], [499, 2])])
 def test_documents_with_prefixes(K, documents, prefixes, softcap, alibi, window):
     run(K, generator(7), 1000, 2, 1, window, 3 if window else 0, 0, softcap, alibi, documents, prefixes)
