@@ -271,43 +271,46 @@ struct Row {
           if (!(seen & (1u << e))) s[c + e] = -CUDART_INF_F;
       }
     }
-    float most;
-    if constexpr (F::BIAS) {
-      most = -CUDART_INF_F;
+    // With a cap the largest magnitude is known, which mostly tells that no score of a row passes its maximum
+    if (!F::CAP || __any_sync(0xffffffffu, highest(a, k, p, key0) > m + WEIGHT_TOP)) {
+      float most;
+      if constexpr (F::BIAS) {
+        most = -CUDART_INF_F;
 #pragma unroll
-      for (int c = 0; c < BK; c += 16) {
-        float mx[2] = {max3(s[c], s[c + 1], s[c + 2]), max3(s[c + 8], s[c + 9], s[c + 10])};
+        for (int c = 0; c < BK; c += 16) {
+          float mx[2] = {max3(s[c], s[c + 1], s[c + 2]), max3(s[c + 8], s[c + 9], s[c + 10])};
 #pragma unroll
-        for (int e = 3; e < 7; e += 2) mx[0] = max3(mx[0], s[c + e], s[c + e + 1]), mx[1] = max3(mx[1], s[c + 8 + e], s[c + 9 + e]);
-        most = fmaxf(most, fmaf((float)(c / 16), rise, begin) + max3(fmaxf(mx[0], mx[1]), s[c + 7], s[c + 15]));
-      }
-    } else {
-      float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-      for (int c = 4; c < BK - 4; c += 8)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[BK - 4 + e]);
-      most = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
-      most *= F::CAP ? k.of(most * most) : a.scale_log2;
-    }
-    const bool passes = most > m + WEIGHT_TOP;
-    if (__any_sync(0xffffffffu, passes)) {
-      const float now = passes ? most - WEIGHT_SET : m, corr = fmaxf(ex2(m - now), 1.17549435e-38f);      // (never 0: infinities stay)
-      m = now;
-      l *= corr;
-      if (n > 0) {
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float o[32];
-          ld32(o_at + 32 * c, o);
-          wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= corr;
-          st32(o_at + 32 * c, reinterpret_cast<const uint32_t*>(o));
+          for (int e = 3; e < 7; e += 2) mx[0] = max3(mx[0], s[c + e], s[c + e + 1]), mx[1] = max3(mx[1], s[c + 8 + e], s[c + 9 + e]);
+          most = fmaxf(most, fmaf((float)(c / 16), rise, begin) + max3(fmaxf(mx[0], mx[1]), s[c + 7], s[c + 15]));
         }
-        wait_st();
+      } else {
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int c = 4; c < BK - 4; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[BK - 4 + e]);
+        most = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
+        most *= F::CAP ? k.of(most * most) : a.scale_log2;
+      }
+      const bool passes = most > m + WEIGHT_TOP;
+      if (__any_sync(0xffffffffu, passes)) {
+        const float now = passes ? most - WEIGHT_SET : m, corr = fmaxf(ex2(m - now), 1.17549435e-38f);      // (never 0: infinities stay)
+        m = now;
+        l *= corr;
+        if (n > 0) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float o[32];
+            ld32(o_at + 32 * c, o);
+            wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= corr;
+            st32(o_at + 32 * c, reinterpret_cast<const uint32_t*>(o));
+          }
+          wait_st();
+        }
       }
     }
     const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), m2 = pack2(-m, -m);
@@ -344,7 +347,7 @@ struct Row {
   // A raw score s becomes s of(s^2) in log2: a polynomial while all of a warp's are in its range, else that much of what they have become by 2^x.  (The coefficient of the
   // highest power is above 0 there too, so that a masked -inf stays one)
   struct Cap {
-    float x[5];
+    float x[5], top;                               // top: log2 of a magnitude that no score has passed
     __device__ __forceinline__ float of(float u) const { return fmaf(fmaf(fmaf(fmaf(x[4], u, x[3]), u, x[2]), u, x[1]), u, x[0]); }
     __device__ __forceinline__ uint64_t of(uint64_t u) const {
       uint64_t y = pack2(x[4], x[4]);
@@ -360,15 +363,23 @@ struct Row {
 #pragma unroll
       for (int e = 0; e < 4; ++e) big[e] = max3(big[e], fabsf(s[c + e]), fabsf(s[c + 4 + e]));
     Cap k;
-    if (__any_sync(0xffffffffu, max3(fmaxf(big[0], big[1]), big[2], big[3]) > a.cap_limit)) {
+    const float most = max3(fmaxf(big[0], big[1]), big[2], big[3]);
+    if (__any_sync(0xffffffffu, most > a.cap_limit)) {
 #pragma unroll
       for (int e = 0; e < BK; ++e) s[e] = tanh_by_exp(s[e] * a.cap_exp) * a.cap_out;
-      k = {{a.scale_log2, 0.f, 0.f, 0.f, 1e-44f}};
+      k = {{a.scale_log2, 0.f, 0.f, 0.f, 1e-44f}, a.cap_out * a.scale_log2};
     } else {
 #pragma unroll
       for (int i = 0; i < 5; ++i) k.x[i] = a.cap_k[i];
+      k.top = most * k.of(most * most);
     }
     return k;
+  }
+  // What no score of a tile passes, with its bias
+  __device__ __forceinline__ float highest(const Call&, const Cap& k, int p, int key0) const {
+    if (!F::BIAS) return k.top;
+    const float nearest = (float)max(p - key0 - (BK - 1), 0), farthest = (float)max(p - key0, key0 + BK - 1 - p);
+    return k.top - slope * (slope >= 0.f ? nearest : farthest);
   }
   // Scores become log2 of what they are with their bias, less what 16 of them share: an instruction for two of them, where whole biases would be two
   __device__ __forceinline__ void bias(const Call& a, float (&s)[BK], int p, int key0, const Cap& k, float& rise, float& begin) const {
