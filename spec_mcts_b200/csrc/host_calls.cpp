@@ -449,10 +449,10 @@ bool books_of(PyObject* const* args, int dev, Books& b) {
   return b.ld >= b.W;
 }
 // Books that are written in place must not overlap, nor `more` them
-bool apart(const Books& b, const at::Tensor* more = nullptr) {
+bool apart(const Books& b, const at::Tensor* more) {
   struct Span { const char *from, *to; };
   const auto span = [](const at::Tensor& t, int64_t n) { return Span{(const char*)t.data_ptr(), (const char*)t.data_ptr() + 4 * n}; };
-  const Span x[] = {span(b.table, (b.B - 1) * b.ld + b.W), span(b.lens, b.B), span(b.refs, b.n), more ? span(*more, more->numel()) : Span{}};
+  const Span x[] = {span(b.table, (b.B - 1) * b.ld + b.W), span(b.lens, b.B), span(b.refs, b.n), span(*more, more->numel())};
   for (int i = 0; i < 4; ++i)
     for (int j = 0; j < i; ++j)
       if (x[i].from < x[j].to && x[j].from < x[i].to) return false;
@@ -533,7 +533,7 @@ PyObject* page_fork(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int64_t ps;
   const at::Tensor* parents = tensor(args[3]);
   if (place < 0 || !books_of(args, dev, b) || !vector_of(parents, dev, at::kInt, b.B) || !whole(args[4], -1, ps) || ps < 1 || ps > MOST_PAGE) Py_RETURN_NONE;
-  if (place && !apart(b)) Py_RETURN_NONE;
+  if (place && !apart(b, parents)) Py_RETURN_NONE;
   const auto stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
   const at::Tensor from = *parents;
   at::Tensor table, lens, refs, ws;
@@ -566,7 +566,7 @@ PyObject* page_extend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (place < 0 || !books_of(args, dev, b) || b.B > 16384 || !vector_of(add, dev, at::kInt, b.B) || !whole(args[8], -1, ps) || ps < 1 || ps > MOST_PAGE ||
       !books_pools_of(args + 3, dev, b, ps, p))
     Py_RETURN_NONE;
-  if (place && !apart(b)) Py_RETURN_NONE;
+  if (place && !apart(b, add)) Py_RETURN_NONE;
   const auto stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
   const at::Tensor more = *add;
   at::Tensor table, lens, refs, ws;

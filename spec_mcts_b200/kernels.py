@@ -1019,8 +1019,8 @@ def _span(t: torch.Tensor):
     return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())) if t.numel() else 0)
 
 
-def _books(what: str, p, lens, refs, page_size: int, out, fresh):
-    """The books of a paged cache as the library reads them, and what it writes them to: `out`, or new tensors like `fresh`."""
+def _books(what: str, p, lens, refs, page_size: int, out, fresh, read=None):
+    """The books of a paged cache as the library reads them, and what it writes them to: `out`, or new tensors like `fresh`.  `read`: what else is read."""
     if p.dim() != 2 or p.dtype != torch.int32 or lens.shape != p.shape[:1] or lens.dtype != torch.int32 or refs.dim() != 1 or refs.dtype != torch.int32:
         raise Q40Error(f"{what}: int32 table [sequences, pages], lengths [sequences] and references [pages of the pool] expected, got {tuple(p.shape)} of {p.dtype}, "
                        f"{tuple(lens.shape)} of {lens.dtype} and {tuple(refs.shape)} of {refs.dtype}")
@@ -1039,11 +1039,11 @@ def _books(what: str, p, lens, refs, page_size: int, out, fresh):
         if t.shape != like.shape or t.dtype != torch.int32 or not t.is_contiguous() and (t.dim() == 1 or t.stride(1) != 1 or t.stride(0) < t.shape[1]):
             raise Q40Error(f"{what}: out like the books expected, got {tuple(t.shape)} of {t.dtype} with strides {t.stride()}")
     for i, t in enumerate(out):
-        for other in [*made, *out[:i]]:
+        for n, other in enumerate([*made, *out[:i], *([] if read is None else [read])]):
             (a, b), (c, d) = _span(t), _span(other)
-            same = other is replaces[i] and a == c and t.stride() == other.stride()
+            same = n < len(made) and other is replaces[i] and a == c and t.stride() == other.stride()
             if max(a, c) < min(b, d) and not same:
-                raise Q40Error(f"{what}: out overlaps the books, or itself, other than by being what it replaces")
+                raise Q40Error(f"{what}: out overlaps what is read, or itself, other than by being what it replaces")
     return p, lens, refs, list(out)
 
 
@@ -1087,7 +1087,7 @@ def page_fork(p, lens, refs, parents, *, page_size: int, out=None):
         if new is not None:
             return new
     dev = _need_cuda(p, lens, refs, parents, *(out or ()))
-    p, lens, refs, new = _books("page_fork", p, lens, refs, page_size, out, (p, lens, refs))
+    p, lens, refs, new = _books("page_fork", p, lens, refs, page_size, out, (p, lens, refs), parents)
     B, W = p.shape
     if parents.shape != (B,) or parents.is_floating_point():
         raise Q40Error(f"page_fork: {B} parents expected, got {tuple(parents.shape)} of {parents.dtype}")
@@ -1113,7 +1113,7 @@ def page_extend(p, lens, refs, kpool, vpool, add, *, page_size: int, k_scale=Non
             return new
     dev = _need_cuda(p, lens, refs, kpool, vpool, add, k_scale, v_scale, *(out or ()))
     k, v, ks, vs, kind = _books_pools("page_extend", kpool, vpool, k_scale, v_scale, refs, page_size)
-    p, lens, refs, new = _books("page_extend", p, lens, refs, page_size, out, (p, lens, refs))
+    p, lens, refs, new = _books("page_extend", p, lens, refs, page_size, out, (p, lens, refs), add)
     B, W = p.shape
     if add.shape != (B,) or add.is_floating_point() or B > 16384:
         raise Q40Error(f"page_extend: numbers of tokens for {B} sequences (at most 16384) expected, got {tuple(add.shape)} of {add.dtype}")

@@ -283,6 +283,10 @@ def test_refusals(K):
     flat = torch.zeros(40, dtype=torch.int32, device="cuda")
     with pytest.raises(K.Q40Error):                       # partly over what is read
         K.page_fork(flat[:12].view(3, 4), lens, refs, lens, page_size=16, out=(flat[4:16].view(3, 4), lens, refs))
+    with pytest.raises(K.Q40Error):                       # over the parents, or what is added
+        K.page_fork(p, lens, refs, lens, page_size=16, out=(p, lens, refs))
+    with pytest.raises(K.Q40Error):
+        K.page_extend(p, lens, refs, pool, pool, refs[2:5], page_size=16, out=(p, lens, refs))
     with pytest.raises(K.Q40Error):                       # over other books
         K.page_fork(p, lens, flat[:8], lens, page_size=16, out=(flat[4:16].view(3, 4), lens, where))
 
