@@ -229,8 +229,11 @@ __device__ __forceinline__ int before_in_cta(int x, int* sums, int& all) {
 }
 
 // ---- extension -----------------------------------------------------------------------------------------------------
-struct Extension : Books {
+// (what the kernels with less to tell get: with 216 bytes of arguments instead of 160 a launch takes 0.5 us longer)
+struct Additions : Books {
   const int32_t* add;
+};
+struct Extension : Additions {
   int *writers, *last;               // of each page: sequences that write to it behind its rows, and the last of them
   int4* plan;                        // of each sequence: entries that stay, entries in all, entries before, length
   Moves moves;
@@ -241,7 +244,7 @@ struct Growth {
   int n, m, n0, n1;                  // tokens and pages, before and after
   int tail, shared;                  // a page that is in part filled and will be written to (-1: none), and its references
   bool grows;                        // into pages that the table has room for
-  __device__ __forceinline__ Growth(const Extension& a, int b) {
+  __device__ __forceinline__ Growth(const Additions& a, int b) {
     n = a.length(b);
     const int add = a.add[b];
     const int64_t to = max((int64_t)n + add, (int64_t)0);
@@ -391,7 +394,7 @@ extend_plan_kernel(const Extension a) {
 // Few: every CTA plans for itself.  A thread has a sequence
 template <bool IN_PLACE>
 __global__ void __launch_bounds__(NT)
-extend_few_kernel(const Extension a, const Pools pools) {
+extend_few_kernel(const Additions a, const Pools pools) {
   extern __shared__ int4 few_smem[];
   int* const tails = reinterpret_cast<int*>(few_smem);       // [FEW_ROWS] pages that several list and this one writes to, or -1
   int* const first = tails + FEW_ROWS;           // [FEW_ROWS] rank of the first page that it gets
@@ -515,8 +518,10 @@ extend_few_kernel(const Extension a, const Pools pools) {
 }
 
 // ---- compaction ----------------------------------------------------------------------------------------------------
-struct Compaction : Books {
+struct Moving : Books {
   int32_t* where;                    // [pages] a page's new id, or -1 (free)
+};
+struct Compaction : Moving {
   int* old_refs;                     // of the pages that move
   Moves moves;
 };
@@ -588,7 +593,7 @@ compact_plan_kernel(const Compaction a) {
 // Few: every CTA plans for itself
 template <bool IN_PLACE>
 __global__ void __launch_bounds__(NT)
-compact_few_kernel(const Compaction a, const Pools pools) {
+compact_few_kernel(const Moving a, const Pools pools) {
   extern __shared__ int4 few_smem[];
   int* const used = reinterpret_cast<int*>(few_smem);        // [FEW_PAGES / 32] a bit for each page in use
   int* const counted = used + FEW_PAGES / 32;    // [FEW_PAGES / 32] pages in use in front of these 32
@@ -855,7 +860,7 @@ extern "C" int q40_page_extend(const int32_t* table, int64_t ld, const int32_t* 
     const auto kern = in_place ? extend_few_kernel<true> : extend_few_kernel<false>;
     cudaError_t e = q40_allow_smem(ready[in_place], (const void*)kern, EXTEND_FEW_SMEM);
     const size_t smem = (8 * FEW_ROWS + 2 * (size_t)((n_pages + 3) / 4 * 4)) * sizeof(int);
-    if (e == cudaSuccess) e = in_place ? launch_few<true>(kern, a, pools, ctas, smem, st) : launch_few<false>(kern, a, pools, ctas, smem, st);
+    if (e == cudaSuccess) e = in_place ? launch_few<true, Additions>(kern, a, pools, ctas, smem, st) : launch_few<false, Additions>(kern, a, pools, ctas, smem, st);
     return e == cudaSuccess ? Q40_OK : (int)e;
   }
   a.plan = (int4*)workspace;
@@ -900,7 +905,7 @@ extern "C" int q40_page_compact(const int32_t* table, int64_t ld, const int32_t*
     const auto kern = in_place ? compact_few_kernel<true> : compact_few_kernel<false>;
     cudaError_t e = q40_allow_smem(ready[in_place], (const void*)kern, COMPACT_FEW_SMEM);
     const size_t smem = (2 * FEW_PAGES / 32 + 2 * half) * sizeof(int);
-    if (e == cudaSuccess) e = in_place ? launch_few<true>(kern, a, pools, ctas, smem, st) : launch_few<false>(kern, a, pools, ctas, smem, st);
+    if (e == cudaSuccess) e = in_place ? launch_few<true, Moving>(kern, a, pools, ctas, smem, st) : launch_few<false, Moving>(kern, a, pools, ctas, smem, st);
     return e == cudaSuccess ? Q40_OK : (int)e;
   }
   int* const at = (int*)workspace;

@@ -390,3 +390,33 @@ def test_a_search_over_a_paged_cache(K, kind):
         used = int((where >= 0).sum())
         assert (refs[:used] > 0).all() and not refs[used:].any() and int(refs.sum()) == sum(hand.pages(x, ps) for x in books[1].tolist())
         assert torch.equal(read(), before)
+
+
+def test_streams_and_threads_beside_each_other(K):
+    """Each with books and prompts of its own."""
+    import threading
+
+    def work(seed, results):
+        torch.cuda.set_device(0)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            table, lens, refs = state(seed, 30, 60, 4, 24, 400)
+            g = torch.Generator(device="cuda").manual_seed(seed)
+            pool, pool2, q = normal(g, 2, 1600, D), normal(g, 2, 1600, D), normal(g, 600, 4, D)
+            torch.cuda.current_stream().synchronize()
+            for i in range(20):
+                books = K.page_fork(int32(table), int32(lens), int32(refs), int32([(b * 7 + i) % 30 for b in range(30)]), page_size=4)
+                books = K.page_extend(*books, pool, pool2, int32([b % 3 for b in range(30)]), page_size=4)
+                o = K.causal_attn(q, q[:, :2], q[:, 2:], documents=int32([0, 100 + i, 600]), softcap=20.0)
+                last = [x.clone() for x in (*books, *K.page_compact(*books, pool, pool2, page_size=4), pool, pool2, o)]
+            torch.cuda.current_stream().synchronize()
+            results.append(last)
+
+    alone, together = [[] for _ in range(4)], [[] for _ in range(4)]
+    for i, r in enumerate(alone):
+        work(i, r)
+    threads = [threading.Thread(target=work, args=(i, r)) for i, r in enumerate(together)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(x, y) for a, b in zip(alone, together) for x, y in zip(a[0], b[0]))
