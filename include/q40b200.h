@@ -343,7 +343,7 @@ int q40_page_fork(const int32_t* table, int64_t ld, const int32_t* lens, const i
  * and share a page which no other lists, the last keeps it): a copy of its rows so far, and its scales, in all `heads` of the pools [heads, P, 128] (P >= n_pages *
  * page_size, cache_type and scales as in q40_attn_pages; `heads` may be those of several layers).  Pages that are free before the call are handed out in ascending
  * order, to the sequences in theirs (a copy first).  A sequence whose pages do not fit in W, or whose last page is none of the pool's, stays as it is; so does the first that wants more pages than are left,
- * and every one behind it that wants any.  Workspace: *_workspace_bytes bytes (in_place: one of the outputs is an input; 0 bytes: may be NULL), 16-byte aligned, no
+ * and every one behind it that wants any, or that keeps a page of which others want a copy.  Workspace: *_workspace_bytes bytes (in_place: one of the outputs is an input; 0 bytes: may be NULL), 16-byte aligned, no
  * initialisation; calls that may overlap need one each. */
 size_t q40_page_extend_workspace_bytes(int B, int n_pages, int in_place);
 int q40_page_extend(const int32_t* table, int64_t ld, const int32_t* lens, const int32_t* refs, const int32_t* add, int32_t* table_out, int64_t ld_out,

@@ -270,7 +270,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(NT)
 extend_plan_kernel(const Extension a) {
   constexpr int COPIES = 1 << 31, GROWS = 1 << 30, WANTS = 1 << 29, PAGES = WANTS - 1;
   extern __shared__ int wanted[];                // [B + 1] pages that the sequences in front want, at most `pages` + 1
-  int* const info = wanted + a.B + 1;            // [B] PAGES: how many before; GROWS, WANTS any page, COPIES one
+  int* const info = wanted + a.B + 1;            // [B] PAGES: how many before; GROWS, WANTS any page or keeps one that others copy, COPIES one
   __shared__ int sums[WARPS], s_free;
   __shared__ long long s_sums[WARPS];
   cg::cluster_group cluster = cg::this_cluster();
@@ -320,13 +320,15 @@ extend_plan_kernel(const Extension a) {
     int need = 0;
     if (b < a.B) {
       const Growth g(a, b);
-      bool copies = false;
+      bool copies = false, keeps = false;
       if (g.grows) {
-        // of sequences that all write to a page which no other lists, the last keeps it
-        copies = g.tail >= 0 && g.shared > 1 && !(__ldcg(a.writers + g.tail) == g.shared && __ldcg(a.last + g.tail) == b);
+        // Of sequences that all write to a page which no other lists, the last keeps it.  One of the others that gets no copy lists it still: the last is refused with it
+        const bool shares = g.tail >= 0 && g.shared > 1;
+        keeps = shares && __ldcg(a.writers + g.tail) == g.shared && __ldcg(a.last + g.tail) == b;
+        copies = shares && !keeps;
         need = g.n1 - g.n0 + (copies ? 1 : 0);
       }
-      info[b] = g.n0 | (g.grows ? GROWS : 0) | (need ? WANTS : 0) | (copies ? COPIES : 0);
+      info[b] = g.n0 | (g.grows ? GROWS : 0) | (need || keeps ? WANTS : 0) | (copies ? COPIES : 0);
     }
     long long x = need;
 #pragma unroll
@@ -428,7 +430,7 @@ extend_few_kernel(const Additions a, const Pools pools) {
   int all_free;
   int rank = before_in_cta(free, sums, all_free);
   bool copies = shares;
-  if (shares) {                                  // of sequences that all write to a page which no other lists, the last keeps it
+  if (shares) {                                  // of sequences that all write to a page which no other lists, the last keeps it (see extend_plan_kernel)
     int writers = 0, last = 0;
     for (int b = 0; b < a.B; b += 4) {
       const int4 t = reinterpret_cast<const int4*>(tails)[b / 4];
@@ -450,7 +452,7 @@ extend_few_kernel(const Additions a, const Pools pools) {
     if (lane >= o) upto += y;
   }
   upto += before_in_cta(__shfl_sync(0xffffffffu, upto, 31), sums, wanted);
-  const bool granted = g.grows && (need == 0 || upto <= all_free);
+  const bool granted = g.grows && ((need == 0 && copies == shares) || upto <= all_free);
   const bool moves = granted && copies;
   const uint32_t moving = __ballot_sync(0xffffffffu, moves);
   const int front = before_in_cta(__popc(moving), sums, n_moves) + __popc(moving & ((1u << lane) - 1u));       // (each CTA has the same order)

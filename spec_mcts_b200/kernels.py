@@ -1106,7 +1106,7 @@ def page_extend(p, lens, refs, kpool, vpool, add, *, page_size: int, k_scale=Non
     0, its last tokens are taken back, and their pages given back.  A last page that has room, and that other sequences list, becomes a page of its own, with a copy of
     its rows in the pools [.., Hkv, P, 128] (of several layers at once, in front of the heads; scales [.., Hkv, P / page_size] of 8-bit ones alike), in place.  Free pages are
     handed out in ascending order; a sequence that its row of the table or the free pages have no room for keeps its length, and so does every one behind the latter that needs a
-    page.  Books and `out` as in page_fork; up to 16384 sequences (q40_page_extend in include/q40b200.h)."""
+    page, or that would go on in a shared one of which others need a copy.  Books and `out` as in page_fork; up to 16384 sequences (q40_page_extend in include/q40b200.h)."""
     if _host_calls is not None:
         new = _host_calls.page_extend(p, lens, refs, kpool, vpool, k_scale, v_scale, add, page_size, out)      # None: not a plain call
         if new is not None:
