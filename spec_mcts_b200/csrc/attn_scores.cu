@@ -38,38 +38,14 @@ template <bool WITH_CAP, bool WITH_BIAS>
 struct Scores {
   using Call = ScoreArgs;
   static constexpr bool CAP = WITH_CAP, BIAS = WITH_BIAS, SPANS = true;
-  struct Places { SpanTiles tiles; SpanSees sees[2]; };
+  using Places = SpanPlaces;
   static __device__ __forceinline__ bool keeps(const ScoreArgs& a) { return a.keep; }
 
-  // The span of a row, documents(k) being where document k begins
-  template <class D>
-  static __device__ __forceinline__ Span span_in(const ScoreArgs& a, int row, D documents) {
-    if (documents(0) > row) return {row, -2};
-    int k = 0, above = a.n_documents + 1;                // the last that begins at the row or in front of it
-    while (above - k > 1) {
-      const int mid = (k + above) >> 1;
-      if (documents(mid) <= row) k = mid;
-      else above = mid;
-    }
-    if (k == a.n_documents) return {row, row - 1};
-    const int start = max(documents(k), 0), end = min(documents(k + 1), a.S);
-    const int prefix = min(max(a.prefixes ? a.prefixes[k] : a.prefix, 0), end - start);
-    return {start, max(row, start + prefix - 1)};
-  }
-  static __device__ __forceinline__ Span span_of(const ScoreArgs& a, int row) {
-    const int p = a.offset + row;
-    return {0, max(p, a.prefix - 1)};
-  }
   // Every thread of the CTA calls it; a thread that has a row gets its span
   template <class B>
   static __device__ __forceinline__ Places places(const ScoreArgs& a, int row0, int split, Span& mine, B begin) {
-    const int n = min(2 * BQ, a.S - row0), p0 = a.offset + row0;
-    const int ends[4] = {0, min(BQ, n) - 1, BQ, n - 1};
+    const int n = min(2 * BQ, a.S - row0);
     Span at[4];
-    const auto places_of = [&]() -> Places {
-      return {SpanTiles(a, row0, 2 * BQ, split, at[0], at[3], BIAS),
-              {SpanSees(p0, at[0], p0 + ends[1], at[1], a.window, a.sinks), SpanSees(p0 + BQ, at[2], p0 + n - 1, at[3], a.window, a.sinks)}};
-    };
     if (a.documents) {
       // Where documents begin is read once by all threads, up to FEW of them; looked up in global memory, a handful took a microsecond
       constexpr int FEW = 256;
@@ -88,17 +64,17 @@ struct Scores {
         mine = few ? span_in(a, row, [&](int k) { return begins[k]; }) : span_in(a, row, [&](int k) { return a.documents[k]; });
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (r == ends[e]) edges[e] = mine;
+          if (r == edge_row(e, n)) edges[e] = mine;
       }
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < 4; ++e) at[e] = edges[e];
-      return places_of();
+      return SpanPlaces(a, row0, split, at, BIAS);
     } else {
       mine = span_of(a, row0 + min((int)threadIdx.x, n - 1));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) at[e] = span_of(a, row0 + min(ends[e], n - 1));
-      const Places there = places_of();
+      for (int e = 0; e < 4; ++e) at[e] = span_of(a, row0 + edge_row(e, n));
+      const Places there(a, row0, split, at, BIAS);
       begin();
       return there;
     }

@@ -30,6 +30,7 @@
 
 #include <algorithm>
 
+#include "attn_tiles.cuh"
 #include "attn_window.cuh"
 #include "q40_tc_common.cuh"
 #include "tanh_cap.cuh"
@@ -44,7 +45,7 @@ using ttc::mbar_expect_tx;
 using ttc::mbar_init;
 using ttc::mbar_wait;
 
-constexpr int BQ = 128, BK = 128, THREADS = 384;            // queries of a CTA's tile, keys of a tile
+constexpr int THREADS = 384;
 constexpr uint32_t TILE = BK * ATTN_D * 2;               // 32 KB: two blocks of 64 dims, rows of 128 bytes
 constexpr uint32_t HALF = TILE / 2;
 // log2 of a row's largest weight: where the maximum is set, and most.  fp16 holds 2^15
@@ -127,96 +128,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // The lowest n bits, of any n
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
-
-// Which tiles of keys (by number: keys BK t ..) a tile of queries sees some keys of, and all of them.  (Comparisons of numbers that are made once: the
-// thread that issues MMAs asks for every tile, and a few hundred cycles of it were a tenth of the time)
-struct Sees {
-  int last, from, sinks, all_last, all_from, all_sinks;
-  // queries at positions first .. end, none if end < first
-  __host__ __device__ __forceinline__ Sees(int first, int end, int window, int n_sinks) {
-    last = end >= first ? end / BK : -1;
-    from = first - window + 1 > 0 ? (first - window + 1) / BK : 0;
-    sinks = (n_sinks + BK - 1) / BK;
-    all_last = (first + 1) / BK - 1;
-    all_from = end - window + 1 > 0 ? (end - window + BK) / BK : 0;
-    all_sinks = n_sinks / BK;
-  }
-  __host__ __device__ __forceinline__ bool some(int t) const { return t <= last && (t >= from || t < sinks); }
-  __host__ __device__ __forceinline__ bool all(int t) const { return t <= all_last && (t >= all_from || t < all_sinks); }
-  __host__ __device__ __forceinline__ bool part(int t) const { return some(t) && !all(t); }
-};
-
-// The tiles of keys that a CTA goes through, tile(0) to tile(n - 1): those that one of its queries sees, or a split's share of them
-struct Tiles {
-  int p_first, p_last;               // positions of the CTA's first and last query
-  int t_first, t_from, j0, n;
-  // `rows` queries from row0 on
-  __host__ __device__ __forceinline__ Tiles(const Args& a, int row0, int rows, int split) {
-    p_first = a.offset + row0;
-    p_last = (p_first + rows < a.offset + a.S ? p_first + rows : a.offset + a.S) - 1;
-    const int from = p_first - a.window + 1 > 0 ? p_first - a.window + 1 : 0, first = a.sinks < from ? a.sinks : from;
-    t_first = (first + BK - 1) / BK;
-    t_from = from / BK > t_first ? from / BK : t_first;
-    const int all = t_first + p_last / BK + 1 - t_from;
-    j0 = (int)((int64_t)all * split / a.splits);
-    n = (int)((int64_t)all * (split + 1) / a.splits) - j0;
-  }
-  __device__ __forceinline__ int tile(int j) const { return j + j0 < t_first ? j + j0 : j + j0 - t_first + t_from; }
-  // `count` queries from the first-th on
-  __host__ __device__ __forceinline__ Sees sees(int first, int count, const Args& a) const {
-    const int end = p_first + first + count - 1;
-    return Sees(p_first + first, end < p_last ? end : p_last, a.window, a.sinks);
-  }
-};
-
-// A row of documents or of a prefix sees keys from `start` on, where its document begins, up to `last`: its own position, or the last of the prefix, which
-// is further on.  A row of no document: start is its position, and last one less, or -2 in front of the documents
-struct Span { int start, last; };
-
-// Sees and Tiles for these.  From row to row neither the first key of a window nor `last` falls, so that the first and the last row of a tile tell
-struct SpanSees {
-  int last, from, sink0, sinks, all_last, all_from, all_sink0, all_sinks;
-  // queries at positions p0 .. p1, none if p1 < p0
-  __device__ __forceinline__ SpanSees(int p0, Span s0, int p1, Span s1, int window, int n_sinks) {
-    const int lo0 = max(s0.start, p0 - window + 1), lo1 = max(s1.start, p1 - window + 1);
-    const bool same = s0.start == s1.start && s0.last >= p0 && s1.last >= p1;
-    last = p1 >= p0 ? max(s1.last, 0) / BK : -1;
-    from = lo0 / BK;
-    sink0 = s0.start / BK;
-    sinks = n_sinks > 0 ? (s0.start + n_sinks - 1) / BK + 1 : 0;
-    all_last = same ? (s0.last + 1) / BK - 1 : -1;
-    all_from = lo1 > 0 ? (lo1 - 1) / BK + 1 : 0;
-    all_sink0 = s0.start > 0 ? (s0.start - 1) / BK + 1 : 0;
-    all_sinks = (s0.start + n_sinks) / BK;
-  }
-  __device__ __forceinline__ bool some(int t) const { return t <= last && (t >= from || (t >= sink0 && t < sinks)); }
-  __device__ __forceinline__ bool all(int t) const { return t <= all_last && (t >= all_from || (t >= all_sink0 && t < all_sinks)); }
-  __device__ __forceinline__ bool part(int t) const { return some(t) && !all(t); }
-};
-
-struct SpanTiles {
-  int p_first, p_last;
-  int t_sink, t_first, t_from, j0, n;
-  bool backwards;                    // scores fall with distance: the largest come first, and no step that follows scales what is there
-  // `rows` queries from row0 on, the first and last of which have these spans
-  __device__ __forceinline__ SpanTiles(const Args& a, int row0, int rows, int split, Span s0, Span s1, bool from_the_end) {
-    backwards = from_the_end;
-    p_first = a.offset + row0;
-    p_last = min(p_first + rows, a.offset + a.S) - 1;
-    const int from = max(s0.start, p_first - a.window + 1), sink_end = min(s0.start + a.sinks, from);
-    t_sink = s0.start / BK;
-    t_first = sink_end > s0.start ? (sink_end - 1) / BK + 1 - t_sink : 0;
-    t_from = max(from / BK, t_sink + t_first);
-    const bool behind = s0.start == p_first && s0.last == p_first - 1;           // all documents: nothing is seen
-    const int all = behind || s1.last < 0 ? 0 : max(t_first + s1.last / BK + 1 - t_from, 0);
-    j0 = (int)((int64_t)all * split / a.splits);
-    n = (int)((int64_t)all * (split + 1) / a.splits) - j0;
-  }
-  __device__ __forceinline__ int tile(int j) const {
-    const int at = j0 + (backwards ? n - 1 - j : j);
-    return at < t_first ? t_sink + at : at - t_first + t_from;
-  }
-};
 
 // What a form of the kernel knows of its rows.  Here: position p sees what is up to it, less than `window` back or below `sinks`, and scores are as they are
 struct Plain {
@@ -675,7 +586,10 @@ attn_tc_kernel(const typename F::Call a, const __grid_constant__ Maps maps, int*
           for (int i = 0; i < 2; ++i) {
             if (failed) break;
             if ((i && F::SPANS ? due : pending[i]) && !product(i)) { failed = true; break; }
-            if (i == 1 && j > 0) ttc::commit(bar(EMPTY + v_slot));
+            if (i == 1 && j > 0) {
+              if (!values_there()) { failed = true; break; }       // (nobody's, where documents do not rise: their copy is waited for all the same)
+              ttc::commit(bar(EMPTY + v_slot));
+            }
             if (!(F::SPANS && scored[i]) && !scores(i)) failed = true;
           }
           if (failed) break;
@@ -692,6 +606,7 @@ attn_tc_kernel(const typename F::Call a, const __grid_constant__ Maps maps, int*
           if (!failed && pending[i] && !product(i)) failed = true;
           ttc::commit(bar(O_DONE + i));
         }
+        if (!failed && tiles.n > 0 && !values_there()) failed = true;
         ttc::commit(bar(ALL_DONE));
       }
       __syncwarp();
