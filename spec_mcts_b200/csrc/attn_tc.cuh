@@ -523,6 +523,8 @@ attn_tc_kernel(const typename F::Call a, const __grid_constant__ Maps maps, int*
     }
     if (!failed && mine.last >= 0) {
       if (!all_wait(bar(O_DONE + i), 0)) failed = true;
+      // write() puts rows where the queries are: who took no step waits for their copy, which nothing else here has waited for
+      if (F::SPANS && row.n == 0 && !all_wait(bar(Q_FULL + i), 0)) failed = true;
       fence_after();
       if (!failed) row.write(a, o_at, p, h, hk, tiles, sees, *s_taken_out, gbase + AT_Q + i * TILE + (warp & 3) * (TILE / 4), lane);
     }

@@ -27,3 +27,17 @@ def test_offsets_that_do_not_rise_end(K):
         K.causal_attn(q, k, v, documents=documents, prefix=[0, 1000][i % 2], window=[None, 150][i % 3 == 0], sinks=[0, 300][i % 5 == 0])
         assert K.tc_error_flag() == 0
     run(K, g, 700, 4, 2, documents=[300, 700])
+
+
+@pytest.mark.parametrize("documents", [[0, 1000], [1500, 2600], [3999, 4000], [0, 0], [2049, 2050, 2300]])
+def test_rows_of_none_are_zeros_in_many_blocks(K, documents):
+    """Each time: what comes into a block's memory for queries that see nothing must not come out."""
+    from test_gpu_pages import D, normal
+    g = generator(4)
+    q, k, v = normal(g, 4000, 32, D), normal(g, 4000, 8, D), normal(g, 4000, 8, D)
+    where = torch.tensor(documents, dtype=torch.int32, device="cuda")
+    wrong = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(200):
+        got = K.causal_attn(q, k, v, documents=where)
+        wrong += got[:documents[0]].count_nonzero() + got[documents[-1]:].count_nonzero()
+    assert wrong.item() == 0 and K.tc_error_flag() == 0
