@@ -25,6 +25,10 @@ extern "C" int block(const Call* a, int row0, int split, int backwards, int* til
   }
   return p.tiles.n;
 }
+extern "C" void span(const Call* a, int row, int* start, int* last) {
+  const Span at = span_at(*a, row);
+  *start = at.start, *last = at.last;
+}
 """
 
 
@@ -33,12 +37,22 @@ class Call(ctypes.Structure):
 
 
 @pytest.fixture(scope="module")
-def block(tmp_path_factory):
+def host(tmp_path_factory):
     where = tmp_path_factory.mktemp("span_tiles")
     source, lib = where / "span_tiles.cpp", where / "span_tiles.so"
     source.write_text(SOURCE)
     subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-Wall", "-Werror", "-shared", "-fPIC", "-I", CSRC, "-o", str(lib), str(source)], check=True)
-    return ctypes.CDLL(str(lib)).block
+    return ctypes.CDLL(str(lib))
+
+
+@pytest.fixture
+def block(host):
+    return host.block
+
+
+@pytest.fixture
+def span(host):
+    return host.span
 
 
 def mask(s, offset, window, sinks, documents, prefixes, prefix):
@@ -101,3 +115,21 @@ def test_of_every_kind(block, seed):
             documents[0], documents[-1] = min(documents[0], 0), max(documents[-1], s)
         prefixes = [r.choice([0, -3, log(s), s]) for _ in range(n)] if r.random() < 0.5 else None
         look(block, s, 0, window, sinks, documents, prefixes, r.choice([0, log(s)]) if prefixes is None else 0, splits)
+
+
+EXTREMES = [-(1 << 31), -(1 << 31) + 1, -1000, -1, 0, 1, 5, 100, 300, 511, 512, 700, 1 << 20, 1 << 30, (1 << 31) - 1]
+
+
+def test_entries_out_of_range_stay_in_range(span):
+    """Spans, tiles and rows that are looked into, whatever the entries are: all within the call's rows."""
+    r = random.Random(5)
+    for _ in range(4000):
+        s, n = r.choice([1, 130, 512]), r.choice([0, 1, 2, 3, 6])
+        documents, prefixes = [r.choice(EXTREMES) for _ in range(n + 1)], [r.choice(EXTREMES) for _ in range(n)]
+        int32 = lambda x: (ctypes.c_int32 * max(1, len(x)))(*x)
+        prefix = r.choice([0, s])
+        call = Call(s, 0, r.choice([1, s]), r.choice([0, s]), 1, n, prefix, int32(documents), int32(prefixes) if r.random() < 0.6 else None)
+        for row in range(0, s, r.randint(1, 40)):
+            start, last = ctypes.c_int(), ctypes.c_int()
+            span(ctypes.byref(call), row, ctypes.byref(start), ctypes.byref(last))
+            assert 0 <= start.value <= row and (last.value in (-2, row - 1) or row <= last.value < s), (documents, row, start.value, last.value)
