@@ -322,7 +322,7 @@ struct Row {
     const float inv = l != 0.f ? 1.f / l : 0.f;
     const bool no_document = F::SPANS && span.last < p, there = p <= tiles.p_last && !(no_document && F::keeps(a));
     // Where CTAs come in waves: all of a row at once, and rows by way of shared memory, sixteen lanes a row (4001 tokens in nine documents 76.3 -> 72.4 us; in one wave 77
-    // tokens take 6.9 this way, and 6.3 as below)
+    // tokens take 6.9 this way, and 6.3 as below).  The rows' place is that of the queries, whose copy has landed
     if (F::SPANS && gridDim.x > 148 && a.splits == 1 && a.wide_out && !taken_out) {
       float o[ATTN_D];
 #pragma unroll
@@ -523,7 +523,7 @@ attn_tc_kernel(const typename F::Call a, const __grid_constant__ Maps maps, int*
     }
     if (!failed && mine.last >= 0) {
       if (!all_wait(bar(O_DONE + i), 0)) failed = true;
-      // write() puts rows where the queries are: who took no step waits for their copy, which nothing else here has waited for
+      // (write() puts rows where the queries are: who took no step waits for their copy, which nothing else here has waited for)
       if (F::SPANS && row.n == 0 && !all_wait(bar(Q_FULL + i), 0)) failed = true;
       fence_after();
       if (!failed) row.write(a, o_at, p, h, hk, tiles, sees, *s_taken_out, gbase + AT_Q + i * TILE + (warp & 3) * (TILE / 4), lane);
@@ -588,10 +588,7 @@ attn_tc_kernel(const typename F::Call a, const __grid_constant__ Maps maps, int*
           for (int i = 0; i < 2; ++i) {
             if (failed) break;
             if ((i && F::SPANS ? due : pending[i]) && !product(i)) { failed = true; break; }
-            if (i == 1 && j > 0) {
-              if (!values_there()) { failed = true; break; }       // (nobody's, where documents do not rise: their copy is waited for all the same)
-              ttc::commit(bar(EMPTY + v_slot));
-            }
+            if (i == 1 && j > 0) ttc::commit(bar(EMPTY + v_slot));
             if (!(F::SPANS && scored[i]) && !scores(i)) failed = true;
           }
           if (failed) break;
@@ -608,7 +605,6 @@ attn_tc_kernel(const typename F::Call a, const __grid_constant__ Maps maps, int*
           if (!failed && pending[i] && !product(i)) failed = true;
           ttc::commit(bar(O_DONE + i));
         }
-        if (!failed && tiles.n > 0 && !values_there()) failed = true;
         ttc::commit(bar(ALL_DONE));
       }
       __syncwarp();

@@ -111,7 +111,8 @@ struct SpanTiles {
   int t_sink, t_first, t_from, j0, n;
   bool backwards;                    // scores fall with distance: the largest come first, and no step that follows scales what is there
   // Two tiles of queries from row0 on, the first and the last row of each of which have these spans.  Where the first tile lies in front of all documents, keys begin with what
-  // the second one's first row sees: there is no tile of keys that neither goes through
+  // the second one's first row sees.  So one of them goes through each tile of keys, also of documents that do not rise (a row's span ends with the row or behind it, the next
+  // one's begins with it or in front), and waits for its copies
   template <class A>
   Q40_HOST_DEVICE SpanTiles(const A& a, int row0, int split, const Span (&at)[4], bool from_the_end) {
     backwards = from_the_end;

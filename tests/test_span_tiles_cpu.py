@@ -133,3 +133,18 @@ def test_entries_out_of_range_stay_in_range(span):
             start, last = ctypes.c_int(), ctypes.c_int()
             span(ctypes.byref(call), row, ctypes.byref(start), ctypes.byref(last))
             assert 0 <= start.value <= row and (last.value in (-2, row - 1) or row <= last.value < s), (documents, row, start.value, last.value)
+
+
+def test_documents_that_do_not_rise(block):
+    """A tile of keys that a block goes through is gone through by one of its tiles of queries at least, whatever the entries are: who copies it is waited for."""
+    r, numbers = random.Random(6), lambda n: (ctypes.c_int * n)()
+    for _ in range(3000):
+        s, n = r.choice([1, 100, 129, 300, 1100]), r.choice([0, 1, 2, 3, 9])
+        documents = [r.choice([r.choice(EXTREMES), r.randint(-50, s + 50)]) for _ in range(n + 1)]
+        prefixes = [r.choice([r.choice(EXTREMES), r.randint(0, s)]) for _ in range(n)]
+        int32 = lambda x: (ctypes.c_int32 * max(1, len(x)))(*x)
+        call = Call(s, 0, r.choice([1, 50, s]), r.choice([0, 5, s]), 1, n, r.choice([0, s]), int32(documents), int32(prefixes) if r.random() < 0.6 else None)
+        for row0 in range(0, s, 256):
+            tiles, some, every = numbers(s // 128 + 2), numbers(2 * (s // 128 + 2)), numbers(2 * (s // 128 + 2))
+            got = block(ctypes.byref(call), row0, 0, r.choice([0, 1]), tiles, some, every)
+            assert 0 <= got <= s // 128 + 1 and all(0 <= tiles[j] <= (s - 1) // 128 and (some[2 * j] or some[2 * j + 1]) for j in range(got)), (documents, prefixes, row0)
