@@ -68,3 +68,19 @@ def test_many(K, b, most, ps, width, n_pages, left, in_place):
         got = extended(K, table, lens, refs, add, ps, pools, in_place)
         assert got[1].tolist() == new_lens and got[2].tolist() == new_refs and torch.equal(got[0], filled(rows, width))
     assert differ
+
+
+@pytest.mark.parametrize("kind", ["f16", "int8"])
+def test_prompts_that_there_is_no_room_for(K, kind):
+    """As documented: their tokens, several each, go nowhere, and not to the page 0 that their rows of zeros would name."""
+    g, ps, n, hkv, lens = generator(5), 16, 4, 2, [30, 40, 10, 20]         # two pages; none for the second, nor for those behind it
+    (kp, ks), (vp, vs) = pool_of(g, kind, hkv, n, ps), pool_of(g, kind, hkv, n, ps)
+    offsets = int32([0, 30, 70, 80, 100])
+    k, v = normal(g, 100, hkv, D), normal(g, 100, hkv, D)
+    table, start, refs = torch.zeros((4, 6), dtype=torch.int32, device="cuda"), int32([0] * 4), int32([0] * n)
+    table, now, refs = K.page_extend(table, start, refs, kp, vp, int32(lens), page_size=ps, k_scale=ks, v_scale=vs)
+    assert now.tolist() == [30, 0, 0, 0] and refs.tolist() == [1, 1, 0, 0]
+    one_k, one_v, scales = kp.clone(), vp.clone(), dict(k_scale=None if ks is None else ks.clone(), v_scale=None if vs is None else vs.clone())
+    K.page_append(table[:1], k[:30], v[:30], one_k, one_v, start[:1], page_size=ps, offsets=offsets[:2], **scales)
+    K.page_append(table, k, v, kp, vp, torch.where(now > start, start, -(1 << 30)), page_size=ps, offsets=offsets, k_scale=ks, v_scale=vs)
+    assert torch.equal(kp, one_k) and torch.equal(vp, one_v) and (ks is None or torch.equal(ks, scales["k_scale"]) and torch.equal(vs, scales["v_scale"]))
