@@ -14,8 +14,9 @@
 //   masks    what a row sees is an interval and the first keys of its document: words of bits, in tiles that some row does not see whole
 // Documents are looked up by each row; what a tile's first and last row see tells which tiles of keys it goes through.
 //
-// Us by the card: 16384 positions, window 4096, 64 heads on 8: 1650 with plain scores, 1780 with slopes, 1910 with a cap, 2310 with both; 4001 positions of 32 heads in nine
-// documents 71 (73 with slopes), where the bytes take 20 and the MMAs 25: 512 CTAs of some ten steps each, 3 us of start and 4 of end around 2 a step, with nothing
+// Us by the card: 16384 positions, window 4096, 64 heads on 8: 1650 with plain scores, 1780 to 1900 with slopes, 1900 with a cap of which no score is above 0.625, 2280 to 2360 with both;
+// 3970 and 3910 where scores reach the cap: three of the sixteen-a-cycle functions a score, 2420 for the visible ones alone.  4001 positions of 32 heads in nine
+// documents with slopes 66 to 71, where the bytes take 20 and the MMAs 25: 512 CTAs of some ten steps each, 3 us of start and 4 of end around 2 a step, with nothing
 // beside them on their SM.  One tile of queries a CTA and two CTAs an SM: 68 (75 with slopes), 2120 for the cap, 2290 for both: not taken, since others lose 5 %.
 #include "attn_tc.cuh"
 

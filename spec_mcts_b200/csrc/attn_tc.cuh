@@ -472,7 +472,7 @@ attn_tc_kernel(const typename F::Call a, const __grid_constant__ Maps maps, int*
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      // the queries and the first keys are on their way while the others meet
+      // the first queries are on their way while the others find out which keys they see
       asm volatile("griddepcontrol.wait;" ::: "memory");
       if (elect_one()) {
         copy(&maps.q, base + AT_Q, h, row0, bar(Q_FULL));

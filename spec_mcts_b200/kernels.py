@@ -1079,8 +1079,8 @@ def _books_pools(what: str, kpool, vpool, k_scale, v_scale, refs, page_size: int
 def page_fork(p, lens, refs, parents, *, page_size: int, out=None):
     """Sequences of a paged cache become continuations of others, whose pages they share: sequence b is from then on what sequence parents[b] was, and holds nothing if that is
     -1.  The cache's books are the table p [B, pages] of page ids and lengths lens [B], as page_append and page_flash_attn read them, and refs [pages of the pool], how many
-    sequences list each page (0: it is free); all int32.  Returns them as they are afterwards (zeros behind a sequence's pages), in new tensors or in
-    out = (p, lens, refs), which may be the books themselves.  page_extend gives sequences that share a page their own before they write to it
+    sequences list each page (0: it is free); all int32.  Returns them as they are afterwards (zeros behind a sequence's pages), in new tensors (which may share one piece
+    of memory: it is held while one of them is, and clone() gives one its own) or in out = (p, lens, refs), which may be the books themselves.  page_extend gives sequences that share a page their own before they write to it
     (q40_page_fork in include/q40b200.h)."""
     if _host_calls is not None:
         new = _host_calls.page_fork(p, lens, refs, parents, page_size, out)      # None: not a plain call
