@@ -1,4 +1,4 @@
-"""Which tiles of keys the blocks of prompt attention with documents and prefixes go through, compiled for the host, against the mask key by key."""
+"""Which tiles of keys the blocks of prompt attention go through, with documents and prefixes and without, compiled for the host, against the mask key by key."""
 import ctypes
 import os
 import random
@@ -24,6 +24,15 @@ extern "C" int block(const Call* a, int row0, int split, int backwards, int* til
     for (int i = 0; i < 2; ++i) some[2 * j + i] = p.sees[i].some(tiles[j]), all[2 * j + i] = p.sees[i].all(tiles[j]);
   }
   return p.tiles.n;
+}
+extern "C" int plain_block(const Call* a, int row0, int split, int, int* tiles, int* some, int* all) {
+  const Tiles t(*a, row0, 2 * BQ, split);
+  const Sees sees[2] = {t.sees(0, BQ, *a), t.sees(BQ, BQ, *a)};
+  for (int j = 0; j < t.n; ++j) {
+    tiles[j] = t.tile(j);
+    for (int i = 0; i < 2; ++i) some[2 * j + i] = sees[i].some(tiles[j]), all[2 * j + i] = sees[i].all(tiles[j]);
+  }
+  return t.n;
 }
 extern "C" void span(const Call* a, int row, int* start, int* last) {
   const Span at = span_at(*a, row);
@@ -86,7 +95,7 @@ def look(block, s, offset=0, window=1 << 29, sinks=0, documents=None, prefixes=N
                         for i in range(2):
                             part = seen[row0 + 128 * i:min(row0 + 128 * (i + 1), s), 128 * tiles[j]:128 * (tiles[j] + 1)]
                             assert some[2 * j + i] or not part.any()
-                            assert not every[2 * j + i] or (part.shape[1] == 128 and part.all())
+                            assert not (some[2 * j + i] and every[2 * j + i]) or (part.shape[1] == 128 and part.all())
                 assert len(set(listed)) == len(listed)
                 rows = seen[row0:row0 + 256]
                 assert {t for t in range((whole + 127) // 128) if rows[:, 128 * t:128 * (t + 1)].any()} <= set(listed)
@@ -148,3 +157,13 @@ def test_documents_that_do_not_rise(block):
             tiles, some, every = numbers(s // 128 + 2), numbers(2 * (s // 128 + 2)), numbers(2 * (s // 128 + 2))
             got = block(ctypes.byref(call), row0, 0, r.choice([0, 1]), tiles, some, every)
             assert 0 <= got <= s // 128 + 1 and all(0 <= tiles[j] <= (s - 1) // 128 and (some[2 * j] or some[2 * j + 1]) for j in range(got)), (documents, prefixes, row0)
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_windows(host, seed):
+    """The form without documents and prefixes."""
+    r = random.Random(seed)
+    log = lambda most: int(round(2 ** r.uniform(0, np.log2(most))))
+    for _ in range(25):
+        s = log(1500)
+        look(host.plain_block, s, r.choice([0, log(1500)]), r.choice([1 << 29, log(s), log(300)]), r.choice([0, log(300), log(8)]), splits=(1, r.randint(2, 6)))
