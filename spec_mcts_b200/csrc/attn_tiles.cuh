@@ -1,5 +1,6 @@
 // Which tiles of keys two tiles of queries of prompt attention go through, and what each of them sees of a tile (attn_tc.cuh): whole numbers alone, which a host compiles too.
 #pragma once
+#include <cstdint>
 
 #ifdef __CUDACC__
 #define Q40_HOST_DEVICE __host__ __device__ __forceinline__
